@@ -70,6 +70,11 @@ SIGNATURES = {
     "komp_stream_read": (_INT, [_P, _I64, _P, _P]),
     "komp_q4_0_decode": (_INT, [_P, _P, _I64, _P]),
     "komp_tq2_0_decode": (_INT, [_P, _P, _I64, _P]),
+    "komp_kv_write": (_INT, [_P, _P, _P, _INT, _P, _I64, _I64, _I64, _I64, _I64, _P]),
+    "komp_kv_read": (_INT, [_P, _P, _I64, _P, _P, _INT, _P]),
+    "komp_kv_attend": (_INT, [_P, _P, _P, _P, _INT, _P, _P, _P, _P, _P, *[_I64] * 11, ctypes.c_float, ctypes.c_float, _I64,
+                              _P, _I64, _P]),
+    "komp_kv_attend_workspace": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _I64, _P]),
     "komp_timing_begin": (_INT, [_I64]),
     "komp_timing_end": (_INT, [_P, _P]),
     "komp_stamps_begin": (_INT, [_P, _I64]),
@@ -78,6 +83,13 @@ SIGNATURES = {
     "komp_clock_khz": (_INT, [_P]),
 }
 ABI_VERSION = 1
+
+class KvCacheStruct(ctypes.Structure):
+    """komp_kv_cache of include/komp_abi.h."""
+
+    _fields_ = [("KQ", _P), ("KS", _P), ("VQ", _P), ("VS", _P), ("pages", _I64), ("heads", _INT), ("head_dim", _INT),
+                ("page", _INT), ("k_fmt", _INT), ("v_fmt", _INT)]  # fmt: skip
+
 
 _lib = None
 

@@ -11,6 +11,7 @@
 
 #include "../../include/komp_abi.h"
 #include "komp_internal.h"
+#include "kv_layout.h"
 
 namespace komp {
 namespace {
@@ -1161,6 +1162,193 @@ int komp_stamps_end(int64_t* words_used, int* clock_khz) {
     if (e != hipSuccess) return hip_status(e, "komp_stamps_end");
   }
   return KOMP_OK;
+}
+
+}  // extern "C"
+
+// ---- quantized key/value cache --------------------------------------------------------------------------------------
+namespace komp {
+namespace {
+
+int kv_cache_of(const char* name, const komp_kv_cache* C, KvCache& c) {
+  if (C == nullptr) return fail(KOMP_EINVAL, "%s: no cache", name);
+  if (C->head_dim != 64 && C->head_dim != 96 && C->head_dim != 128 && C->head_dim != 256)
+    return fail(KOMP_EINVAL, "%s: head_dim=%d (64, 96, 128 or 256)", name, C->head_dim);
+  if (C->page < 32 || C->page > 65536 || (C->page & (C->page - 1)) != 0)
+    return fail(KOMP_EINVAL, "%s: page=%d must be a power of two from 32 to 65536", name, C->page);
+  if (C->heads < 1 || C->heads > 65535) return fail(KOMP_EINVAL, "%s: heads=%d (1 to 65535)", name, C->heads);
+  if (C->pages < 0 || C->pages > INT64_C(0x7FFFFFFF))
+    return fail(KOMP_EINVAL, "%s: pages=%lld (0 to 2^31 - 1)", name, static_cast<long long>(C->pages));
+  const bool formats = (C->k_fmt == FMT_Q4_0 || C->k_fmt == FMT_Q8_0) && (C->v_fmt == FMT_Q4_0 || C->v_fmt == FMT_Q8_0) &&
+                       !(C->k_fmt == FMT_Q4_0 && C->v_fmt == FMT_Q8_0);
+  if (!formats)
+    return fail(KOMP_EINVAL, "%s: formats %d, %d (keys and values q4_0, keys q8_0 and values q4_0, or both q8_0)", name,
+                C->k_fmt, C->v_fmt);
+  if (C->pages > 0 && (C->KQ == nullptr || C->KS == nullptr || C->VQ == nullptr || C->VS == nullptr))
+    return fail(KOMP_EINVAL, "%s: a plane of the cache is NULL", name);
+  if (!aligned(C->KQ, 16) || !aligned(C->KS, 16) || !aligned(C->VQ, 16) || !aligned(C->VS, 16))
+    return fail(KOMP_EINVAL, "%s: the cache's planes must be 16-byte aligned", name);
+  c.kq = C->KQ;
+  c.ks = reinterpret_cast<uint16_t*>(C->KS);
+  c.vq = C->VQ;
+  c.vs = reinterpret_cast<uint16_t*>(C->VS);
+  c.pages = C->pages;
+  c.heads = C->heads;
+  c.dim = C->head_dim;
+  c.page = C->page;
+  c.page_log2 = __builtin_ctz(static_cast<unsigned>(C->page));
+  c.kf = C->k_fmt;
+  c.vf = C->v_fmt;
+  return KOMP_OK;
+}
+
+int kv_type_of(const char* name, int type, int& size) {
+  if (type < KV_F32 || type > KV_BF16) return fail(KOMP_EINVAL, "%s: type=%d (0 f32, 1 f16, 2 bf16)", name, type);
+  size = type == KV_F32 ? 4 : 2;
+  return KOMP_OK;
+}
+
+// tokens of one call: 32-bit workgroup numbers (256 lanes of 4 values)
+int kv_tokens(const char* name, const KvCache& c, int64_t T) {
+  if (T < 0 || T > (INT64_C(1) << 38) / (static_cast<int64_t>(c.heads) * c.dim / 4))
+    return fail(KOMP_EINVAL, "%s: T=%lld tokens", name, static_cast<long long>(T));
+  return KOMP_OK;
+}
+
+int kv_attend_call(const char* name, const komp_kv_cache* C, int type, int64_t T, int64_t batch, int64_t heads,
+                   int64_t max_queries, int64_t max_length, KvAttendCall& c, int& size) {
+  int st = kv_cache_of(name, C, c.cache);
+  if (st == KOMP_OK) st = kv_type_of(name, type, size);
+  if (st != KOMP_OK) return st;
+  if (batch < 0 || batch > 65535) return fail(KOMP_EINVAL, "%s: batch=%lld (0 to 65535)", name, static_cast<long long>(batch));
+  if (heads < 1 || heads > INT64_C(1) << 20 || heads % c.cache.heads != 0)
+    return fail(KOMP_EINVAL, "%s: heads=%lld must be a multiple of the cache's %d", name, static_cast<long long>(heads),
+                c.cache.heads);
+  const int64_t most = INT64_C(0x3FFFFFFF) / heads;
+  if (T < 0 || T > most) return fail(KOMP_EINVAL, "%s: T=%lld rows (0 to %lld)", name, static_cast<long long>(T), static_cast<long long>(most));
+  if (max_queries < 0 || max_queries > T)
+    return fail(KOMP_EINVAL, "%s: max_queries=%lld (0 to T=%lld)", name, static_cast<long long>(max_queries), static_cast<long long>(T));
+  if (max_length < 0 || max_length > INT64_C(0x7FFFFFFF) - 65536)
+    return fail(KOMP_EINVAL, "%s: max_length=%lld", name, static_cast<long long>(max_length));
+  c.type = type;
+  c.rows = T;
+  c.batch = static_cast<int>(batch);
+  c.heads = static_cast<int>(heads);
+  c.max_queries = max_queries;
+  c.max_length = max_length;
+  return KOMP_OK;
+}
+
+}  // namespace
+}  // namespace komp
+
+extern "C" {
+
+int komp_kv_write(const komp_kv_cache* C, const void* K, const void* V, int type, const int64_t* SLOTS, int64_t T,
+                  int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, void* stream) {
+  const char* name = "komp_kv_write";
+  KvWriteCall w;
+  int size = 0;
+  int st = kv_cache_of(name, C, w.cache);
+  if (st == KOMP_OK) st = kv_type_of(name, type, size);
+  if (st == KOMP_OK) st = kv_tokens(name, w.cache, T);
+  if (st != KOMP_OK) return st;
+  if (T == 0) return KOMP_OK;
+  if (K == nullptr || V == nullptr || SLOTS == nullptr) return fail(KOMP_EINVAL, "%s: K, V or SLOTS is NULL", name);
+  if (!aligned(K, size) || !aligned(V, size) || !aligned(SLOTS, 8))
+    return fail(KOMP_EINVAL, "%s: K, V and SLOTS must be aligned to their elements", name);
+  w.k = K;
+  w.v = V;
+  w.type = type;
+  w.slots = SLOTS;
+  w.tokens = T;
+  w.stride_t[0] = k_stride_t;
+  w.stride_h[0] = k_stride_h;
+  w.stride_t[1] = v_stride_t;
+  w.stride_h[1] = v_stride_h;
+  return hip_status(launch_kv_write(w, static_cast<hipStream_t>(stream)), name);
+}
+
+int komp_kv_read(const komp_kv_cache* C, const int64_t* SLOTS, int64_t T, void* K, void* V, int type, void* stream) {
+  const char* name = "komp_kv_read";
+  KvReadCall r;
+  int size = 0;
+  int st = kv_cache_of(name, C, r.cache);
+  if (st == KOMP_OK) st = kv_type_of(name, type, size);
+  if (st == KOMP_OK) st = kv_tokens(name, r.cache, T);
+  if (st != KOMP_OK) return st;
+  if (T == 0) return KOMP_OK;
+  if (K == nullptr || V == nullptr || SLOTS == nullptr) return fail(KOMP_EINVAL, "%s: K, V or SLOTS is NULL", name);
+  if (!aligned(K, 16) || !aligned(V, 16) || !aligned(SLOTS, 8))
+    return fail(KOMP_EINVAL, "%s: K and V must be 16-byte aligned, SLOTS 8-byte", name);
+  r.slots = SLOTS;
+  r.tokens = T;
+  r.k = K;
+  r.v = V;
+  r.type = type;
+  return hip_status(launch_kv_read(r, static_cast<hipStream_t>(stream)), name);
+}
+
+int komp_kv_attend_workspace(const komp_kv_cache* C, int type, int64_t T, int64_t batch, int64_t heads,
+                             int64_t max_queries, int64_t max_length, int64_t* bytes) {
+  const char* name = "komp_kv_attend_workspace";
+  KvAttendCall c;
+  int size = 0;
+  const int st = kv_attend_call(name, C, type, T, batch, heads, max_queries, max_length, c, size);
+  if (st != KOMP_OK) return st;
+  if (bytes == nullptr) return fail(KOMP_EINVAL, "%s: bytes is NULL", name);
+  *bytes = kv_attend_work_bytes(c);
+  return KOMP_OK;
+}
+
+int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE, int type, const int32_t* TABLES,
+                   const int32_t* LENGTHS, const int32_t* STARTS, const int32_t* PREFIX, const float* SLOPES, int64_t T,
+                   int64_t batch, int64_t heads, int64_t q_stride_t, int64_t q_stride_h, int64_t out_stride_t,
+                   int64_t out_stride_h, int64_t table_stride, int64_t table_cols, int64_t max_queries,
+                   int64_t max_length, float scale, float softcap, int64_t window, void* WORK, int64_t work_bytes,
+                   void* stream) {
+  const char* name = "komp_kv_attend";
+  KvAttendCall c;
+  int size = 0;
+  const int st = kv_attend_call(name, C, type, T, batch, heads, max_queries, max_length, c, size);
+  if (st != KOMP_OK) return st;
+  if (STARTS == nullptr && T != batch)
+    return fail(KOMP_EINVAL, "%s: T=%lld rows for batch=%lld without STARTS (one row a sequence)", name,
+                static_cast<long long>(T), static_cast<long long>(batch));
+  if (!(softcap >= 0.f) || softcap > 3.0e38f) return fail(KOMP_EINVAL, "%s: softcap=%g", name, static_cast<double>(softcap));
+  if (window < 0 || window > INT64_C(0x3FFFFFFF)) return fail(KOMP_EINVAL, "%s: window=%lld", name, static_cast<long long>(window));
+  if (table_cols < 0 || table_cols > (INT64_C(0x7FFFFFFF) - 65536) / c.cache.page)
+    return fail(KOMP_EINVAL, "%s: table_cols=%lld", name, static_cast<long long>(table_cols));
+  if (T == 0 || batch == 0 || max_queries == 0) return KOMP_OK;
+  if (Q == nullptr || OUT == nullptr || LENGTHS == nullptr || (TABLES == nullptr && table_cols > 0))
+    return fail(KOMP_EINVAL, "%s: Q, OUT, TABLES or LENGTHS is NULL", name);
+  if (!aligned(Q, size) || !aligned(OUT, size) || !aligned(LSE, 4) || !aligned(TABLES, 4) || !aligned(LENGTHS, 4) ||
+      !aligned(STARTS, 4) || !aligned(PREFIX, 4) || !aligned(SLOPES, 4))
+    return fail(KOMP_EINVAL, "%s: a pointer is not aligned to its elements", name);
+  const int64_t need = kv_attend_work_bytes(c);
+  if (need > 0 && (WORK == nullptr || work_bytes < need || !aligned(WORK, 16)))
+    return fail(KOMP_EINVAL, "%s: WORK must hold %lld bytes (komp_kv_attend_workspace), 16-byte aligned", name,
+                static_cast<long long>(need));
+  c.q = Q;
+  c.out = OUT;
+  c.lse = LSE;
+  c.tables = TABLES;
+  c.lengths = LENGTHS;
+  c.starts = STARTS;
+  c.prefix = PREFIX;
+  c.slopes = SLOPES;
+  c.q_stride_t = q_stride_t;
+  c.q_stride_h = q_stride_h;
+  c.out_stride_t = out_stride_t;
+  c.out_stride_h = out_stride_h;
+  c.table_stride = table_stride;
+  c.table_cols = static_cast<int>(table_cols);
+  c.scale = scale;
+  c.softcap = softcap;
+  c.window = static_cast<int>(window);
+  c.work = WORK;
+  c.work_bytes = work_bytes;
+  return hip_status(launch_kv_attend(c, static_cast<hipStream_t>(stream)), name);
 }
 
 }  // extern "C"

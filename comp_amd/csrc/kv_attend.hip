@@ -1,0 +1,146 @@
+// The plan of an attention call over the quantized key/value cache, and the join of a sequence's splits.
+#include <algorithm>
+
+#include "kv_attend.h"
+
+namespace komp {
+namespace {
+
+constexpr int kMaxSplits = 64;
+
+AttendPlan plan_of(const KvAttendCall& c) {
+  const int group = c.heads / c.cache.heads;
+  const int64_t cols = c.max_queries * group;
+  const int64_t units = static_cast<int64_t>(c.batch) * c.cache.heads;
+  const int most = c.type != KV_F32 && c.cache.dim <= 128 ? 4 : 2;
+  AttendPlan p;
+  p.ct = cols <= 16 ? 1 : cols <= 32 || most == 2 ? 2 : most;
+  p.wide = false;
+  p.splits = 1;
+  const int64_t wide_groups = (cols + 16 * most * kAttendWaves - 1) / (16 * most * kAttendWaves);
+  if (cols > 16 * most && units * wide_groups >= 256) {
+    p.ct = most;
+    p.wide = true;
+    p.groups = static_cast<int>(wide_groups);
+    return p;
+  }
+  p.groups = static_cast<int>((cols + 16 * p.ct - 1) / (16 * p.ct));
+  const int64_t tiles = (c.max_length + 31) / 32;
+  const int64_t want = 1024 / (units * p.groups), most_splits = tiles / (2 * kAttendWaves);
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most_splits, kMaxSplits})));
+  return p;
+}
+
+// One wave a row and head: the splits' sums, brought to the largest of their references.  D / 4 lanes hold a split's
+// channels, 64 / (D / 4) splits at a time.
+template <int D>
+__global__ void __launch_bounds__(256) kv_attend_join_kernel(const AttendArgs a) {
+  constexpr int LANES = D / 4, PAR = 64 / LANES;
+  const int lane = threadIdx.x & 63;
+  const int64_t n = a.rows * a.heads, at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (at >= n) return;
+  float2 m = float2{-__builtin_inff(), 0.f};
+  if (lane < a.splits) m = a.part_m[lane * n + at];
+  float top = m.x;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float f = m.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m.x - top);
+  const float l = group_sum(f * m.y, 64);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const int part = lane / LANES, ch = lane - part * LANES;
+  for (int s0 = 0; s0 < a.splits; s0 += PAR) {
+    const int s = s0 + part;
+    const float fs = __shfl(f, s < a.splits ? s : 0, 64);
+    const float ms = __shfl(m.x, s < a.splits ? s : 0, 64);
+    if (part < PAR && s < a.splits && ms != -__builtin_inff())
+      o += fs * *reinterpret_cast<const f32x4*>(a.part_o + (s * n + at) * D + ch * 4);
+  }
+#pragma unroll
+  for (int p = 1; p < PAR; ++p) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float other = __shfl(o[e], (p * LANES + ch) & 63, 64);
+      if (part == 0) o[e] += other;
+    }
+  }
+  if (part == 0) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t row = at / a.heads;
+    const int head = static_cast<int>(at - row * a.heads);
+    store_out(a.out, a.type, a.wide_out, row * a.out_stride_t + head * a.out_stride_h + ch * 4, o * inv);
+    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -__builtin_inff() : (top + __log2f(l)) * (1.f / kLog2e);
+  }
+}
+
+int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+
+}  // namespace
+
+int64_t kv_attend_work_bytes(const KvAttendCall& c) {
+  if (c.batch == 0 || c.rows == 0) return 0;
+  const AttendPlan p = plan_of(c);
+  if (p.splits == 1) return 0;
+  const int64_t n = p.splits * c.rows * c.heads;
+  return round256(n * c.cache.dim * 4) + n * 8;
+}
+
+hipError_t launch_kv_attend(const KvAttendCall& c, hipStream_t stream) {
+  const AttendPlan p = plan_of(c);
+  AttendArgs a;
+  a.c = c.cache;
+  a.q = c.q;
+  a.q_stride_t = c.q_stride_t;
+  a.q_stride_h = c.q_stride_h;
+  a.out = c.out;
+  a.out_stride_t = c.out_stride_t;
+  a.out_stride_h = c.out_stride_h;
+  a.lse = c.lse;
+  a.tables = c.tables;
+  a.table_stride = c.table_stride;
+  a.table_cols = c.table_cols;
+  a.lengths = c.lengths;
+  a.starts = c.starts;
+  a.prefix = c.prefix;
+  a.slopes = c.slopes;
+  a.rows = c.rows;
+  a.heads = c.heads;
+  a.group = c.heads / c.cache.heads;
+  a.type = c.type;
+  a.window = c.window;
+  a.scale = c.scale * kLog2e;
+  a.cap = c.softcap;
+  const int size = c.type == KV_F32 ? 4 : 2;
+  auto fits = [&](const void* p, int64_t st, int64_t sh, int bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && st * size % bytes == 0 && sh * size % bytes == 0;
+  };
+  a.wide_q = fits(c.q, c.q_stride_t, c.q_stride_h, 16);
+  a.wide_out = fits(c.out, c.out_stride_t, c.out_stride_h, 4 * size);
+  a.splits = p.splits;
+  a.groups = p.groups;
+  a.part_o = static_cast<float*>(c.work);
+  const int64_t n = p.splits * c.rows * c.heads;
+  a.part_m = reinterpret_cast<float2*>(static_cast<char*>(c.work) + round256(n * c.cache.dim * 4));
+  hipError_t e;
+  if (c.cache.kf == KV_Q4_0) e = launch_attend_q4_q4(a, p, c.batch, stream);
+  else if (c.cache.vf == KV_Q4_0) e = launch_attend_q8_q4(a, p, c.batch, stream);
+  else e = launch_attend_q8_q8(a, p, c.batch, stream);
+  if (e != hipSuccess || p.splits == 1) return e;
+  const dim3 grid(static_cast<unsigned>((c.rows * c.heads + 3) / 4));
+  auto run = [&](auto kern) {
+    const Timing tm = timing_slot(KIND_PROBE);
+    if (tm.on) {
+      hipExtLaunchKernelGGL(kern, grid, dim3(256), 0, stream, tm.start, tm.stop, 0, a);
+    } else {
+      hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, a);
+    }
+    return hipGetLastError();
+  };
+  switch (c.cache.dim) {
+    case 64: return run(kv_attend_join_kernel<64>);
+    case 96: return run(kv_attend_join_kernel<96>);
+    case 128: return run(kv_attend_join_kernel<128>);
+    default: return run(kv_attend_join_kernel<256>);
+  }
+}
+
+}  // namespace komp

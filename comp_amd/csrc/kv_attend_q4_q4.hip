@@ -1,0 +1,10 @@
+// Attention over a cache of Q4_0 keys and Q4_0 values (kv_attend.h).
+#include "kv_attend.h"
+
+namespace komp {
+
+hipError_t launch_attend_q4_q4(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream) {
+  return launch_attend_format<KV_Q4_0, KV_Q4_0>(a, plan, batch, stream);
+}
+
+}  // namespace komp

@@ -239,12 +239,64 @@ int komp_q4_0_decode(const uint8_t* WQ, int32_t* OUT, int64_t R, void* stream);
 /* [NBLK][64] TQ2_0 quant bytes -> [NBLK][256] int32 values.  Replaces: kernels.tq2_0_decode (src/komp/kernels.py:160-170). */
 int komp_tq2_0_decode(const uint8_t* WQ, int32_t* OUT, int64_t nblk, void* stream);
 
+/* Quantized key/value cache: keys and values as ggml Q4_0 or Q8_0 blocks of 32 along the head, in pages of `page` tokens,
+ * for the attention of a decode step or a prompt beside the GEMVs and GEMMs above.  No reference counterpart.
+ *   KQ u8 [pages][heads][page * head_dim * (Q4_0 1/2, Q8_0 1)], KS i16 [pages][heads][page * head_dim / 32] (f16 bits), VQ
+ *   and VS alike, each 16-byte aligned; the order of the bytes inside a page and head is the library's own (tiles in the
+ *   matrix instruction's order), so a cache is written and read through these entries.
+ *   head_dim 64, 96, 128 or 256; page a power of two from 32 to 65536; k_fmt and v_fmt 0 (q4_0) or 2 (q8_0), not q4_0
+ *   keys with q8_0 values.  A token's slot is page index * page + its place in the page.
+ * type: 0 f32, 1 f16, 2 bf16 (K, V, Q, OUT).  Strides count elements; the head_dim elements of a row are contiguous. */
+typedef struct komp_kv_cache {
+  uint8_t* KQ;
+  int16_t* KS;
+  uint8_t* VQ;
+  int16_t* VS;
+  int64_t pages;
+  int heads;
+  int head_dim;
+  int page;
+  int k_fmt;
+  int v_fmt;
+} komp_kv_cache;
+
+/* Quantize K, V [T][heads][head_dim] into the T slots of SLOTS.  Codes and scales are ggml's (Q8_0 as komp_quant_q8_0, Q4_0
+ * as ggml's quantize_row_q4_0_ref); a block that holds a NaN reads back as NaN.  A slot below 0 or past the cache leaves
+ * its token out; of equal slots in one call, either token's bytes may stay, also in part. */
+int komp_kv_write(const komp_kv_cache* C, const void* K, const void* V, int type, const int64_t* SLOTS, int64_t T,
+                  int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, void* stream);
+
+/* The values of T slots, K and V [T][heads][head_dim] contiguous and 16-byte aligned: f32(code) * f32(scale), rounded once
+ * to `type`.  A slot below 0 or past the cache gives zeros. */
+int komp_kv_read(const komp_kv_cache* C, const int64_t* SLOTS, int64_t T, void* K, void* V, int type, void* stream);
+
+/* Attention of T query rows over the cache.  Sequence s (of `batch`) has LENGTHS[s] keys, key j in page TABLES[s][j / page]
+ * (row stride table_stride), and the query rows STARTS[s] .. STARTS[s + 1] - 1 of Q [T][heads][head_dim] (STARTS NULL: row
+ * s); its n rows are its last n positions, the new tokens' own keys being in the cache already.  `heads` is a multiple
+ * of the cache's: each kv head serves heads / C->heads consecutive query heads.  For a row at position i
+ *   score_j = scale * q . k_j;  softcap > 0: softcap * tanh(score / softcap);  SLOPES f32 [heads]: - slope * |i - j|
+ *   visible: j < LENGTHS[s], j <= i or j < PREFIX[s] (NULL: 0), and with window > 0 also i - j < window
+ *   OUT [T][heads][head_dim] = softmax over the visible keys times their values, 0 where none is visible
+ *   LSE f32 [T][heads] (or NULL) = the natural logarithm of the sum of exp(score), -inf where none is visible
+ * A page number that the cache does not have hides its keys; lengths past table_cols pages end there.  max_queries: at
+ * least the most rows a sequence has (at most T); max_length: the longest length, for the plan alone (any value is right).
+ * WORK: komp_kv_attend_workspace bytes for the same arguments (0: may be NULL), 16-byte aligned, free again when the call
+ * has run.  Rows of Q that no sequence holds get unspecified results. */
+int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE, int type, const int32_t* TABLES,
+                   const int32_t* LENGTHS, const int32_t* STARTS, const int32_t* PREFIX, const float* SLOPES, int64_t T,
+                   int64_t batch, int64_t heads, int64_t q_stride_t, int64_t q_stride_h, int64_t out_stride_t,
+                   int64_t out_stride_h, int64_t table_stride, int64_t table_cols, int64_t max_queries,
+                   int64_t max_length, float scale, float softcap, int64_t window, void* WORK, int64_t work_bytes,
+                   void* stream);
+int komp_kv_attend_workspace(const komp_kv_cache* C, int type, int64_t T, int64_t batch, int64_t heads,
+                             int64_t max_queries, int64_t max_length, int64_t* bytes);
+
 /* Dispatch timing for the tuning harness (no reference counterpart; the reference was never timed).
  * Between komp_timing_begin() and komp_timing_end(), every launch made by this library on the calling process is
  * issued with hipExtLaunchKernel start/stop events, which the runtime stamps with the dispatch's own begin and end.
  * komp_timing_end() waits for those events and returns, per kernel kind, the summed dispatch time in milliseconds and
- * the dispatch count.  Kinds: 0 quant_q8_0, 1 quant_q8_K, 2 q4_0 GEMV / GEMM, 3 tq2_0 GEMV / GEMM, 4 probes and
- * weight splits, 5 q8_0 GEMV / GEMM, 6 iq4_nl GEMV / GEMM, 7 q4_k GEMV (arrays of length 8).
+ * the dispatch count.  Kinds: 0 quant_q8_0, 1 quant_q8_K, 2 q4_0 GEMV / GEMM, 3 tq2_0 GEMV / GEMM, 4 probes,
+ * weight splits and the key/value cache's operators, 5 q8_0 GEMV / GEMM, 6 iq4_nl GEMV / GEMM, 7 q4_k GEMV (arrays of length 8).
  * max_dispatches bounds the events created. */
 #define KOMP_TIMING_KINDS 8
 int komp_timing_begin(int64_t max_dispatches);
