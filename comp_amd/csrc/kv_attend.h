@@ -25,6 +25,7 @@
 #include <hip/hip_ext.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "komp_device.h"
 #include "komp_internal.h"
@@ -144,15 +145,68 @@ __device__ __forceinline__ Span visible(int i, int length, int prefix, int windo
   return s;
 }
 
-// One 32-key tile as it lies in a lane's registers.
+// Key codes of a lane's dword (Q4_0) or two (Q8_0) as operand A: subnormals (exact multiples of 2^-24; the channels of a
+// high nibble 16 times that) or signed values.
+template <bool SIGNED, int KF>
+__device__ __forceinline__ f16x8 key_codes(unsigned w, unsigned y) {
+  if constexpr (KF == KV_Q4_0) {
+    const unsigned x = w >> 8;
+    if constexpr (SIGNED)
+      return as_f16x8(signed_low(w & 0x000F000Fu, 8.f), signed_high(w & 0x00F000F0u), signed_low(x & 0x000F000Fu, 8.f),
+                      signed_high(x & 0x00F000F0u));
+    return as_f16x8(w & 0x000F000Fu, w & 0x00F000F0u, x & 0x000F000Fu, x & 0x00F000F0u);
+  } else {
+    if constexpr (SIGNED)
+      return as_f16x8(signed_low(w & 0x00FF00FFu, 128.f), signed_low(w >> 8 & 0x00FF00FFu, 128.f),
+                      signed_low(y & 0x00FF00FFu, 128.f), signed_low(y >> 8 & 0x00FF00FFu, 128.f));
+    return as_f16x8(w & 0x00FF00FFu, w >> 8 & 0x00FF00FFu, y & 0x00FF00FFu, y >> 8 & 0x00FF00FFu);
+  }
+}
+// Signed value codes of a lane's two dwords (tokens 4 quarter + r, 16 + 4 quarter + r) as operand A.  Q4_0: channels c
+// (half 0) or c + 16.
+template <int VF>
+__device__ __forceinline__ f16x8 value_codes(unsigned w0, unsigned w1, int half) {
+  if constexpr (VF == KV_Q4_0) {
+    const unsigned x0 = w0 >> 8, x1 = w1 >> 8;
+    if (half == 0)
+      return as_f16x8(signed_low(w0 & 0x000F000Fu, 8.f), signed_low(x0 & 0x000F000Fu, 8.f), signed_low(w1 & 0x000F000Fu, 8.f),
+                      signed_low(x1 & 0x000F000Fu, 8.f));
+    return as_f16x8(signed_high(w0 & 0x00F000F0u), signed_high(x0 & 0x00F000F0u), signed_high(w1 & 0x00F000F0u),
+                    signed_high(x1 & 0x00F000F0u));
+  } else {
+    return as_f16x8(signed_low(w0 & 0x00FF00FFu, 128.f), signed_low(w0 >> 8 & 0x00FF00FFu, 128.f),
+                    signed_low(w1 & 0x00FF00FFu, 128.f), signed_low(w1 >> 8 & 0x00FF00FFu, 128.f));
+  }
+}
+
+// f(integral_constant<int, 0>{}) .. f(integral_constant<int, N - 1>{})
+template <typename F, int... I>
+__device__ __forceinline__ void each_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  each_impl(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
+}
+
+// lane I of each 16 lanes, in all of them
+template <int I>
+__device__ __forceinline__ unsigned row_lane(unsigned v) {
+  return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x150 | I, 0xF, 0xF, false);
+}
+
+// One 32-key tile as it lies in a wave's registers.  The scales that a quarter needs are the same in its 16 lanes: each
+// lane loads one dword of them, and a DPP broadcast hands it to the row where it is used, which costs 8 NB instructions a
+// tile and saves 8 NB - 2 registers a tile in flight.
 template <int NB, int KF, int VF>
 struct KvTile {
   static constexpr int KW = NB * kv_code_bytes(KF) / 16;  // key dwords a lane of each 16 tokens
   static constexpr int VW = NB * kv_code_bytes(VF) / 8;   // value dwords a lane
+  static constexpr int SW = (4 * NB + 15) / 16;           // scale dwords a lane
   unsigned kc[2][KW];
-  unsigned ks[2][2 * NB];  // the f16 scales of keys 4 quarter + r: half r * NB + b
+  unsigned ks[SW];  // of a quarter, t * 2 NB + j: halves 2 j and 2 j + 1 of its 4 keys of the 16 tokens t (r * NB + b)
   unsigned vc[VW];
-  unsigned vs[4 * NB];  // of the lane's 8 tokens, block by block
+  unsigned vs[SW];  // of a quarter, 4 b + i: its tokens' pair i of block b
 
   __device__ __forceinline__ void load(const KvCache& c, int64_t unit, int lane) {
     constexpr int kbd = kv_kb(NB, KF) * (KF == KV_Q8_0 ? 2 : 1);  // dwords of one load
@@ -160,55 +214,36 @@ struct KvTile {
     const int quarter = lane >> 4;
     const uint8_t* k = c.kq + unit * (NB * 32 * kv_code_bytes(KF));
     const uint8_t* v = c.vq + unit * (NB * 32 * kv_code_bytes(VF));
-    const uint8_t* ksp = reinterpret_cast<const uint8_t*>(c.ks) + unit * (64 * NB);
-    const uint8_t* vsp = reinterpret_cast<const uint8_t*>(c.vs) + unit * (64 * NB);
+    const unsigned* ksp = reinterpret_cast<const unsigned*>(c.ks) + unit * (16 * NB);
+    const unsigned* vsp = reinterpret_cast<const unsigned*>(c.vs) + unit * (16 * NB);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < KW / kbd; ++i)
         load_words<kbd, kbd>(k + (t * KW * 64 + i * kbd * 64 + lane * kbd) * 4, &kc[t][i * kbd]);
-      load_words<2 * NB, NB % 2 == 0 ? 4 : 2>(ksp + t * 32 * NB + quarter * 8 * NB, ks[t]);
+#pragma unroll
+    for (int i = 0; i < SW; ++i) {
+      const int at = min(i * 16 + (lane & 15), 4 * NB - 1), t = at / (2 * NB);
+      ks[i] = ksp[t * 8 * NB + quarter * 2 * NB + at - t * 2 * NB];
+      vs[i] = vsp[quarter * 4 * NB + at];
     }
 #pragma unroll
     for (int i = 0; i < VW / vbd; ++i) load_words<vbd, vbd>(v + (i * vbd * 64 + lane * vbd) * 4, &vc[i * vbd]);
-    load_words<4 * NB, 4>(vsp + quarter * 16 * NB, vs);
   }
   // key codes of tokens 16 t ..., block b: operand A, as subnormals (exact multiples of 2^-24; the channels of a high
   // nibble 16 times that) or signed
   template <bool SIGNED>
   __device__ __forceinline__ f16x8 key(int t, int b) const {
     if constexpr (KF == KV_Q4_0) {
-      const unsigned w = kc[t][b], x = w >> 8;
-      if constexpr (SIGNED)
-        return as_f16x8(signed_low(w & 0x000F000Fu, 8.f), signed_high(w & 0x00F000F0u), signed_low(x & 0x000F000Fu, 8.f),
-                        signed_high(x & 0x00F000F0u));
-      return as_f16x8(w & 0x000F000Fu, w & 0x00F000F0u, x & 0x000F000Fu, x & 0x00F000F0u);
+      return key_codes<SIGNED, KF>(kc[t][b], 0u);
     } else {
-      const unsigned w = kc[t][2 * b], x = kc[t][2 * b + 1];
-      if constexpr (SIGNED)
-        return as_f16x8(signed_low(w & 0x00FF00FFu, 128.f), signed_low(w >> 8 & 0x00FF00FFu, 128.f),
-                        signed_low(x & 0x00FF00FFu, 128.f), signed_low(x >> 8 & 0x00FF00FFu, 128.f));
-      return as_f16x8(w & 0x00FF00FFu, w >> 8 & 0x00FF00FFu, x & 0x00FF00FFu, x >> 8 & 0x00FF00FFu);
+      return key_codes<SIGNED, KF>(kc[t][2 * b], kc[t][2 * b + 1]);
     }
-  }
-  __device__ __forceinline__ float key_scale(int t, int r, int b) const {
-    const int i = r * NB + b;
-    return static_cast<float>(as_f16x2(ks[t][i >> 1])[i & 1]);
   }
   // signed value codes of block b, channels 16 half ...: operand A
   __device__ __forceinline__ f16x8 value(int b, int half) const {
-    if constexpr (VF == KV_Q4_0) {
-      const unsigned w0 = vc[2 * b], w1 = vc[2 * b + 1], x0 = w0 >> 8, x1 = w1 >> 8;
-      if (half == 0)
-        return as_f16x8(signed_low(w0 & 0x000F000Fu, 8.f), signed_low(x0 & 0x000F000Fu, 8.f),
-                        signed_low(w1 & 0x000F000Fu, 8.f), signed_low(x1 & 0x000F000Fu, 8.f));
-      return as_f16x8(signed_high(w0 & 0x00F000F0u), signed_high(x0 & 0x00F000F0u), signed_high(w1 & 0x00F000F0u),
-                      signed_high(x1 & 0x00F000F0u));
-    } else {
-      const unsigned w0 = vc[4 * b + 2 * half], w1 = vc[4 * b + 2 * half + 1];
-      return as_f16x8(signed_low(w0 & 0x00FF00FFu, 128.f), signed_low(w0 >> 8 & 0x00FF00FFu, 128.f),
-                      signed_low(w1 & 0x00FF00FFu, 128.f), signed_low(w1 >> 8 & 0x00FF00FFu, 128.f));
-    }
+    if constexpr (VF == KV_Q4_0) return value_codes<VF>(vc[2 * b], vc[2 * b + 1], half);
+    return value_codes<VF>(vc[4 * b + 2 * half], vc[4 * b + 2 * half + 1], half);
   }
 };
 
@@ -254,282 +289,281 @@ __device__ __forceinline__ void store_out(void* out, int type, bool wide, int64_
   }
 }
 
-// `WIDE`: the workgroup's waves have columns of their own and walk the same keys; else they have the same columns and
-// share the keys out among them.
-template <int NB, int KF, int VF, bool PREC, int CT, bool WIDE>
-__global__ void __launch_bounds__(kAttendWaves * 64, 2) kv_attend_kernel(const AttendArgs a) {
-  constexpr int W = kAttendWaves, D = NB * 32, COLS = 16 * CT;
-  constexpr bool SIGNED = CT > 1 || PREC;
-  constexpr int PARTS = PREC ? 2 : 1;
-  constexpr int OT = 2 * NB;  // 16-channel tiles of the output
-  const int lane = threadIdx.x & 63, quarter = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y, seq = blockIdx.z;
-  const int split = blockIdx.x / a.groups;
-  const int grp = blockIdx.x - split * a.groups;
-  const int64_t row0 = a.starts ? a.starts[seq] : seq;
-  const int64_t row1 = a.starts ? a.starts[seq + 1] : seq + 1;
-  // rows past the query tensor do not exist, whatever `starts` says
-  const int count = row0 < 0 || row1 > a.rows || row1 < row0 ? 0 : static_cast<int>(row1 - row0);
-  const int length = max(0, min(static_cast<int64_t>(a.lengths[seq]), static_cast<int64_t>(a.table_cols) << a.c.page_log2));
-  const int shift = a.lengths[seq] - count;  // position of the sequence's first query
-  const int cols = count * a.group;
-  const int col0 = (WIDE ? grp * W + wave : grp) * COLS;
-  if (col0 >= cols) return;  // (the same for all waves where they join)
-  const int prefix = a.prefix ? a.prefix[seq] : 0;
+// What a call asks of one (sequence, kv head): its rows, its keys, and the visible ones.
+struct Sequence {
+  int64_t row0;
+  int cols;    // columns: rows * group
+  int length;  // keys
+  int shift;   // position of the first row
+  int prefix;
+  __device__ __forceinline__ Sequence(const AttendArgs& a, int seq) {
+    row0 = a.starts ? a.starts[seq] : seq;
+    const int64_t row1 = a.starts ? a.starts[seq + 1] : seq + 1;
+    // rows past the query tensor do not exist, whatever `starts` says
+    const int count = row0 < 0 || row1 > a.rows || row1 < row0 ? 0 : static_cast<int>(row1 - row0);
+    length = max(int64_t{0}, min(static_cast<int64_t>(a.lengths[seq]), static_cast<int64_t>(a.table_cols) << a.c.page_log2));
+    shift = a.lengths[seq] - count;
+    cols = count * a.group;
+    prefix = a.prefix ? a.prefix[seq] : 0;
+  }
+  __device__ __forceinline__ Span seen(const AttendArgs& a, int token) const {
+    return visible(shift + token, length, prefix, a.window);
+  }
+};
 
-  // this lane's columns
-  Span span[CT];
-  int64_t row[CT];
-  int head[CT];
+// A wave's columns and their softmax: queries, references and sums.  MODE: the type of the queries.
+template <int NB, int KF, int VF, int MODE, int CT>
+struct Columns {
+  static constexpr int COLS = 16 * CT;
+  static constexpr bool PREC = MODE == KV_F32;
+  static constexpr bool SIGNED = CT > 1 || PREC;
+  static constexpr int PARTS = PREC ? 2 : 1;
+  static constexpr int OT = 2 * NB;  // 16-channel tiles of the output
+  static constexpr float NONE = -__builtin_inff();
+
+  Span all;           // keys that some column sees
+  Span span[CT];      // of the lane's columns
   int pos[CT];
-  bool live[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int c = col0 + ct * 16 + (lane & 15);
-    live[ct] = c < cols;
-    const int token = live[ct] ? c / a.group : 0;
-    head[ct] = h * a.group + (live[ct] ? c - token * a.group : 0);
-    row[ct] = row0 + token;
-    pos[ct] = shift + token;
-    span[ct] = visible(pos[ct], length, prefix, a.window);
-    if (!live[ct]) span[ct] = Span{0, 0x7FFFFFFF};  // no column: never masked, never stored
-  }
-  // the wave's keys: from its first token's window to its last token's last key, and where all of them see every key
-  const int first_token = col0 / a.group, last_token = (min(cols, col0 + COLS) - 1) / a.group;
-  const Span s0 = visible(shift + first_token, length, prefix, a.window);
-  const Span s1 = visible(shift + last_token, length, prefix, a.window);
-  int tile0 = s0.lo >> 5, tile1 = (s1.hi + 31) >> 5;
-  if (tile0 > tile1) tile0 = tile1 = 0;
-  const int full_lo = s1.lo, full_hi = s0.hi;
-  if (a.splits > 1) {
-    const int per = (tile1 - tile0 + a.splits - 1) / a.splits;
-    tile0 = min(tile1, tile0 + split * per);
-    tile1 = min(tile1, tile0 + per);
-  }
-  constexpr int STEP = WIDE ? 1 : W;
-  if (!WIDE) tile0 += wave;
-
-  // queries: f16 parts, scaled so that a column's largest is in [2^13, 2^14)
   f16x8 qf[CT][NB][PARTS];
   f32x4 init[SIGNED ? 1 : NB];
-  float factor[CT];  // of the raw score, towards log2 units
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    float v[NB][8];
-    float top = 0.f;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int64_t at = row[ct] * a.q_stride_t + head[ct] * a.q_stride_h + b * 32 + quarter * 8;
-      if (!live[ct]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[b][e] = 0.f;
-      } else if (a.wide_q) {
-        if (a.type == KV_F32) {
-          const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at);
-          const f32x4 x = p[0], y = p[1];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[b][e] = x[e], v[b][4 + e] = y[e];
-        } else {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const unsigned u = e & 1 ? x[e >> 1] >> 16 : x[e >> 1] & 0xFFFFu;
-            v[b][e] = a.type == KV_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u)))
-                                       : __uint_as_float(u << 16);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[b][e] = load_query(a.q, a.type, at + e);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[b][e]));
-    }
-    top = quarters_max(top);
-    int up = 0;  // 2^up brings the largest to [2^13, 2^14); none for 0, infinity and NaN
-    if (top > 0.f && top < __builtin_inff()) up = 13 - (static_cast<int>(__builtin_amdgcn_frexp_expf(top)) - 1);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int ch = key_place<KF>(e);
-        float x = __builtin_ldexpf(v[b][ch], up);
-        const bool high = !SIGNED && KF == KV_Q4_0 && (e & 2);  // meets 16 times its code
-        const float y = high ? x * 0.0625f : x;
-        const _Float16 hi = static_cast<_Float16>(y);
-        qf[ct][b][0][e] = hi;
-        float used = static_cast<float>(hi);
-        if constexpr (PREC) {
-          const _Float16 lo = static_cast<_Float16>(y - used);
-          qf[ct][b][1][e] = lo;
-          used += static_cast<float>(lo);
-        }
-        sum += high ? used * 16.f : used;
-      }
-      if constexpr (!SIGNED) {
-        const float off = (KF == KV_Q4_0 ? -8.f : -128.f) * 0x1p-24f * quarters_sum(sum);
-        init[b] = f32x4{off, off, off, off};
-      }
-    }
-    factor[ct] = __builtin_ldexpf(a.cap > 0.f ? 2.f * a.scale / a.cap : a.scale, (SIGNED ? 0 : 24) - up);
-  }
-  const float cap2 = a.cap * kLog2e;
+  float fx[CT];       // of y, the raw or capped and biased score, to log2 units
+  float raw[CT];      // of the raw score, when it is capped or biased
   float slope[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) slope[ct] = a.slopes ? a.slopes[head[ct]] * kLog2e : 0.f;
-
-  // P = 2^(x - M), M = max - off.  A score may pass the max by 8 before M moves, so P <= 2^(8 + off), and P' stays below
-  // 2^15 with value scales below 2^(7 - off).  P in f16 allows off = 6, which serves scales below 2; f32 queries, whose P'
-  // is a product in f32, begin higher, so that P' of small scales keeps its bits.  Larger scales lower it.
-  int off = PREC ? 20 : 6;
   f32x4 acc[CT][OT];
-  float M[CT], lim[CT], l[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    M[ct] = -__builtin_inff();
-    lim[ct] = -__builtin_inff();
-    l[ct] = 0.f;
-#pragma unroll
-    for (int i = 0; i < OT; ++i) acc[ct][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float neg[CT];      // -M, or 0 before anything was seen
+  float lim[CT];      // y above which M moves
+  float l[CT];
+  int off;
+
+  // the lane's column ct: its query row and head; false where there is none
+  __device__ __forceinline__ bool place(const AttendArgs& a, const Sequence& s, int h, int col0, int ct, int lane,
+                                        int64_t& row, int& head) const {
+    const int c = col0 + ct * 16 + (lane & 15);
+    const int token = c < s.cols ? c / a.group : 0;
+    row = s.row0 + token;
+    head = h * a.group + (c < s.cols ? c - token * a.group : 0);
+    return c < s.cols;
   }
 
-  const int tiles_log2 = a.c.page_log2 - 5;
-  const int32_t* table = a.tables + seq * a.table_stride;
-  // the unit (32 tokens of a page and head) of a tile, or -1 for a page that the cache does not have
-  auto unit_of = [&](int tile) -> int64_t {
-    const int page = table[tile >> tiles_log2];
-    if (page < 0 || page >= a.c.pages) return -1;
-    return ((static_cast<int64_t>(page) * a.c.heads + h) << tiles_log2) + (tile & ((1 << tiles_log2) - 1));
-  };
+  // M of column ct (-inf before anything was seen)
+  __device__ __forceinline__ float reference(int ct) const { return lim[ct] == NONE ? NONE : -neg[ct]; }
 
-  auto step = [&](const KvTile<NB, KF, VF>& kv, int tile, auto masked_c) {
-    constexpr bool MASKED = decltype(masked_c)::value;
-    const int key0 = tile * 32 + quarter * 4;
-    float x[CT][2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const f16x8 k = kv.template key<SIGNED>(t, b);
-        float d[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) d[r] = kv.key_scale(t, r, b);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          f32x4 c = SIGNED ? f32x4{0.f, 0.f, 0.f, 0.f} : init[SIGNED ? 0 : b];
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[ct][b][p], c, 0, 0, 0);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[ct][t][r] = b == 0 ? d[r] * c[r] : fmaf(d[r], c[r], x[ct][t][r]);
-        }
-      }
-    }
-    // the scales of keys that no column sees are not looked at (they may hold anything)
-    unsigned vs[4 * NB];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      unsigned m = 0xFFFFFFFFu;
-      if constexpr (MASKED) {
-        auto in = [&](int r) {
-          const int j = key0 + 16 * (i >> 1) + r;
-          return j >= s0.lo && j < s1.hi;
-        };
-        m = (in(i & 1) ? 0xFFFFu : 0u) | (in(2 + (i & 1)) ? 0xFFFF0000u : 0u);
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) vs[4 * b + i] = kv.vs[4 * b + i] & m;
-    }
-    // larger scales may need a lower `off`: f32 queries look at every tile's largest, the others at scales of 2 or more
-    // (an f16 with bit 14 set)
-    int off_now = off;
-    bool look = PREC;
-    if constexpr (!PREC) {
-      unsigned bits = 0;
-#pragma unroll
-      for (int i = 0; i < 4 * NB; ++i) bits |= vs[i];
-      look = __builtin_amdgcn_ballot_w64((bits & 0x40004000u) != 0) != 0;
-    }
-    if (look) {
-      unsigned e = 0;  // the largest finite scale's exponent field, in bits 10..14
-#pragma unroll
-      for (int i = 0; i < 4 * NB; ++i) {
-        const unsigned lo = vs[i] & 0x7C00u, hi = vs[i] >> 16 & 0x7C00u;
-        e = max(e, max(lo == 0x7C00u ? 0u : lo, hi == 0x7C00u ? 0u : hi));
-      }
-      const int top = static_cast<int>(quarters_max(static_cast<float>(e >> 10)));
-      off_now = __builtin_amdgcn_readfirstlane(min(off, 21 - max(top, 1)));
-    }
-    bool move = off_now < off;
+  __device__ __forceinline__ void begin(const AttendArgs& a, const Sequence& s, int h, int col0, int lane) {
+    const int quarter = lane >> 4;
+    off = PREC ? 20 : 6;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
+      int64_t row;
+      int head;
+      const bool live = place(a, s, h, col0, ct, lane, row, head);
+      pos[ct] = s.shift + static_cast<int>(row - s.row0);
+      span[ct] = live ? s.seen(a, static_cast<int>(row - s.row0)) : Span{0, 0x7FFFFFFF};  // no column: never masked or stored
+      slope[ct] = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+      // queries: f16 parts, scaled so that a column's largest is in [2^13, 2^14)
+      float v[NB][8];
+      float top = 0.f;
+      const float sign = a.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int64_t at = row * a.q_stride_t + head * a.q_stride_h + b * 32 + quarter * 8;
+        if (!live) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[b][e] = 0.f;
+        } else if (a.wide_q) {
+          if constexpr (PREC) {
+            const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at);
+            const f32x4 x = p[0], y = p[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[b][e] = x[e], v[b][4 + e] = y[e];
+          } else {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const unsigned u = e & 1 ? x[e >> 1] >> 16 : x[e >> 1] & 0xFFFFu;
+              v[b][e] = MODE == KV_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u)))
+                                       : __uint_as_float(u << 16);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[b][e] = load_query(a.q, MODE, at + e);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          top = fmaxf(top, fabsf(v[b][e]));
+          v[b][e] *= sign;
+        }
+      }
+      top = quarters_max(top);
+      int up = 0;  // 2^up brings the largest to [2^13, 2^14); none for 0, infinity and NaN
+      if (top > 0.f && top < __builtin_inff()) up = 13 - (static_cast<int>(__builtin_amdgcn_frexp_expf(top)) - 1);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_ldexpf(v[b][key_place<KF>(e)], up);
+          const bool high = !SIGNED && KF == KV_Q4_0 && (e & 2);  // meets 16 times its code
+          const float y = high ? x * 0.0625f : x;
+          const _Float16 hi = static_cast<_Float16>(y);
+          qf[ct][b][0][e] = hi;
+          if constexpr (PREC) qf[ct][b][1][e] = static_cast<_Float16>(y - static_cast<float>(hi));
+          sum += high ? static_cast<float>(hi) * 16.f : static_cast<float>(hi);
+        }
+        if constexpr (!SIGNED) {
+          const float o = (KF == KV_Q4_0 ? -8.f : -128.f) * 0x1p-24f * quarters_sum(sum);
+          init[b] = f32x4{o, o, o, o};
+        }
+      }
+      const float unit = __builtin_ldexpf(fabsf(a.scale), (SIGNED ? 0 : 24) - up);
+      raw[ct] = a.cap > 0.f ? 2.f * unit / a.cap : unit;
+      fx[ct] = a.cap > 0.f || a.slopes ? 1.f : unit;
+      neg[ct] = 0.f;
+      lim[ct] = NONE;
+      l[ct] = 0.f;
+#pragma unroll
+      for (int i = 0; i < OT; ++i) acc[ct][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // capped and biased scores from raw ones
+  __device__ __forceinline__ void shape(const AttendArgs& a, int ct, int key0, float (&y)[2][4]) const {
+    if (a.cap == 0.f && a.slopes == nullptr) return;
+    const float cap = a.cap * kLog2e;
+    const float back = static_cast<float>(pos[ct] - key0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = y[t][r] * raw[ct];
+        // cap tanh(s / cap), tanh u = 1 - 2 / (e^2u + 1)
+        if (a.cap > 0.f) x = cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.f);
+        y[t][r] = fmaf(-slope[ct], fabsf(back - (16 * t + r)), x);
+      }
+  }
+
+  // M moves to the largest score so far, and what was summed with it
+  __device__ __forceinline__ void move(int off_now, const float (&y)[CT][2][4]) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float top = y[ct][0][0];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[ct][t][r] *= factor[ct];
-      if (a.cap > 0.f) {  // cap tanh(s / cap), tanh u = 1 - 2 / (e^2u + 1)
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, y[ct][t][r]);
+      top = quarters_max(top * fx[ct]);
+      const float before = reference(ct);
+      top = fmaxf(top, before + off);
+      const float now = top - off_now;
+      // (nothing seen yet: nothing to rescale)
+      const float by = before == NONE ? 0.f : __builtin_amdgcn_exp2f(before - now);
+      l[ct] *= by;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int i = 0; i < OT; ++i) acc[ct][i] *= by;
+      neg[ct] = now == NONE ? 0.f : -now;
+      lim[ct] = now == NONE ? NONE : fx[ct] > 0.f ? (top + 8.f) / fx[ct] : __builtin_inff();
+    }
+    off = off_now;
+  }
+
+  // A tile of 32 keys from key `first` on.  MASKED: some column does not see some of them; a key that a column does not
+  // see gets a P' of 0 there whatever its scale holds.
+  template <bool MASKED>
+  __device__ __forceinline__ void step(const AttendArgs& a, const KvTile<NB, KF, VF>& kv, int first, int lane) {
+    const int quarter = lane >> 4, key0 = first + quarter * 4;
+    float y[CT][2][4];
+    each<2>([&](auto tc) {
+      constexpr int t = tc.value;
+      f32x4 c[CT][NB];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            x[ct][t][r] = cap2 - 2.f * cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x[ct][t][r]) + 1.f);
+      for (int b = 0; b < NB; ++b) {
+        const f16x8 k = kv.template key<SIGNED>(t, b);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          c[ct][b] = SIGNED ? f32x4{0.f, 0.f, 0.f, 0.f} : init[SIGNED ? 0 : b];
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) c[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[ct][b][p], c[ct][b], 0, 0, 0);
+        }
       }
-      if (a.slopes) {
-        const float back = static_cast<float>(pos[ct] - key0);
+      each<2 * NB>([&](auto jc) {
+        constexpr int j = jc.value, at = t * 2 * NB + j;
+        const f16x2 d = as_f16x2(row_lane<at % 16>(kv.ks[at / 16]));
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int e = 0; e < 2; ++e) {
+          constexpr int i0 = 2 * j;
+          const int r = (i0 + e) / NB, b = (i0 + e) % NB;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[ct][t][r] = fmaf(-slope[ct], fabsf(back - (16 * t + r)), x[ct][t][r]);
+          for (int ct = 0; ct < CT; ++ct)
+            y[ct][t][r] = b == 0 ? static_cast<float>(d[e]) * c[ct][b][r] : fmaf(static_cast<float>(d[e]), c[ct][b][r], y[ct][t][r]);
+        }
+      });
+    });
+    // larger value scales may need a lower `off`; the scales of keys that no column sees are not looked at
+    unsigned vs[KvTile<NB, KF, VF>::SW];
+    bool above = false;
+#pragma unroll
+    for (int i = 0; i < KvTile<NB, KF, VF>::SW; ++i) {
+      vs[i] = kv.vs[i];
+      if constexpr (MASKED) {
+        const int pair = min(i * 16 + (lane & 15), 4 * NB - 1) & 3, j = key0 + 16 * (pair >> 1) + (pair & 1);
+        vs[i] &= (j >= all.lo && j < all.hi ? 0xFFFFu : 0u) | (j + 2 >= all.lo && j + 2 < all.hi ? 0xFFFF0000u : 0u);
       }
+      const unsigned lo = vs[i] & 0x7C00u, hi = vs[i] >> 16 & 0x7C00u, most = static_cast<unsigned>(21 - off) << 10;
+      above |= (lo > most && lo != 0x7C00u) || (hi > most && hi != 0x7C00u);
+    }
+    bool go = above;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      shape(a, ct, key0, y[ct]);
       if constexpr (MASKED) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = key0 + 16 * t + r;
-            if (j < span[ct].lo || j >= span[ct].hi) x[ct][t][r] = -__builtin_inff();
+            if (j < span[ct].lo || j >= span[ct].hi) y[ct][t][r] = NONE;
           }
       }
-      const float top = fmaxf(fmaxf(fmaxf(x[ct][0][0], x[ct][0][1]), fmaxf(x[ct][0][2], x[ct][0][3])),
-                              fmaxf(fmaxf(x[ct][1][0], x[ct][1][1]), fmaxf(x[ct][1][2], x[ct][1][3])));
-      move |= top > lim[ct];
+      const float top = fmaxf(fmaxf(fmaxf(y[ct][0][0], y[ct][0][1]), fmaxf(y[ct][0][2], y[ct][0][3])),
+                              fmaxf(fmaxf(y[ct][1][0], y[ct][1][1]), fmaxf(y[ct][1][2], y[ct][1][3])));
+      go |= top > lim[ct];
     }
-    if (__builtin_amdgcn_ballot_w64(move) != 0) {
-      const int before = off;
-      off = off_now;
+    if (__builtin_amdgcn_ballot_w64(go) != 0) {
+      int off_now = off;
+      if (__builtin_amdgcn_ballot_w64(above) != 0) {
+        unsigned e = 0;  // the largest finite scale's exponent field
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        float top = M[ct] + before;
+        for (int i = 0; i < KvTile<NB, KF, VF>::SW; ++i) {
+          const unsigned lo = vs[i] >> 10 & 31, hi = vs[i] >> 26 & 31;
+          e = max(e, max(lo == 31 ? 0u : lo, hi == 31 ? 0u : hi));
+        }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, x[ct][t][r]);
-        top = quarters_max(top);
-        const float now = top - off;
-        // (nothing seen yet: M stays -inf, and there is nothing to rescale)
-        const float by = M[ct] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(M[ct] - now);
-        l[ct] *= by;
-#pragma unroll
-        for (int i = 0; i < OT; ++i) acc[ct][i] *= by;
-        M[ct] = now;
-        lim[ct] = top + 8.f;
+        for (int o = 32; o > 0; o >>= 1) e = max(e, static_cast<unsigned>(__shfl_xor(static_cast<int>(e), o, 64)));
+        off_now = __builtin_amdgcn_readfirstlane(min(off, 21 - static_cast<int>(max(e, 1u))));
       }
+      move(off_now, y);
     }
-    unsigned keep[CT][4];  // masked tiles: a masked key's P' is 0 whatever its scale holds
-    float p[CT][2][4];
     unsigned ph[CT][4];
+    unsigned keep[MASKED ? CT : 1][4];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const float ref = M[ct] == -__builtin_inff() ? 0.f : M[ct];
+      float(&p)[2][4] = y[ct];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[ct][t][r] = __builtin_amdgcn_exp2f(x[ct][t][r] - ref);
-          l[ct] += p[ct][t][r];
+          float x = fmaf(p[t][r], fx[ct], neg[ct]);
+          if constexpr (MASKED) {
+            const int j = key0 + 16 * t + r;
+            if (j < span[ct].lo || j >= span[ct].hi) x = NONE;
+          }
+          p[t][r] = __builtin_amdgcn_exp2f(x);
+          l[ct] += p[t][r];
         }
-        ph[ct][2 * t] = pack_f16(p[ct][t][0], p[ct][t][2]);
-        ph[ct][2 * t + 1] = pack_f16(p[ct][t][1], p[ct][t][3]);
+        if constexpr (MODE == KV_BF16) {
+          ph[ct][2 * t] = pack_f16(p[t][0], p[t][2]);
+          ph[ct][2 * t + 1] = pack_f16(p[t][1], p[t][3]);
+        }
         if constexpr (MASKED) {
           auto in = [&](int r) {
             const int j = key0 + 16 * t + r;
@@ -540,29 +574,31 @@ __global__ void __launch_bounds__(kAttendWaves * 64, 2) kv_attend_kernel(const A
         }
       }
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
+    each<NB>([&](auto bc) {
+      constexpr int b = bc.value;
       unsigned w[CT][PARTS][4];
+      each<4>([&](auto ic) {
+        constexpr int i = ic.value, at = 4 * b + i;
+        const f16x2 d = as_f16x2(row_lane<at % 16>(vs[at / 16]));
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (PREC) {
-            const f16x2 d = as_f16x2(vs[4 * b + i]);
-            const float y0 = p[ct][i >> 1][i & 1] * static_cast<float>(d[0]);
-            const float y1 = p[ct][i >> 1][2 + (i & 1)] * static_cast<float>(d[1]);
-            w[ct][0][i] = pack_f16(y0, y1);
-            const f16x2 hi = as_f16x2(w[ct][0][i]);
-            w[ct][1][i] = pack_f16(y0 - static_cast<float>(hi[0]), y1 - static_cast<float>(hi[1]));
+        for (int ct = 0; ct < CT; ++ct) {
+          if constexpr (MODE == KV_BF16) {
+            w[ct][0][i] = __builtin_bit_cast(unsigned, as_f16x2(ph[ct][i]) * d);
           } else {
-            w[ct][0][i] = __builtin_bit_cast(unsigned, as_f16x2(ph[ct][i]) * as_f16x2(vs[4 * b + i]));
+            const float y0 = y[ct][i >> 1][i & 1] * static_cast<float>(d[0]);
+            const float y1 = y[ct][i >> 1][2 + (i & 1)] * static_cast<float>(d[1]);
+            w[ct][0][i] = pack_f16(y0, y1);
+            if constexpr (PREC) {
+              const f16x2 hi = as_f16x2(w[ct][0][i]);
+              w[ct][PARTS - 1][i] = pack_f16(y0 - static_cast<float>(hi[0]), y1 - static_cast<float>(hi[1]));
+            }
           }
           if constexpr (MASKED) {
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) w[ct][part][i] &= keep[ct][i];
           }
         }
-      }
+      });
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const f16x8 v = kv.value(b, half);
@@ -573,101 +609,167 @@ __global__ void __launch_bounds__(kAttendWaves * 64, 2) kv_attend_kernel(const A
             acc[ct][2 * b + half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                 v, as_f16x8(w[ct][part][0], w[ct][part][1], w[ct][part][2], w[ct][part][3]), acc[ct][2 * b + half], 0, 0, 0);
       }
-    }
-  };
-
-  for (int tile = tile0; tile < tile1; tile += STEP) {
-    const int64_t unit = unit_of(tile);
-    if (unit < 0) continue;
-    KvTile<NB, KF, VF> kv;
-    kv.load(a.c, unit, lane);
-    if (tile * 32 >= full_lo && tile * 32 + 32 <= full_hi)
-      step(kv, tile, std::false_type{});
-    else
-      step(kv, tile, std::true_type{});
+    });
   }
 
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) l[ct] = quarters_sum(l[ct]);
-
-  if constexpr (!WIDE) {
-    // join the waves, a column tile at a time: the upper half hands its sums to the lower half, then wave 1 to wave 0
-    __shared__ f32x4 so[W / 2][OT][64];
-    __shared__ float2 sm[W / 2][16];
+  // the columns' results, or their part of a split
+  __device__ __forceinline__ void store(const AttendArgs& a, const Sequence& s, int h, int col0, int split, int lane) const {
+    constexpr int D = NB * 32;
+    const int quarter = lane >> 4;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
+      int64_t row;
+      int head;
+      if (!place(a, s, h, col0, ct, lane, row, head)) continue;
+      const float M = reference(ct);
+      if (a.splits > 1) {
+        const int64_t at = (split * a.rows + row) * a.heads + head;
+        if (lane < 16) a.part_m[at] = float2{M, l[ct]};
+        if (M == NONE) continue;
 #pragma unroll
-      for (int half = W / 2; half >= 1; half >>= 1) {
-        if (wave >= half && wave < 2 * half) {
-          if (lane < 16) sm[wave - half][lane] = float2{M[ct], l[ct]};
+        for (int i = 0; i < OT; ++i)
+          *reinterpret_cast<f32x4*>(a.part_o + at * D + i * 16 + quarter * 4) = acc[ct][i];
+      } else {
+        const float inv = l[ct] == 0.f ? 0.f : 1.f / l[ct];
+        if (a.lse && lane < 16)
+          a.lse[row * a.heads + head] = l[ct] == 0.f ? NONE : (M + __log2f(l[ct])) * (1.f / kLog2e);
+        const int64_t at = row * a.out_stride_t + head * a.out_stride_h + quarter * 4;
 #pragma unroll
-          for (int i = 0; i < OT; ++i) so[wave - half][i][lane] = acc[ct][i];
-        }
-        __syncthreads();
-        if (wave < half) {
-          const float2 other = sm[wave][lane & 15];
-          const float top = fmaxf(M[ct], other.x);
-          const float f0 = M[ct] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(M[ct] - top);
-          const float f1 = other.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(other.x - top);
-          l[ct] = l[ct] * f0 + other.y * f1;
-          M[ct] = top;
-#pragma unroll
-          for (int i = 0; i < OT; ++i) acc[ct][i] = acc[ct][i] * f0 + so[wave][i][lane] * f1;
-        }
-        __syncthreads();
+        for (int i = 0; i < OT; ++i) store_out(a.out, MODE, a.wide_out, at + i * 16, acc[ct][i] * inv);
       }
     }
-    if (wave != 0) return;
+  }
+};
+
+// The pages of a sequence and head: where a tile of 32 keys lies, in units of 32 tokens of a page and head; -1 for a page
+// that the cache does not have.
+struct Pages {
+  const int32_t* table;
+  int64_t pages;
+  int heads, h, log2;
+  __device__ __forceinline__ Pages(const AttendArgs& a, int seq, int h)
+      : table(a.tables + seq * a.table_stride), pages(a.c.pages), heads(a.c.heads), h(h), log2(a.c.page_log2 - 5) {}
+  __device__ __forceinline__ int64_t unit(int tile) const {
+    const int page = table[tile >> log2];
+    if (page < 0 || page >= pages) return -1;
+    return ((static_cast<int64_t>(page) * heads + h) << log2) + (tile & ((1 << log2) - 1));
+  }
+};
+
+// Few columns over many keys: the waves of a workgroup have the same columns and share its keys out among them, a tile
+// each in turn, with DEEP tiles in flight a wave; they join their sums in shared memory.
+template <int NB, int KF, int VF, int MODE, int CT>
+constexpr int kv_few_waves() {  // waves a SIMD that its registers leave room for
+  return NB == 8 || (NB == 4 && CT == 2) ? 1 : 2;
+}
+template <int NB, int KF, int VF, int MODE, int CT>
+__global__ void __launch_bounds__(kAttendWaves * 64, (kv_few_waves<NB, KF, VF, MODE, CT>())) kv_attend_few_kernel(const AttendArgs a) {
+  constexpr int W = kAttendWaves, DEEP = 2;
+  using Cols = Columns<NB, KF, VF, MODE, CT>;
+  constexpr int COLS = Cols::COLS, OT = Cols::OT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.y, seq = blockIdx.z, split = blockIdx.x / a.groups, col0 = (blockIdx.x - split * a.groups) * COLS;
+  const Sequence s(a, seq);
+  if (col0 >= s.cols) return;
+  const Span s0 = s.seen(a, col0 / a.group), s1 = s.seen(a, (min(s.cols, col0 + COLS) - 1) / a.group);
+  // the workgroup's tiles, and those of them that all columns see
+  int tile0 = s0.lo >> 5, tile1 = (s1.hi + 31) >> 5;
+  if (tile0 > tile1) tile0 = tile1 = 0;
+  const int per = (tile1 - tile0 + a.splits - 1) / a.splits;
+  tile0 = min(tile1, tile0 + split * per);
+  tile1 = min(tile1, tile0 + per);
+  int full0 = max(tile0, (s1.lo + 31) >> 5), full1 = min(tile1, s0.hi >> 5);
+  if (full0 >= full1) full0 = full1 = tile1;
+
+  const Pages pages(a, seq, h);
+  KvTile<NB, KF, VF> kv[DEEP];
+  int64_t unit[DEEP];
+#pragma unroll
+  for (int i = 0; i < DEEP; ++i) {
+    const int tile = full0 + wave + i * W;
+    unit[i] = tile < full1 ? pages.unit(tile) : -1;
+    if (unit[i] >= 0) kv[i].load(a.c, unit[i], lane);
+  }
+  Cols cols;
+  cols.all = Span{s0.lo, s1.hi};
+  cols.begin(a, s, h, col0, lane);
+  for (int tile = full0 + wave; tile < full1; tile += DEEP * W) {
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) {
+      const int now = tile + i * W, next = now + DEEP * W;
+      if (unit[i] >= 0) cols.template step<false>(a, kv[i], now * 32, lane);
+      unit[i] = next < full1 ? pages.unit(next) : -1;
+      if (unit[i] >= 0) kv[i].load(a.c, unit[i], lane);
+    }
+  }
+  // the tiles at the masks' edges: before the full ones, and after them
+  const int before = min(full0, tile1) - tile0, edges = before + tile1 - full1;
+  for (int e = wave; e < edges; e += W) {
+    const int tile = e < before ? tile0 + e : full1 + e - before;
+    const int64_t u = pages.unit(tile);
+    if (u < 0) continue;
+    KvTile<NB, KF, VF> one;
+    one.load(a.c, u, lane);
+    cols.template step<true>(a, one, tile * 32, lane);
   }
 
+  // join the waves, a column tile at a time: the upper half hands its sums to the lower half, then wave 1 to wave 0
+  __shared__ f32x4 so[W / 2][OT][64];
+  __shared__ float2 sm[W / 2][16];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    if (!live[ct]) continue;
-    if (a.splits > 1) {
-      const int64_t at = (split * a.rows + row[ct]) * a.heads + head[ct];
-      if (lane < 16) a.part_m[at] = float2{M[ct], l[ct]};
-      if (M[ct] == -__builtin_inff()) continue;
+    float M = cols.reference(ct);
+    cols.l[ct] = quarters_sum(cols.l[ct]);
 #pragma unroll
-      for (int i = 0; i < OT; ++i)
-        *reinterpret_cast<f32x4*>(a.part_o + at * D + i * 16 + quarter * 4) = acc[ct][i];
-    } else {
-      const float inv = l[ct] == 0.f ? 0.f : 1.f / l[ct];
-      if (a.lse && lane < 16)
-        a.lse[row[ct] * a.heads + head[ct]] = l[ct] == 0.f ? -__builtin_inff() : (M[ct] + __log2f(l[ct])) * (1.f / kLog2e);
-      const int64_t at = row[ct] * a.out_stride_t + head[ct] * a.out_stride_h + quarter * 4;
+    for (int half = W / 2; half >= 1; half >>= 1) {
+      if (wave >= half && wave < 2 * half) {
+        if (lane < 16) sm[wave - half][lane] = float2{M, cols.l[ct]};
 #pragma unroll
-      for (int i = 0; i < OT; ++i) {
-        const f32x4 o = acc[ct][i] * inv;
-        store_out(a.out, a.type, a.wide_out, at + i * 16, o);
+        for (int i = 0; i < OT; ++i) so[wave - half][i][lane] = cols.acc[ct][i];
       }
+      __syncthreads();
+      if (wave < half) {
+        const float2 other = sm[wave][lane & 15];
+        const float top = fmaxf(M, other.x);
+        const float f0 = M == Cols::NONE ? 0.f : __builtin_amdgcn_exp2f(M - top);
+        const float f1 = other.x == Cols::NONE ? 0.f : __builtin_amdgcn_exp2f(other.x - top);
+        cols.l[ct] = cols.l[ct] * f0 + other.y * f1;
+        M = top;
+#pragma unroll
+        for (int i = 0; i < OT; ++i) cols.acc[ct][i] = cols.acc[ct][i] * f0 + so[wave][i][lane] * f1;
+      }
+      __syncthreads();
     }
+    cols.neg[ct] = -M;
+    cols.lim[ct] = M == Cols::NONE ? Cols::NONE : 0.f;
   }
+  if (wave == 0) cols.store(a, s, h, col0, split, lane);
 }
 
-// `plan` says the kernel: column tiles a wave, and whether the waves have columns of their own
-template <int NB, int KF, int VF>
-hipError_t launch_attend_blocks(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream) {
+// WIDE_KERNEL
+
+// Run the kernel of `plan`: few columns or many.
+template <int NB, int KF, int VF, int MODE>
+hipError_t launch_attend_mode(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(a.splits) * static_cast<unsigned>(a.groups), static_cast<unsigned>(a.c.heads),
                   static_cast<unsigned>(batch));
-  auto run = [&](auto kern) {
+  auto run = [&](auto kern, int threads) {
     const Timing tm = timing_slot(KIND_PROBE);
     if (tm.on) {
-      hipExtLaunchKernelGGL(kern, grid, dim3(kAttendWaves * 64), 0, stream, tm.start, tm.stop, 0, a);
+      hipExtLaunchKernelGGL(kern, grid, dim3(threads), 0, stream, tm.start, tm.stop, 0, a);
     } else {
-      hipLaunchKernelGGL(kern, grid, dim3(kAttendWaves * 64), 0, stream, a);
+      hipLaunchKernelGGL(kern, grid, dim3(threads), 0, stream, a);
     }
     return hipGetLastError();
   };
-  if (a.type == KV_F32) {
-    if (plan.wide) return run(kv_attend_kernel<NB, KF, VF, true, 2, true>);
-    if (plan.ct == 1) return run(kv_attend_kernel<NB, KF, VF, true, 1, false>);
-    return run(kv_attend_kernel<NB, KF, VF, true, 2, false>);
-  }
-  constexpr int MOST = NB <= 4 ? 4 : 2;
-  if (plan.wide) return run(kv_attend_kernel<NB, KF, VF, false, MOST, true>);
-  if (plan.ct == 1) return run(kv_attend_kernel<NB, KF, VF, false, 1, false>);
-  if (plan.ct == 2 || MOST == 2) return run(kv_attend_kernel<NB, KF, VF, false, 2, false>);
-  return run(kv_attend_kernel<NB, KF, VF, false, MOST, false>);
+  if (plan.ct == 1) return run(kv_attend_few_kernel<NB, KF, VF, MODE, 1>, kAttendWaves * 64);
+  return run(kv_attend_few_kernel<NB, KF, VF, MODE, 2>, kAttendWaves * 64);
+}
+template <int NB, int KF, int VF>
+hipError_t launch_attend_blocks(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream) {
+  if (a.type == KV_F32) return launch_attend_mode<NB, KF, VF, KV_F32>(a, plan, batch, stream);
+  if (a.type == KV_F16) return launch_attend_mode<NB, KF, VF, KV_F16>(a, plan, batch, stream);
+  return launch_attend_mode<NB, KF, VF, KV_BF16>(a, plan, batch, stream);
 }
 
 template <int KF, int VF>

@@ -12,18 +12,9 @@ AttendPlan plan_of(const KvAttendCall& c) {
   const int group = c.heads / c.cache.heads;
   const int64_t cols = c.max_queries * group;
   const int64_t units = static_cast<int64_t>(c.batch) * c.cache.heads;
-  const int most = c.type != KV_F32 && c.cache.dim <= 128 ? 4 : 2;
   AttendPlan p;
-  p.ct = cols <= 16 ? 1 : cols <= 32 || most == 2 ? 2 : most;
   p.wide = false;
-  p.splits = 1;
-  const int64_t wide_groups = (cols + 16 * most * kAttendWaves - 1) / (16 * most * kAttendWaves);
-  if (cols > 16 * most && units * wide_groups >= 256) {
-    p.ct = most;
-    p.wide = true;
-    p.groups = static_cast<int>(wide_groups);
-    return p;
-  }
+  p.ct = cols <= 16 ? 1 : 2;
   p.groups = static_cast<int>((cols + 16 * p.ct - 1) / (16 * p.ct));
   const int64_t tiles = (c.max_length + 31) / 32;
   const int64_t want = 1024 / (units * p.groups), most_splits = tiles / (2 * kAttendWaves);
