@@ -67,10 +67,10 @@ struct AttendArgs {
   float2* part_m;  // [split][row][head]: M and l
 };
 
-// column tiles of 16 a wave, own columns a wave or shared ones, column groups a sequence, splits of its keys
+// many: the kernel of kv_many.h; else ct column tiles of 16 a workgroup.  Column groups a sequence, splits of its keys
 struct AttendPlan {
+  bool many;
   int ct;
-  bool wide;
   int groups;
   int splits;
 };
@@ -81,6 +81,7 @@ hipError_t launch_attend_q8_q8(const AttendArgs& a, const AttendPlan& plan, int 
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kAttendWaves = 4;
+constexpr int many_cols(int dim, int type) { return dim == 256 ? 128 : type == KV_F32 ? 192 : 256; }  // of a workgroup of kv_many.h
 
 template <typename T>
 __device__ __forceinline__ T quarters_max(T v) {  // over the lanes of a column: lane ^ 16, lane ^ 32
@@ -192,7 +193,7 @@ __device__ __forceinline__ void each(F&& f) {
 // lane I of each 16 lanes, in all of them
 template <int I>
 __device__ __forceinline__ unsigned row_lane(unsigned v) {
-  return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x150 | I, 0xF, 0xF, false);
+  return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x150 | I, 0xF, 0xF, true);  // (no lane keeps an old value)
 }
 
 // One 32-key tile as it lies in a wave's registers.  The scales that a quarter needs are the same in its 16 lanes: each
@@ -311,12 +312,12 @@ struct Sequence {
   }
 };
 
-// A wave's columns and their softmax: queries, references and sums.  MODE: the type of the queries.
-template <int NB, int KF, int VF, int MODE, int CT>
+// A wave's columns and their softmax: queries, references and sums.  MODE: the type of the queries.  SIGNED: how it takes
+// key codes.
+template <int NB, int KF, int VF, int MODE, int CT, bool SIGNED = (CT > 1 || MODE == KV_F32)>
 struct Columns {
   static constexpr int COLS = 16 * CT;
   static constexpr bool PREC = MODE == KV_F32;
-  static constexpr bool SIGNED = CT > 1 || PREC;
   static constexpr int PARTS = PREC ? 2 : 1;
   static constexpr int OT = 2 * NB;  // 16-channel tiles of the output
   static constexpr float NONE = -__builtin_inff();
@@ -428,7 +429,6 @@ struct Columns {
 
   // capped and biased scores from raw ones
   __device__ __forceinline__ void shape(const AttendArgs& a, int ct, int key0, float (&y)[2][4]) const {
-    if (a.cap == 0.f && a.slopes == nullptr) return;
     const float cap = a.cap * kLog2e;
     const float back = static_cast<float>(pos[ct] - key0);
 #pragma unroll
@@ -464,6 +464,75 @@ struct Columns {
       lim[ct] = now == NONE ? NONE : fx[ct] > 0.f ? (top + 8.f) / fx[ct] : __builtin_inff();
     }
     off = off_now;
+  }
+
+  // Raw scores to probabilities 2^(x - M + ev), and the sums of 2^(x - M).
+  template <bool MASKED>
+  __device__ __forceinline__ void soften(const AttendArgs& a, int key0, int off_now, int ev, float (&y)[CT][2][4]) {
+    const bool shaped = a.cap > 0.f || a.slopes != nullptr;
+    bool go = off_now < off;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      if (shaped) shape(a, ct, key0, y[ct]);
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = key0 + 16 * t + r;
+            if (j < span[ct].lo || j >= span[ct].hi) y[ct][t][r] = NONE;
+          }
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float top = fmaxf(fmaxf(fmaxf(y[ct][0][0], y[ct][0][1]), fmaxf(y[ct][0][2], y[ct][0][3])),
+                              fmaxf(fmaxf(y[ct][1][0], y[ct][1][1]), fmaxf(y[ct][1][2], y[ct][1][3])));
+      go |= top > lim[ct];
+    }
+    if (__builtin_amdgcn_ballot_w64(go) != 0) move(off_now, y);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float n = neg[ct] + ev;
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = fmaf(y[ct][t][r], fx[ct], n);
+          if constexpr (MASKED) {
+            const int j = key0 + 16 * t + r;
+            if (j < span[ct].lo || j >= span[ct].hi) x = NONE;
+          }
+          y[ct][t][r] = __builtin_amdgcn_exp2f(x);
+          sum += y[ct][t][r];
+        }
+      l[ct] += __builtin_ldexpf(sum, -ev);
+    }
+  }
+
+  // probabilities in f16, in the order of the value codes' places
+  __device__ __forceinline__ static void pack(const float (&p)[2][4], unsigned (&w)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_f16(p[i >> 1][i & 1], p[i >> 1][2 + (i & 1)]);
+  }
+  // masks of the pairs of keys that column ct sees
+  __device__ __forceinline__ void seen_pairs(int ct, int key0, unsigned (&keep)[4]) const {
+    auto in = [&](int j) { return j >= span[ct].lo && j < span[ct].hi; };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = key0 + 16 * (i >> 1) + (i & 1);
+      keep[i] = (in(j) ? 0xFFFFu : 0u) | (in(j + 2) ? 0xFFFF0000u : 0u);
+    }
+  }
+  // P' = P * d of a pair of keys, in f16 parts
+  __device__ __forceinline__ static void weigh(float p0, float p1, f16x2 d, unsigned (&w)[PARTS][4], int i) {
+    const float y0 = p0 * static_cast<float>(d[0]), y1 = p1 * static_cast<float>(d[1]);
+    w[0][i] = pack_f16(y0, y1);
+    if constexpr (PREC) {
+      const f16x2 hi = as_f16x2(w[0][i]);
+      w[PARTS - 1][i] = pack_f16(y0 - static_cast<float>(hi[0]), y1 - static_cast<float>(hi[1]));
+    }
   }
 
   // A tile of 32 keys from key `first` on.  MASKED: some column does not see some of them; a key that a column does not
@@ -511,68 +580,24 @@ struct Columns {
       const unsigned lo = vs[i] & 0x7C00u, hi = vs[i] >> 16 & 0x7C00u, most = static_cast<unsigned>(21 - off) << 10;
       above |= (lo > most && lo != 0x7C00u) || (hi > most && hi != 0x7C00u);
     }
-    bool go = above;
+    int off_now = off;
+    if (__builtin_amdgcn_ballot_w64(above) != 0) {
+      unsigned e = 0;  // the largest finite scale's exponent field
+#pragma unroll
+      for (int i = 0; i < KvTile<NB, KF, VF>::SW; ++i) {
+        const unsigned lo = vs[i] >> 10 & 31, hi = vs[i] >> 26 & 31;
+        e = max(e, max(lo == 31 ? 0u : lo, hi == 31 ? 0u : hi));
+      }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) e = max(e, static_cast<unsigned>(__shfl_xor(static_cast<int>(e), o, 64)));
+      off_now = __builtin_amdgcn_readfirstlane(min(off, 21 - static_cast<int>(max(e, 1u))));
+    }
+    soften<MASKED>(a, key0, off_now, 0, y);
+    unsigned ph[CT][4], keep[CT][4];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      shape(a, ct, key0, y[ct]);
-      if constexpr (MASKED) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = key0 + 16 * t + r;
-            if (j < span[ct].lo || j >= span[ct].hi) y[ct][t][r] = NONE;
-          }
-      }
-      const float top = fmaxf(fmaxf(fmaxf(y[ct][0][0], y[ct][0][1]), fmaxf(y[ct][0][2], y[ct][0][3])),
-                              fmaxf(fmaxf(y[ct][1][0], y[ct][1][1]), fmaxf(y[ct][1][2], y[ct][1][3])));
-      go |= top > lim[ct];
-    }
-    if (__builtin_amdgcn_ballot_w64(go) != 0) {
-      int off_now = off;
-      if (__builtin_amdgcn_ballot_w64(above) != 0) {
-        unsigned e = 0;  // the largest finite scale's exponent field
-#pragma unroll
-        for (int i = 0; i < KvTile<NB, KF, VF>::SW; ++i) {
-          const unsigned lo = vs[i] >> 10 & 31, hi = vs[i] >> 26 & 31;
-          e = max(e, max(lo == 31 ? 0u : lo, hi == 31 ? 0u : hi));
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) e = max(e, static_cast<unsigned>(__shfl_xor(static_cast<int>(e), o, 64)));
-        off_now = __builtin_amdgcn_readfirstlane(min(off, 21 - static_cast<int>(max(e, 1u))));
-      }
-      move(off_now, y);
-    }
-    unsigned ph[CT][4];
-    unsigned keep[MASKED ? CT : 1][4];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float(&p)[2][4] = y[ct];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = fmaf(p[t][r], fx[ct], neg[ct]);
-          if constexpr (MASKED) {
-            const int j = key0 + 16 * t + r;
-            if (j < span[ct].lo || j >= span[ct].hi) x = NONE;
-          }
-          p[t][r] = __builtin_amdgcn_exp2f(x);
-          l[ct] += p[t][r];
-        }
-        if constexpr (MODE == KV_BF16) {
-          ph[ct][2 * t] = pack_f16(p[t][0], p[t][2]);
-          ph[ct][2 * t + 1] = pack_f16(p[t][1], p[t][3]);
-        }
-        if constexpr (MASKED) {
-          auto in = [&](int r) {
-            const int j = key0 + 16 * t + r;
-            return j >= span[ct].lo && j < span[ct].hi;
-          };
-          keep[ct][2 * t] = (in(0) ? 0xFFFFu : 0u) | (in(2) ? 0xFFFF0000u : 0u);
-          keep[ct][2 * t + 1] = (in(1) ? 0xFFFFu : 0u) | (in(3) ? 0xFFFF0000u : 0u);
-        }
-      }
+      if constexpr (MODE == KV_BF16) pack(y[ct], ph[ct]);
+      if constexpr (MASKED) seen_pairs(ct, key0, keep[ct]);
     }
     each<NB>([&](auto bc) {
       constexpr int b = bc.value;
@@ -585,13 +610,7 @@ struct Columns {
           if constexpr (MODE == KV_BF16) {
             w[ct][0][i] = __builtin_bit_cast(unsigned, as_f16x2(ph[ct][i]) * d);
           } else {
-            const float y0 = y[ct][i >> 1][i & 1] * static_cast<float>(d[0]);
-            const float y1 = y[ct][i >> 1][2 + (i & 1)] * static_cast<float>(d[1]);
-            w[ct][0][i] = pack_f16(y0, y1);
-            if constexpr (PREC) {
-              const f16x2 hi = as_f16x2(w[ct][0][i]);
-              w[ct][PARTS - 1][i] = pack_f16(y0 - static_cast<float>(hi[0]), y1 - static_cast<float>(hi[1]));
-            }
+            weigh(y[ct][i >> 1][i & 1], y[ct][i >> 1][2 + (i & 1)], d, w[ct], i);
           }
           if constexpr (MASKED) {
 #pragma unroll
@@ -660,7 +679,7 @@ struct Pages {
 // each in turn, with DEEP tiles in flight a wave; they join their sums in shared memory.
 template <int NB, int KF, int VF, int MODE, int CT>
 constexpr int kv_few_waves() {  // waves a SIMD that its registers leave room for
-  return NB == 8 || (NB == 4 && CT == 2) ? 1 : 2;
+  return NB == 8 || (NB == 4 && CT == 2) ? 1 : CT == 1 && NB == 2 ? 4 : CT == 1 && NB == 3 ? 3 : 2;
 }
 template <int NB, int KF, int VF, int MODE, int CT>
 __global__ void __launch_bounds__(kAttendWaves * 64, (kv_few_waves<NB, KF, VF, MODE, CT>())) kv_attend_few_kernel(const AttendArgs a) {
@@ -744,42 +763,6 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (kv_few_waves<NB, KF, VF, M
     cols.lim[ct] = M == Cols::NONE ? Cols::NONE : 0.f;
   }
   if (wave == 0) cols.store(a, s, h, col0, split, lane);
-}
-
-// WIDE_KERNEL
-
-// Run the kernel of `plan`: few columns or many.
-template <int NB, int KF, int VF, int MODE>
-hipError_t launch_attend_mode(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.splits) * static_cast<unsigned>(a.groups), static_cast<unsigned>(a.c.heads),
-                  static_cast<unsigned>(batch));
-  auto run = [&](auto kern, int threads) {
-    const Timing tm = timing_slot(KIND_PROBE);
-    if (tm.on) {
-      hipExtLaunchKernelGGL(kern, grid, dim3(threads), 0, stream, tm.start, tm.stop, 0, a);
-    } else {
-      hipLaunchKernelGGL(kern, grid, dim3(threads), 0, stream, a);
-    }
-    return hipGetLastError();
-  };
-  if (plan.ct == 1) return run(kv_attend_few_kernel<NB, KF, VF, MODE, 1>, kAttendWaves * 64);
-  return run(kv_attend_few_kernel<NB, KF, VF, MODE, 2>, kAttendWaves * 64);
-}
-template <int NB, int KF, int VF>
-hipError_t launch_attend_blocks(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream) {
-  if (a.type == KV_F32) return launch_attend_mode<NB, KF, VF, KV_F32>(a, plan, batch, stream);
-  if (a.type == KV_F16) return launch_attend_mode<NB, KF, VF, KV_F16>(a, plan, batch, stream);
-  return launch_attend_mode<NB, KF, VF, KV_BF16>(a, plan, batch, stream);
-}
-
-template <int KF, int VF>
-hipError_t launch_attend_format(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream) {
-  switch (a.c.dim) {
-    case 64: return launch_attend_blocks<2, KF, VF>(a, plan, batch, stream);
-    case 96: return launch_attend_blocks<3, KF, VF>(a, plan, batch, stream);
-    case 128: return launch_attend_blocks<4, KF, VF>(a, plan, batch, stream);
-    default: return launch_attend_blocks<8, KF, VF>(a, plan, batch, stream);
-  }
 }
 
 }  // namespace komp

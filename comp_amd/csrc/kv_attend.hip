@@ -13,12 +13,15 @@ AttendPlan plan_of(const KvAttendCall& c) {
   const int64_t cols = c.max_queries * group;
   const int64_t units = static_cast<int64_t>(c.batch) * c.cache.heads;
   AttendPlan p;
-  p.wide = false;
+  p.many = cols > 32;
   p.ct = cols <= 16 ? 1 : 2;
-  p.groups = static_cast<int>((cols + 16 * p.ct - 1) / (16 * p.ct));
-  const int64_t tiles = (c.max_length + 31) / 32;
-  const int64_t want = 1024 / (units * p.groups), most_splits = tiles / (2 * kAttendWaves);
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most_splits, kMaxSplits})));
+  const int wide = p.many ? many_cols(c.cache.dim, c.type) : 16 * p.ct;
+  p.groups = static_cast<int>((cols + wide - 1) / wide);
+  // enough workgroups to fill the CUs (one many-column workgroup each, two to four of the others), no split of less than
+  // two tiles a wave or four buffers
+  const int64_t want = (p.many ? 256 : 1024) / (units * p.groups);
+  const int64_t most = p.many ? c.max_length / 256 : (c.max_length + 31) / 32 / (2 * kAttendWaves);
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits})));
   return p;
 }
 

@@ -1,5 +1,5 @@
-// Attention over a cache of Q8_0 keys and Q8_0 values (kv_attend.h).
-#include "kv_attend.h"
+// Attention over a cache of Q8_0 keys and Q8_0 values (kv_attend.h, kv_many.h).
+#include "kv_launch.h"
 
 namespace komp {
 

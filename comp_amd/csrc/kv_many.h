@@ -1,0 +1,410 @@
+// Attention over the quantized key/value cache for many columns, as a prompt has: the keys and values are unpacked once
+// for all of a workgroup's columns (kv_attend.h has the mathematics and the columns' softmax).
+//
+// The waves of a workgroup have CT column tiles each and walk the same keys, which the workgroup unpacks into shared
+// memory as the f16 operands that the waves then read (16 bytes a lane, in lane order: no bank conflicts).  Two buffers of
+// KEYS keys, one barrier a buffer: while a wave computes with one, it unpacks its share of the next and has the codes
+// after that in flight.
+//
+// Key operands hold the codes, exact; their scales lie beside them and multiply the partial dots as in Columns::step.  So do
+// value operands for f16 and f32 queries.  For bf16 queries value operands hold d * code, rounded to f16 after a power of
+// two that brings the tile's largest scale to [1, 2) and that the probabilities' exponent takes back: 2^-12 of a value, an
+// eighth of what bf16 keeps of the result, for a quarter of the instructions a column.  A value block whose scale is no
+// number is held as zeros then, and makes NaN of its channels in the columns that see it.
+#pragma once
+
+#include "kv_attend.h"
+
+namespace komp {
+
+template <int NB, int KF, int VF, int MODE>
+struct Many {
+  // two column tiles a wave halve the operand reads and the unpacking a column, where the registers (of two waves a SIMD)
+  // hold their queries and sums: not f32 queries, in two parts, nor 256 channels
+  static constexpr bool PAIR = NB <= 4 && MODE != KV_F32;
+  static constexpr int CT = PAIR ? 2 : 1, WAVES = PAIR || NB == 8 ? 8 : 12, COLS = 16 * CT;
+  static constexpr int HALVES = NB == 8 ? 2 : PAIR ? 4 : 3, KEYS = 32 * HALVES;  // (a "half" is 32 keys: two key tiles)
+  static constexpr bool SCALED = MODE == KV_BF16;  // value operands
+  static constexpr int KB = kv_kb(NB, KF), VB = kv_vb(NB, VF);
+  static constexpr int KD = KB * kv_code_bytes(KF) / 16, VD = VB * kv_code_bytes(VF) / 8;  // code dwords of a lane's chunk
+  static constexpr int KG = NB / KB, VG = NB / VB;                                         // chunks a 16- or 32-token tile
+  static constexpr int KCHUNKS = KEYS / 16 * KG, VCHUNKS = HALVES * VG, CHUNKS = KCHUNKS + VCHUNKS;
+  static constexpr int TURNS = (CHUNKS + WAVES - 1) / WAVES;  // chunks of one wave
+  static constexpr int SW = (16 * NB + 63) / 64;              // dwords a lane of a half's scales, in a wave
+  using Cols = Columns<NB, KF, VF, MODE, CT, true>;
+  using Units = int64_t[HALVES];  // where the halves of a tile lie, -1 for nowhere
+
+  struct Shared {
+    f16x8 k[2][HALVES * 2 * NB][64];  // [16 tokens][block]
+    f16x8 v[2][HALVES * NB * 2][64];  // [32 tokens][block][channels 0..15, 16..31]
+    unsigned ks[2][HALVES][16 * NB];
+    unsigned vs[2][SCALED ? 1 : HALVES][16 * NB];
+    unsigned most[4];                          // of the values' scales: the largest exponent field
+    unsigned bad[4][SCALED ? 1 + HALVES * NB : 1];  // whether there are, and which, tokens of a half and block whose value
+                                                    // scale is no number
+  };
+  // a wave's chunks on their way from the cache to shared memory, and for the first waves the scales of a half
+  struct Chunk {
+    unsigned code[KD > VD ? KD : VD];
+    unsigned scale[SCALED ? 4 * VB : 1];
+  };
+  Chunk chunk[TURNS];
+  bool there[TURNS];
+  unsigned ks[SW], vs[SCALED ? 1 : SW];
+
+  static __device__ __forceinline__ int half_of(int c) { return c < KCHUNKS ? c / KG >> 1 : (c - KCHUNKS) / VG; }
+
+  __device__ __forceinline__ void load(const KvCache& cache, const Units& unit, int wave, int lane) {
+    auto of = [&](int half) {
+      int64_t u = unit[0];
+#pragma unroll
+      for (int j = 1; j < HALVES; ++j) u = half == j ? unit[j] : u;
+      return u;
+    };
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+      const int c = i * WAVES + wave;
+      const int64_t u = c < CHUNKS ? of(half_of(c)) : -1;
+      there[i] = u >= 0;
+      if (!there[i]) continue;
+      if (c < KCHUNKS) {
+        const int t16 = c / KG & 1, g = c % KG;
+        load_words<KD, KD>(cache.kq + u * (NB * 32 * kv_code_bytes(KF)) + t16 * (NB * 16 * kv_code_bytes(KF)) + (g * 64 + lane) * (KD * 4),
+                           chunk[i].code);
+      } else {
+        const int g = (c - KCHUNKS) % VG;
+        load_words<VD, VD>(cache.vq + u * (NB * 32 * kv_code_bytes(VF)) + (g * 64 + lane) * (VD * 4), chunk[i].code);
+        if constexpr (SCALED) {
+          const uint16_t* sp = cache.vs + u * (32 * NB) + ((lane >> 4) * NB + g * VB) * 8;
+          load_words<4 * VB, 4>(reinterpret_cast<const uint8_t*>(sp), chunk[i].scale);
+        }
+      }
+    }
+    if (wave < HALVES) {
+      const int64_t u = of(wave);
+#pragma unroll
+      for (int i = 0; i < SW; ++i) {
+        const int at = min(i * 64 + lane, 16 * NB - 1);
+        ks[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.ks)[u * (16 * NB) + at];
+        if constexpr (!SCALED) vs[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.vs)[u * (16 * NB) + at];
+      }
+    }
+  }
+
+  // the tokens of a pair of value scales, place i of a quarter's four: this one and the one 2 on
+  static __device__ __forceinline__ int value_token(int quarter, int i) { return 16 * (i >> 1 & 1) + 4 * quarter + (i & 1); }
+  static __device__ __forceinline__ unsigned value_mask(int quarter, int i, int left) {  // leaves those before `left`
+    const int token = value_token(quarter, i);
+    return (token < left ? 0xFFFFu : 0u) | (token + 2 < left ? 0xFFFF0000u : 0u);
+  }
+
+  // The loaded value scales: those of keys from `length` on become 0, and so do such as are no numbers, which go into
+  // bad[slot]; the largest exponent goes to most[slot].  (f16 and f32 queries: their products stay numbers by the masks.)
+  __device__ __forceinline__ void look(Shared& sh, int slot, int first, int length, int wave, int lane) {
+    unsigned e = 0;
+    if constexpr (SCALED) {
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        const int c = i * WAVES + wave;
+        if (c < KCHUNKS || !there[i]) continue;
+        const int left = length - first - half_of(c) * 32;
+        unsigned worst = 0;
+#pragma unroll
+        for (int j = 0; j < 4 * VB; ++j) {
+          if (left < 32) chunk[i].scale[j] &= value_mask(lane >> 4, j, left);
+          worst = max(worst, max(chunk[i].scale[j] & 0x7C00u, chunk[i].scale[j] >> 16 & 0x7C00u));
+        }
+        if (__builtin_amdgcn_ballot_w64(worst == 0x7C00u) != 0) {
+          worst = 0;
+#pragma unroll
+          for (int j = 0; j < 4 * VB; ++j) {
+            unsigned lo = chunk[i].scale[j] & 0xFFFFu, hi = chunk[i].scale[j] >> 16;
+            const unsigned token = value_token(lane >> 4, j & 3);
+            unsigned none = 0;
+            if ((lo & 0x7C00u) == 0x7C00u) none |= 1u << token, lo = 0;
+            if ((hi & 0x7C00u) == 0x7C00u) none |= 4u << token, hi = 0;
+            if (none && (lane & 15) == 0) {
+              atomicOr(&sh.bad[slot][1 + half_of(c) * NB + (c - KCHUNKS) % VG * VB + (j >> 2)], none);
+              sh.bad[slot][0] = 1;
+            }
+            chunk[i].scale[j] = lo | hi << 16;
+            worst = max(worst, max(lo & 0x7C00u, hi & 0x7C00u));
+          }
+        }
+        e = max(e, worst >> 10);
+      }
+    } else if (wave < HALVES) {
+#pragma unroll
+      for (int i = 0; i < SW; ++i) {
+        const int at = min(i * 64 + lane, 16 * NB - 1);
+        vs[i] &= value_mask(at / (4 * NB), at, length - first - wave * 32);
+        const unsigned lo = vs[i] >> 10 & 31, hi = vs[i] >> 26 & 31;
+        e = max(e, max(lo == 31 ? 0u : lo, hi == 31 ? 0u : hi));
+      }
+    }
+    int top = static_cast<int>(e);
+    if constexpr (!SCALED) top = row16_max_i(top);  // (value operands: a row's lanes have the same scales)
+    top = static_cast<int>(quarters_max(static_cast<float>(top)));
+    if (top && lane == 0) atomicMax(&sh.most[slot], static_cast<unsigned>(top));
+  }
+
+  // the loaded codes as operands in buffer `buf`
+  __device__ __forceinline__ void unpack(Shared& sh, int buf, int slot, int wave, int lane) {
+    f16x2 fv = {};
+    if constexpr (SCALED) {  // 2^(15 - field)
+      const _Float16 v = static_cast<_Float16>(__builtin_ldexpf(1.f, 15 - static_cast<int>(max(sh.most[slot], 1u))));
+      fv = f16x2{v, v};
+    }
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+      const int c = i * WAVES + wave;
+      if (!there[i]) continue;
+      if (c < KCHUNKS) {
+        f16x8* to = &sh.k[buf][c / KG * NB + c % KG * KB][lane];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          if constexpr (KF == KV_Q4_0) to[b * 64] = key_codes<true, KF>(chunk[i].code[b], 0u);
+          else to[b * 64] = key_codes<true, KF>(chunk[i].code[2 * b], chunk[i].code[2 * b + 1]);
+        }
+      } else {
+        f16x8* to = &sh.v[buf][(c - KCHUNKS) * VB * 2][lane];
+#pragma unroll
+        for (int b = 0; b < VB; ++b) {
+          u32x4 d;
+          if constexpr (SCALED) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j] = __builtin_bit_cast(unsigned, as_f16x2(chunk[i].scale[4 * b + j]) * fv);
+          }
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            f16x8 x;
+            if constexpr (VF == KV_Q4_0) x = value_codes<VF>(chunk[i].code[2 * b], chunk[i].code[2 * b + 1], hh);
+            else x = value_codes<VF>(chunk[i].code[4 * b + 2 * hh], chunk[i].code[4 * b + 2 * hh + 1], 0);
+            if constexpr (SCALED) x *= __builtin_bit_cast(f16x8, d);
+            to[(b * 2 + hh) * 64] = x;
+          }
+        }
+      }
+    }
+    if (wave < HALVES) {
+#pragma unroll
+      for (int i = 0; i < SW; ++i) {
+        const int at = min(i * 64 + lane, 16 * NB - 1);
+        sh.ks[buf][wave][at] = ks[i];
+        if constexpr (!SCALED) sh.vs[buf][wave][at] = vs[i];
+      }
+    }
+  }
+
+  // a wave's columns over half `half` of the tile in `buf`, its keys from `first` on
+  template <bool MASKED>
+  static __device__ __forceinline__ void step(Cols& cols, const AttendArgs& a, const Shared& sh, int buf, int slot, int half,
+                                              int first, int lane) {
+    constexpr int ROWS = (4 * NB + 15) / 16;  // a quarter's scales: dwords a lane of its 16
+    const int quarter = lane >> 4, key0 = first + quarter * 4;
+    const int e = __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot], 1u)));
+    unsigned ks[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int at = min(i * 16 + (lane & 15), 4 * NB - 1), t = at / (2 * NB);
+      ks[i] = sh.ks[buf][half][t * 8 * NB + quarter * 2 * NB + at - t * 2 * NB];
+    }
+    float y[CT][2][4];
+    each<2>([&](auto tc) {
+      constexpr int t = tc.value;
+      f32x4 c[CT][NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const f16x8 k = sh.k[buf][(half * 2 + t) * NB + b][lane];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          c[ct][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = 0; p < Cols::PARTS; ++p) c[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, cols.qf[ct][b][p], c[ct][b], 0, 0, 0);
+        }
+      }
+      each<2 * NB>([&](auto jc) {
+        constexpr int j = jc.value, at = t * 2 * NB + j;
+        const f16x2 d = as_f16x2(row_lane<at % 16>(ks[at / 16]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = (2 * j + h) / NB, b = (2 * j + h) % NB;
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            y[ct][t][r] = b == 0 ? static_cast<float>(d[h]) * c[ct][b][r] : fmaf(static_cast<float>(d[h]), c[ct][b][r], y[ct][t][r]);
+        }
+      });
+    });
+    cols.template soften<MASKED>(a, key0, min(cols.off, 21 - e), SCALED ? e - 15 : 0, y);
+    if constexpr (SCALED) {
+      unsigned w[CT][4];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) Cols::pack(y[ct], w[ct]);
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) {
+        const f16x8 v = sh.v[buf][half * NB * 2 + i][lane];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          cols.acc[ct][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, as_f16x8(w[ct][0], w[ct][1], w[ct][2], w[ct][3]),
+                                                                  cols.acc[ct][i], 0, 0, 0);
+      }
+    } else {
+      unsigned vs[ROWS], keep[CT][4];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) vs[i] = sh.vs[buf][half][quarter * 4 * NB + min(i * 16 + (lane & 15), 4 * NB - 1)];
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) cols.seen_pairs(ct, key0, keep[ct]);
+      }
+      each<NB>([&](auto bc) {
+        constexpr int b = bc.value;
+        unsigned w[CT][Cols::PARTS][4];
+        each<4>([&](auto ic) {
+          constexpr int i = ic.value, at = 4 * b + i;
+          const f16x2 d = as_f16x2(row_lane<at % 16>(vs[at / 16]));
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            Cols::weigh(y[ct][i >> 1][i & 1], y[ct][i >> 1][2 + (i & 1)], d, w[ct], i);
+            if constexpr (MASKED) {
+#pragma unroll
+              for (int p = 0; p < Cols::PARTS; ++p) w[ct][p][i] &= keep[ct][i];
+            }
+          }
+        });
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const f16x8 v = sh.v[buf][(half * NB + b) * 2 + hh][lane];
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int p = 0; p < Cols::PARTS; ++p)
+              cols.acc[ct][2 * b + hh] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  v, as_f16x8(w[ct][p][0], w[ct][p][1], w[ct][p][2], w[ct][p][3]), cols.acc[ct][2 * b + hh], 0, 0, 0);
+        }
+      });
+    }
+  }
+
+  // the channels of blocks without a scale, in the columns that see their tokens
+  static __device__ __forceinline__ void spoil(Cols& cols, const Shared& sh, int slot, int half, int first) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int lo = max(0, cols.span[ct].lo - first), hi = min(32, cols.span[ct].hi - first);
+      const unsigned seen = lo >= hi ? 0u : (hi == 32 ? ~0u : (1u << hi) - 1) & ~((1u << lo) - 1);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const bool to = (sh.bad[slot][SCALED ? 1 + half * NB + b : 0] & seen) != 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          cols.acc[ct][2 * b][r] = to ? __builtin_nanf("") : cols.acc[ct][2 * b][r];
+          cols.acc[ct][2 * b + 1][r] = to ? __builtin_nanf("") : cols.acc[ct][2 * b + 1][r];
+        }
+      }
+    }
+  }
+};
+
+template <int NB, int KF, int VF, int MODE>
+__global__ void __launch_bounds__((64 * Many<NB, KF, VF, MODE>::WAVES), (Many<NB, KF, VF, MODE>::WAVES / 4)) kv_attend_many_kernel(const AttendArgs a) {
+  using M = Many<NB, KF, VF, MODE>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char shared_bytes[];
+  typename M::Shared& sh = *reinterpret_cast<typename M::Shared*>(shared_bytes);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.x, seq = blockIdx.y, split = blockIdx.z / a.groups;
+  // the groups of the latest positions, which see the most keys, begin first, those of all heads and sequences together
+  const int group0 = (a.groups - 1 - (static_cast<int>(blockIdx.z) - split * a.groups)) * (M::WAVES * M::COLS);
+  const Sequence s(a, seq);
+  if (group0 >= s.cols) return;
+  const Span g0 = s.seen(a, group0 / a.group), g1 = s.seen(a, (min(s.cols, group0 + M::WAVES * M::COLS) - 1) / a.group);
+  int tile0 = g0.lo / M::KEYS, tile1 = (g1.hi + M::KEYS - 1) / M::KEYS;
+  if (tile0 > tile1) tile0 = tile1 = 0;
+  const int per = (tile1 - tile0 + a.splits - 1) / a.splits;
+  tile0 = min(tile1, tile0 + split * per);
+  tile1 = min(tile1, tile0 + per);
+
+  // the wave's own columns: what they see, and what all of them see
+  const int col0 = group0 + wave * M::COLS;
+  const bool any = col0 < s.cols;
+  const Span w0 = s.seen(a, any ? col0 / a.group : 0), w1 = s.seen(a, any ? (min(s.cols, col0 + M::COLS) - 1) / a.group : 0);
+
+  const Pages pages(a, seq, h);
+  auto units = [&](int tile, typename M::Units& u) {  // -> a bit for each half that lies somewhere
+    unsigned there = 0;
+#pragma unroll
+    for (int i = 0; i < M::HALVES; ++i) {
+      const int at = tile * M::HALVES + i;
+      u[i] = tile < tile1 && at * 32 < s.length ? pages.unit(at) : -1;
+      there |= u[i] < 0 ? 0u : 1u << i;
+    }
+    return there;
+  };
+  M m;
+  typename M::Units unit;
+  if (threadIdx.x < 4) sh.most[threadIdx.x] = 0;
+  constexpr int BAD = M::SCALED ? 1 + M::HALVES * NB : 0;
+  if (threadIdx.x < 4 * BAD) (&sh.bad[0][0])[threadIdx.x] = 0;
+  unsigned now = units(tile0, unit);
+  m.load(a.c, unit, wave, lane);
+  typename M::Cols cols;
+  cols.all = Span{w0.lo, w1.hi};
+  cols.begin(a, s, h, col0, lane);
+  __syncthreads();
+  m.look(sh, 0, tile0 * M::KEYS, s.length, wave, lane);
+  __syncthreads();
+  m.unpack(sh, 0, 0, wave, lane);
+  unsigned next = units(tile0 + 1, unit);
+  m.load(a.c, unit, wave, lane);
+  m.look(sh, 1, (tile0 + 1) * M::KEYS, s.length, wave, lane);
+  __syncthreads();
+  for (int tile = tile0; tile < tile1; ++tile) {
+    // most[] and bad[]: this tile's are in slot i, the next one's in i + 1, the one after's are filled in i + 2, and i + 3,
+    // last read a turn ago, is cleared for the turn to come
+    const int i = tile - tile0, buf = i & 1;
+    if (threadIdx.x == 0) sh.most[(i + 3) & 3] = 0;
+    if (threadIdx.x < BAD) sh.bad[(i + 3) & 3][threadIdx.x] = 0;
+    m.unpack(sh, buf ^ 1, (i + 1) & 3, wave, lane);
+    const unsigned after = units(tile + 2, unit);
+    m.load(a.c, unit, wave, lane);
+    const bool spoilt = M::SCALED && __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) != 0;
+#pragma unroll 1
+    for (int half = 0; half < M::HALVES; ++half) {
+      const int first = tile * M::KEYS + half * 32;
+      if (!any || first >= w1.hi || first + 32 <= w0.lo || !(now >> half & 1)) continue;
+      if (first >= w1.lo && first + 32 <= w0.hi)
+        M::template step<false>(cols, a, sh, buf, i & 3, half, first, lane);
+      else
+        M::template step<true>(cols, a, sh, buf, i & 3, half, first, lane);
+    }
+    if (spoilt) {
+#pragma unroll 1
+      for (int half = 0; half < M::HALVES; ++half)
+        if (any && (now >> half & 1)) M::spoil(cols, sh, i & 3, half, tile * M::KEYS + half * 32);
+    }
+    m.look(sh, (i + 2) & 3, (tile + 2) * M::KEYS, s.length, wave, lane);
+    now = next;
+    next = after;
+    __syncthreads();
+  }
+  if (!any) return;
+#pragma unroll
+  for (int ct = 0; ct < M::CT; ++ct) cols.l[ct] = quarters_sum(cols.l[ct]);
+  cols.store(a, s, h, col0, split, lane);
+}
+
+template <int NB, int KF, int VF, int MODE>
+hipError_t launch_attend_many(const AttendArgs& a, const dim3& grid, hipStream_t stream) {
+  static std::atomic<unsigned> limit[kMaxDevices];
+  const auto kern = kv_attend_many_kernel<NB, KF, VF, MODE>;
+  constexpr size_t bytes = sizeof(typename Many<NB, KF, VF, MODE>::Shared);
+  const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), bytes, limit);
+  if (e != hipSuccess) return e;
+  const Timing tm = timing_slot(KIND_PROBE);
+  if (tm.on) {
+    hipExtLaunchKernelGGL(kern, grid, dim3(64 * Many<NB, KF, VF, MODE>::WAVES), bytes, stream, tm.start, tm.stop, 0, a);
+  } else {
+    hipLaunchKernelGGL(kern, grid, dim3(64 * Many<NB, KF, VF, MODE>::WAVES), bytes, stream, a);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace komp
