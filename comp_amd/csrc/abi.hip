@@ -1208,9 +1208,9 @@ int kv_type_of(const char* name, int type, int& size) {
   return KOMP_OK;
 }
 
-// tokens of one call: 32-bit workgroup numbers (256 lanes of 4 values)
+// tokens of one call: 2^30 threads a launch at most, 8 for each block of 32 values, in groups of 4 tokens or more
 int kv_tokens(const char* name, const KvCache& c, int64_t T) {
-  if (T < 0 || T > (INT64_C(1) << 38) / (static_cast<int64_t>(c.heads) * c.dim / 4))
+  if (T < 0 || T > (INT64_C(1) << 30) / (static_cast<int64_t>(c.heads) * c.dim / 4))
     return fail(KOMP_EINVAL, "%s: T=%lld tokens", name, static_cast<long long>(T));
   return KOMP_OK;
 }

@@ -67,10 +67,9 @@ struct AttendArgs {
   float2* part_m;  // [split][row][head]: M and l
 };
 
-// many: the kernel of kv_many.h; else ct column tiles of 16 a workgroup.  Column groups a sequence, splits of its keys
+// many: the kernel of kv_many.h; else 16 columns a workgroup.  Column groups a sequence, splits of its keys
 struct AttendPlan {
   bool many;
-  int ct;
   int groups;
   int splits;
 };
@@ -314,7 +313,7 @@ struct Sequence {
 
 // A wave's columns and their softmax: queries, references and sums.  MODE: the type of the queries.  SIGNED: how it takes
 // key codes.
-template <int NB, int KF, int VF, int MODE, int CT, bool SIGNED = (CT > 1 || MODE == KV_F32)>
+template <int NB, int KF, int VF, int MODE, int CT, bool SIGNED>
 struct Columns {
   static constexpr int COLS = 16 * CT;
   static constexpr bool PREC = MODE == KV_F32;
@@ -675,16 +674,19 @@ struct Pages {
   }
 };
 
-// Few columns over many keys: the waves of a workgroup have the same columns and share its keys out among them, a tile
-// each in turn, with DEEP tiles in flight a wave; they join their sums in shared memory.
-template <int NB, int KF, int VF, int MODE, int CT>
-constexpr int kv_few_waves() {  // waves a SIMD that its registers leave room for
-  return NB == 8 || (NB == 4 && CT == 2) ? 1 : CT == 1 && NB == 2 ? 4 : CT == 1 && NB == 3 ? 3 : 2;
-}
-template <int NB, int KF, int VF, int MODE, int CT>
-__global__ void __launch_bounds__(kAttendWaves * 64, (kv_few_waves<NB, KF, VF, MODE, CT>())) kv_attend_few_kernel(const AttendArgs a) {
-  constexpr int W = kAttendWaves, DEEP = 2;
-  using Cols = Columns<NB, KF, VF, MODE, CT>;
+// Few columns over many keys: the waves of a workgroup have the same 16 columns and share its keys out among them, a tile
+// each in turn; they join their sums in shared memory.  Registers decide how it hides the memory's latency: 3 waves a SIMD
+// (4 of 64 channels, 2 of 256, or 1 with f32 queries) with one tile in flight each, or for 8-bit tiles, twice as large, 2 waves with two.
+template <int NB, int KF, int VF, int MODE>
+struct Few {
+  static constexpr int DEEP = KF == KV_Q8_0 && VF == KV_Q8_0 && NB <= 4 ? 2 : 1;
+  static constexpr int WAVES = NB == 2 ? 4 : NB == 8 ? (MODE == KV_F32 ? 1 : 2) : NB == 4 && DEEP == 2 ? 2 : 3;  // a SIMD
+  static constexpr bool SIGNED = NB == 8;  // (the subnormals' accumulators would take 32 registers)
+};
+template <int NB, int KF, int VF, int MODE>
+__global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAVES)) kv_attend_few_kernel(const AttendArgs a) {
+  constexpr int W = kAttendWaves, DEEP = Few<NB, KF, VF, MODE>::DEEP, CT = 1;
+  using Cols = Columns<NB, KF, VF, MODE, CT, (Few<NB, KF, VF, MODE>::SIGNED || MODE == KV_F32)>;
   constexpr int COLS = Cols::COLS, OT = Cols::OT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.y, seq = blockIdx.z, split = blockIdx.x / a.groups, col0 = (blockIdx.x - split * a.groups) * COLS;

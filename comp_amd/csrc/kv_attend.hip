@@ -14,50 +14,57 @@ AttendPlan plan_of(const KvAttendCall& c) {
   const int64_t units = static_cast<int64_t>(c.batch) * c.cache.heads;
   AttendPlan p;
   p.many = cols > 32;
-  p.ct = cols <= 16 ? 1 : 2;
-  const int wide = p.many ? many_cols(c.cache.dim, c.type) : 16 * p.ct;
+  const int wide = p.many ? many_cols(c.cache.dim, c.type) : 16;
   p.groups = static_cast<int>((cols + wide - 1) / wide);
-  // enough workgroups to fill the CUs (one many-column workgroup each, two to four of the others), no split of less than
-  // two tiles a wave or four buffers
-  const int64_t want = (p.many ? 256 : 1024) / (units * p.groups);
+  // Enough workgroups to fill the CUs (one of many columns each, four of the others), eight where unlike lengths have to
+  // even out (64 sequences of up to 8192 keys, 8 kv heads, bf16: 106 us with 1024 workgroups, 97 with 2048, 103 with
+  // 4096), and no split of less than two tiles a wave or two buffers.
+  const int64_t aim = p.many ? 256 : units * p.groups >= 256 ? 2048 : 1024;
+  const int64_t want = (aim + units * p.groups - 1) / (units * p.groups);
   const int64_t most = p.many ? c.max_length / 256 : (c.max_length + 31) / 32 / (2 * kAttendWaves);
   p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits})));
   return p;
 }
 
-// One wave a row and head: the splits' sums, brought to the largest of their references.  D / 4 lanes hold a split's
-// channels, 64 / (D / 4) splits at a time.
+// One workgroup a row and head: the splits' sums, brought to the largest of their references.  A wave takes every fourth
+// split, D / 4 lanes a split; their sums meet in shared memory.
 template <int D>
 __global__ void __launch_bounds__(256) kv_attend_join_kernel(const AttendArgs a) {
-  constexpr int LANES = D / 4, PAR = 64 / LANES;
-  const int lane = threadIdx.x & 63;
-  const int64_t n = a.rows * a.heads, at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (at >= n) return;
+  constexpr int LANES = D / 4, PAR = 64 / LANES;  // lanes a split, splits a wave at a time
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n = a.rows * a.heads, at = blockIdx.x;
   float2 m = float2{-__builtin_inff(), 0.f};
   if (lane < a.splits) m = a.part_m[lane * n + at];
+  const int part = lane / LANES, ch = lane - part * LANES;
+  // every split's sums are loaded before its reference is known (kMaxSplits / 4 / PAR loads at most, all in flight)
+  constexpr int MOST = kMaxSplits / 4 / PAR;
+  f32x4 x[MOST];
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    const int s = (i * 4 + wave) * PAR + part;
+    x[i] = part < PAR && s < a.splits ? *reinterpret_cast<const f32x4*>(a.part_o + (s * n + at) * D + ch * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   float top = m.x;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   const float f = m.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m.x - top);
   const float l = group_sum(f * m.y, 64);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  const int part = lane / LANES, ch = lane - part * LANES;
-  for (int s0 = 0; s0 < a.splits; s0 += PAR) {
-    const int s = s0 + part;
-    const float fs = __shfl(f, s < a.splits ? s : 0, 64);
-    const float ms = __shfl(m.x, s < a.splits ? s : 0, 64);
-    if (part < PAR && s < a.splits && ms != -__builtin_inff())
-      o += fs * *reinterpret_cast<const f32x4*>(a.part_o + (s * n + at) * D + ch * 4);
-  }
 #pragma unroll
-  for (int p = 1; p < PAR; ++p) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float other = __shfl(o[e], (p * LANES + ch) & 63, 64);
-      if (part == 0) o[e] += other;
-    }
+  for (int i = 0; i < MOST; ++i) {
+    const int s = (i * 4 + wave) * PAR + part;
+    const float fs = __shfl(f, s & 63, 64), ms = __shfl(m.x, s & 63, 64);
+    if (ms != -__builtin_inff()) o += fs * x[i];  // (a split that saw nothing has stored no sums)
   }
-  if (part == 0) {
+  __shared__ f32x4 sum[4][64];
+  sum[wave][lane] = o;
+  __syncthreads();
+  if (threadIdx.x < LANES) {
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int p = 0; p < PAR; ++p) o += sum[w][p * LANES + threadIdx.x];
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t row = at / a.heads;
     const int head = static_cast<int>(at - row * a.heads);
@@ -119,7 +126,7 @@ hipError_t launch_kv_attend(const KvAttendCall& c, hipStream_t stream) {
   else if (c.cache.vf == KV_Q4_0) e = launch_attend_q8_q4(a, p, c.batch, stream);
   else e = launch_attend_q8_q8(a, p, c.batch, stream);
   if (e != hipSuccess || p.splits == 1) return e;
-  const dim3 grid(static_cast<unsigned>((c.rows * c.heads + 3) / 4));
+  const dim3 grid(static_cast<unsigned>(c.rows * c.heads));
   auto run = [&](auto kern) {
     const Timing tm = timing_slot(KIND_PROBE);
     if (tm.on) {

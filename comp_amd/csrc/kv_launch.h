@@ -21,8 +21,7 @@ hipError_t launch_attend_mode(const AttendArgs& a, const AttendPlan& plan, int b
     return hipGetLastError();
   };
   if (plan.many) return launch_attend_many<NB, KF, VF, MODE>(a, dim3(grid.y, grid.z, grid.x), stream);
-  if (plan.ct == 1) return run(kv_attend_few_kernel<NB, KF, VF, MODE, 1>, kAttendWaves * 64);
-  return run(kv_attend_few_kernel<NB, KF, VF, MODE, 2>, kAttendWaves * 64);
+  return run(kv_attend_few_kernel<NB, KF, VF, MODE>, kAttendWaves * 64);
 }
 template <int NB, int KF, int VF>
 hipError_t launch_attend_blocks(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream) {

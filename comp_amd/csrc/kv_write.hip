@@ -14,7 +14,7 @@
 namespace komp {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kGroups = kThreads / 8;
 
 struct WriteArgs {
   KvCache c;
@@ -22,7 +22,7 @@ struct WriteArgs {
   int64_t stride_t[2];
   int64_t stride_h[2];
   const int64_t* slots;
-  int64_t lanes;  // tokens * heads * blocks * 8
+  int64_t tokens;
   bool wide[2];   // four elements of a row may be loaded at once
 };
 
@@ -30,7 +30,7 @@ struct ReadArgs {
   KvCache c;
   void* x[2];
   const int64_t* slots;
-  int64_t lanes;
+  int64_t tokens;
 };
 
 template <int TYPE>
@@ -104,54 +104,207 @@ __device__ __forceinline__ unsigned quantize8(f32x4 v, int lane8, uint16_t& scal
   return packed;
 }
 
-// where the page and head of a slot begin, in units of 32 tokens * blocks (times bytes of each plane)
-__device__ __forceinline__ int64_t unit_of(const KvCache& c, int64_t slot, int h) {
-  const int64_t page = slot >> c.page_log2;
-  const int tile = static_cast<int>(slot & (c.page - 1)) >> 5;
-  return (page * c.heads + h) * (c.page >> 5) + tile;
+// where a tile of 32 tokens of a page and head lies, in units of such tiles
+__device__ __forceinline__ int64_t unit_of(const KvCache& c, int64_t tile, int h) {
+  const int log2 = c.page_log2 - 5;
+  return (((tile >> log2) * c.heads + h) << log2) + (tile & ((int64_t{1} << log2) - 1));
 }
 
-// Eight lanes a block; a token's slot decides where its codes go.  Only this token's bytes are written, so tokens of
-// any slots may be written together.
-template <int KF, int VF, int NB, int TYPE>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
-  const int64_t gid = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (gid >= a.lanes) return;  // in groups of 8 lanes
-  const int lane8 = static_cast<int>(gid & 7);
-  const int64_t blk = gid >> 3;
-  const int b = static_cast<int>(blk % NB);
-  const int64_t th = blk / NB;
-  const int64_t t = th / a.c.heads;
-  const int h = static_cast<int>(th - t * a.c.heads);
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >= a.c.pages << a.c.page_log2) return;
-  const int64_t unit = unit_of(a.c, slot, h);
-  const int token32 = static_cast<int>(slot & 31), token16 = token32 & 15;
-  uint16_t scale;
-  if (blockIdx.y == 0) {
-    const f32x4 v = load4<TYPE>(a.x[0], t * a.stride_t[0] + h * a.stride_h[0] + b * 32 + lane8 * 4, a.wide[0]);
-    const unsigned q = quantize8<KF>(v, lane8, scale);
-    const int64_t tile = unit * 2 + (token32 >> 4);  // 16 tokens
-    const int dword = kv_k_dword(NB, KF, token16, b, lane8 >> 1, lane8 & 1);
-    if constexpr (KF == KV_Q8_0) {
-      reinterpret_cast<unsigned*>(a.c.kq)[tile * (128 * NB) + dword] = q;
+// A block's codes, four of eight lanes each, into the 32-token tile at `codes` and `scales` (global or shared memory).
+// Only this token's bytes are written.
+template <int FMT, int NB, bool VALUE>
+__device__ __forceinline__ void put(uint8_t* codes, uint16_t* scales, int token32, int b, int lane8, unsigned q, uint16_t scale) {
+  const int token16 = token32 & 15;
+  if constexpr (!VALUE) {
+    uint8_t* tile = codes + (token32 >> 4) * (16 * NB * kv_code_bytes(FMT));
+    const int dword = kv_k_dword(NB, FMT, token16, b, lane8 >> 1, lane8 & 1);
+    if constexpr (FMT == KV_Q8_0) {
+      reinterpret_cast<unsigned*>(tile)[dword] = q;
     } else {
       const unsigned n = (q & 15) | (q >> 4 & 0xF0) | (q >> 8 & 0xF00) | (q >> 12 & 0xF000);
-      reinterpret_cast<uint16_t*>(a.c.kq)[(tile * (64 * NB) + dword) * 2 + (lane8 & 1)] = static_cast<uint16_t>(n);
+      reinterpret_cast<uint16_t*>(tile)[dword * 2 + (lane8 & 1)] = static_cast<uint16_t>(n);
     }
-    if (lane8 == 0) a.c.ks[tile * (16 * NB) + kv_k_scale(NB, token16, b)] = scale;
+    if (lane8 == 0) scales[(token32 >> 4) * (16 * NB) + kv_k_scale(NB, token16, b)] = scale;
   } else {
-    const f32x4 v = load4<TYPE>(a.x[1], t * a.stride_t[1] + h * a.stride_h[1] + b * 32 + lane8 * 4, a.wide[1]);
-    unsigned q = quantize8<VF>(v, lane8, scale);
-    uint8_t* base = a.c.vq + unit * (32 * NB * kv_code_bytes(VF));
-    const int channel = (lane8 & 3) * 4;
-    if constexpr (VF == KV_Q4_0) q |= __shfl_xor(static_cast<int>(q), 4, 64) << 4;  // used by lanes 0..3: channels + 16
-    if (VF == KV_Q8_0 || lane8 < 4) {
+    if constexpr (FMT == KV_Q4_0) q |= __shfl_xor(static_cast<int>(q), 4, 64) << 4;  // used by lanes 0..3: channels + 16
+    if (FMT == KV_Q8_0 || lane8 < 4) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        base[kv_v_byte(NB, VF, token32, b, channel + e, lane8 >> 2)] = static_cast<uint8_t>(q >> (8 * e));
+        codes[kv_v_byte(NB, FMT, token32, b, (lane8 & 3) * 4 + e, lane8 >> 2)] = static_cast<uint8_t>(q >> (8 * e));
     }
-    if (lane8 == 0) a.c.vs[unit * (32 * NB) + kv_v_scale(NB, token32, b)] = scale;
+    if (lane8 == 0) scales[kv_v_scale(NB, token32, b)] = scale;
+  }
+}
+
+// the four values of a lane of eight
+template <int FMT, int NB, bool VALUE>
+__device__ __forceinline__ f32x4 get(const uint8_t* codes, const uint16_t* scales, int token32, int b, int lane8) {
+  const int token16 = token32 & 15;
+  uint16_t scale;
+  int q[4];
+  if constexpr (!VALUE) {
+    const uint8_t* tile = codes + (token32 >> 4) * (16 * NB * kv_code_bytes(FMT));
+    const int dword = kv_k_dword(NB, FMT, token16, b, lane8 >> 1, lane8 & 1);
+    scale = scales[(token32 >> 4) * (16 * NB) + kv_k_scale(NB, token16, b)];
+    if constexpr (FMT == KV_Q8_0) {
+      const unsigned w = reinterpret_cast<const unsigned*>(tile)[dword];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = static_cast<int>(w >> (8 * e) & 255) - 128;
+    } else {
+      const unsigned w = reinterpret_cast<const uint16_t*>(tile)[dword * 2 + (lane8 & 1)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = static_cast<int>(w >> (4 * e) & 15) - 8;
+    }
+  } else {
+    scale = scales[kv_v_scale(NB, token32, b)];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int w = codes[kv_v_byte(NB, FMT, token32, b, (lane8 & 3) * 4 + e, lane8 >> 2)];
+      q[e] = FMT == KV_Q8_0 ? w - 128 : (lane8 < 4 ? w & 15 : w >> 4) - 8;
+    }
+  }
+  const float d = f16_bits_to_f32(static_cast<int16_t>(scale));
+  return f32x4{q[0] * d, q[1] * d, q[2] * d, q[3] * d};
+}
+
+// keys or values of a cache
+struct Plane {
+  uint8_t* codes;
+  uint16_t* scales;
+};
+template <bool VALUE>
+__device__ __forceinline__ Plane plane_of(const KvCache& c) {
+  return VALUE ? Plane{c.vq, c.vs} : Plane{c.kq, c.ks};
+}
+template <int FMT, int NB>
+__device__ __forceinline__ Plane at_unit(const Plane& p, int64_t unit) {
+  return Plane{p.codes + unit * (32 * NB * kv_code_bytes(FMT)), p.scales + unit * (32 * NB)};
+}
+
+// Few tokens: eight lanes a block, a workgroup's blocks those of `tokens` tokens of one head.
+template <int FMT, int NB, int TYPE, bool VALUE>
+__device__ __forceinline__ void write_few(const WriteArgs& a) {
+  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.y;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kGroups / NB) + group / NB;
+  const int b = group % NB;
+  if (group >= kGroups / NB * NB || t >= a.tokens) return;  // in groups of 8 lanes
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= a.c.pages << a.c.page_log2) return;
+  const f32x4 v = load4<TYPE>(a.x[VALUE], t * a.stride_t[VALUE] + h * a.stride_h[VALUE] + b * 32 + lane8 * 4, a.wide[VALUE]);
+  uint16_t scale;
+  const unsigned q = quantize8<FMT>(v, lane8, scale);
+  const Plane p = at_unit<FMT, NB>(plane_of<VALUE>(a.c), unit_of(a.c, slot >> 5, h));
+  put<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8, q, scale);
+}
+
+// Many tokens: a workgroup has 32 tokens of the list and one head.  Consecutive slots fall into two tiles of 32 at most,
+// which it puts together in shared memory and stores by dwords where all the tokens of a dword are its own (four for value
+// codes, two for their scales); tokens of further tiles go one by one.
+template <int FMT, int NB>
+struct Tiles {
+  static constexpr int CODES = 32 * NB * kv_code_bytes(FMT), SCALES = 32 * NB;
+  uint8_t codes[2][CODES];
+  uint16_t scales[2][SCALES];
+  int64_t slot[32];
+  unsigned mask[2];  // tokens of the tiles that are written or read here
+};
+// Fills slot[] and mask[] and finds the two tiles, the first and the last valid slot's; -1 for none.
+template <int FMT, int NB>
+__device__ __forceinline__ void find_tiles(const KvCache& c, const int64_t* slots, int64_t tokens, Tiles<FMT, NB>& sh, int64_t (&tile)[2]) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 32 + (lane & 31);
+  int64_t slot = t < tokens ? slots[t] : -1;
+  if (slot < 0 || slot >= c.pages << c.page_log2) slot = -1;
+  const unsigned there = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(slot >= 0 && lane < 32));
+  tile[0] = tile[1] = -1;
+  if (there) {
+    const int64_t own = slot >> 5;
+    tile[0] = __shfl(own, __builtin_ctz(there), 64);
+    tile[1] = __shfl(own, 31 - __builtin_clz(there), 64);
+    if (tile[1] == tile[0]) tile[1] = -1;
+  }
+  if (threadIdx.x < 2) sh.mask[threadIdx.x] = 0;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    sh.slot[threadIdx.x] = slot;
+    if (slot >= 0 && (slot >> 5) == tile[0]) atomicOr(&sh.mask[0], 1u << (slot & 31));
+    if (slot >= 0 && (slot >> 5) == tile[1]) atomicOr(&sh.mask[1], 1u << (slot & 31));
+  }
+  __syncthreads();
+}
+
+template <int FMT, int NB, int TYPE, bool VALUE>
+__device__ __forceinline__ void write_many(const WriteArgs& a, Tiles<FMT, NB>& sh) {
+  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.y;
+  int64_t tile[2];
+  find_tiles(a.c, a.slots, a.tokens, sh, tile);
+  const Plane plane = plane_of<VALUE>(a.c);
+  // all loads first: a token left out loads nothing
+  f32x4 v[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const int token = (i * kGroups + group) / NB, b = (i * kGroups + group) % NB;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 32 + token;
+    v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (sh.slot[token] >= 0)
+      v[i] = load4<TYPE>(a.x[VALUE], t * a.stride_t[VALUE] + h * a.stride_h[VALUE] + b * 32 + lane8 * 4, a.wide[VALUE]);
+  }
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const int token = (i * kGroups + group) / NB, b = (i * kGroups + group) % NB;
+    const int64_t slot = sh.slot[token];
+    uint16_t scale;
+    const unsigned q = quantize8<FMT>(v[i], lane8, scale);
+    if (slot < 0) continue;
+    const int64_t own = slot >> 5;
+    if (own == tile[0] || own == tile[1]) {
+      const int to = own == tile[0] ? 0 : 1;
+      put<FMT, NB, VALUE>(sh.codes[to], sh.scales[to], static_cast<int>(slot & 31), b, lane8, q, scale);
+    } else {
+      const Plane p = at_unit<FMT, NB>(plane, unit_of(a.c, own, h));
+      put<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8, q, scale);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int to = 0; to < 2; ++to) {
+    if (tile[to] < 0) continue;
+    const unsigned mask = sh.mask[to];
+    const Plane p = at_unit<FMT, NB>(plane, unit_of(a.c, tile[to], h));
+    const unsigned* codes = reinterpret_cast<const unsigned*>(sh.codes[to]);
+    for (int w = threadIdx.x; w < Tiles<FMT, NB>::CODES / 4; w += kThreads) {
+      if constexpr (!VALUE) {
+        constexpr int each = kv_kb(NB, FMT) * (FMT == KV_Q8_0 ? 2 : 1), half = 4 * NB * kv_code_bytes(FMT);
+        if (mask >> (w / half * 16 + w / each % 16) & 1) reinterpret_cast<unsigned*>(p.codes)[w] = codes[w];
+      } else {
+        constexpr int each = kv_vb(NB, FMT) * (FMT == KV_Q8_0 ? 4 : 2);  // dwords a lane
+        const unsigned own = mask >> ((w & 1) * 16 + (w / each >> 4 & 3) * 4) & 15;
+        if (own == 15) {
+          reinterpret_cast<unsigned*>(p.codes)[w] = codes[w];
+        } else {
+          for (int e = 0; e < 4; ++e)
+            if (own >> e & 1) p.codes[w * 4 + e] = sh.codes[to][w * 4 + e];
+        }
+      }
+    }
+    for (int i = threadIdx.x; i < Tiles<FMT, NB>::SCALES; i += kThreads) {
+      // the token of scale i: kv_k_scale, kv_v_scale
+      const int k = i & 3, value = (i >> 2 & 1) * 16 + i / (8 * NB) * 4 + (k & 1) * 2 + (k >> 1);
+      if (mask >> (VALUE ? value : i / NB) & 1) p.scales[i] = sh.scales[to][i];
+    }
+  }
+}
+
+template <int KF, int VF, int NB, int TYPE, bool MANY>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
+  if constexpr (MANY) {
+    constexpr size_t bytes = sizeof(Tiles<KF, NB>) > sizeof(Tiles<VF, NB>) ? sizeof(Tiles<KF, NB>) : sizeof(Tiles<VF, NB>);
+    __shared__ __attribute__((aligned(16))) unsigned char shared[bytes];
+    if (blockIdx.z == 0) write_many<KF, NB, TYPE, false>(a, *reinterpret_cast<Tiles<KF, NB>*>(shared));
+    else write_many<VF, NB, TYPE, true>(a, *reinterpret_cast<Tiles<VF, NB>*>(shared));
+  } else {
+    if (blockIdx.z == 0) write_few<KF, NB, TYPE, false>(a);
+    else write_few<VF, NB, TYPE, true>(a);
   }
 }
 
@@ -169,55 +322,80 @@ __device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
   }
 }
 
-template <int KF, int VF, int NB, int TYPE>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
-  const int64_t gid = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (gid >= a.lanes) return;
-  const int lane8 = static_cast<int>(gid & 7);
-  const int64_t blk = gid >> 3;
-  const int b = static_cast<int>(blk % NB);
-  const int64_t th = blk / NB;
-  const int64_t t = th / a.c.heads;
-  const int h = static_cast<int>(th - t * a.c.heads);
+template <int FMT, int NB, int TYPE, bool VALUE>
+__device__ __forceinline__ void read_few(const ReadArgs& a) {
+  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.y;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kGroups / NB) + group / NB;
+  const int b = group % NB;
+  if (group >= kGroups / NB * NB || t >= a.tokens) return;
   const int64_t slot = a.slots[t];
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   if (slot >= 0 && slot < a.c.pages << a.c.page_log2) {
-    const int64_t unit = unit_of(a.c, slot, h);
-    const int token32 = static_cast<int>(slot & 31), token16 = token32 & 15;
-    uint16_t scale;
-    int q[4];
-    if (blockIdx.y == 0) {
-      const int64_t tile = unit * 2 + (token32 >> 4);
-      const int dword = kv_k_dword(NB, KF, token16, b, lane8 >> 1, lane8 & 1);
-      scale = a.c.ks[tile * (16 * NB) + kv_k_scale(NB, token16, b)];
-      if constexpr (KF == KV_Q8_0) {
-        const unsigned w = reinterpret_cast<const unsigned*>(a.c.kq)[tile * (128 * NB) + dword];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = static_cast<int>(w >> (8 * e) & 255) - 128;
-      } else {
-        const unsigned w = reinterpret_cast<const uint16_t*>(a.c.kq)[(tile * (64 * NB) + dword) * 2 + (lane8 & 1)];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = static_cast<int>(w >> (4 * e) & 15) - 8;
-      }
-    } else {
-      const uint8_t* base = a.c.vq + unit * (32 * NB * kv_code_bytes(VF));
-      scale = a.c.vs[unit * (32 * NB) + kv_v_scale(NB, token32, b)];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int w = base[kv_v_byte(NB, VF, token32, b, (lane8 & 3) * 4 + e, lane8 >> 2)];
-        q[e] = VF == KV_Q8_0 ? w - 128 : (lane8 < 4 ? w & 15 : w >> 4) - 8;
-      }
-    }
-    const float d = f16_bits_to_f32(static_cast<int16_t>(scale));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(q[e]) * d;
+    const Plane p = at_unit<FMT, NB>(plane_of<VALUE>(a.c), unit_of(a.c, slot >> 5, h));
+    v = get<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8);
   }
-  store4<TYPE>(a.x[blockIdx.y], (th * NB + b) * 32 + lane8 * 4, v);
+  store4<TYPE>(a.x[VALUE], ((t * a.c.heads + h) * NB + b) * 32 + lane8 * 4, v);
 }
 
+// (a tile is loaded whole, 16 bytes a lane, whatever part of it is read)
+template <int FMT, int NB, int TYPE, bool VALUE>
+__device__ __forceinline__ void read_many(const ReadArgs& a, Tiles<FMT, NB>& sh) {
+  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.y;
+  int64_t tile[2];
+  find_tiles(a.c, a.slots, a.tokens, sh, tile);
+  const Plane plane = plane_of<VALUE>(a.c);
+#pragma unroll
+  for (int to = 0; to < 2; ++to) {
+    if (tile[to] < 0) continue;
+    const Plane p = at_unit<FMT, NB>(plane, unit_of(a.c, tile[to], h));
+    for (int w = threadIdx.x; w < Tiles<FMT, NB>::CODES / 16; w += kThreads)
+      reinterpret_cast<u32x4*>(sh.codes[to])[w] = reinterpret_cast<const u32x4*>(p.codes)[w];
+    for (int w = threadIdx.x; w < Tiles<FMT, NB>::SCALES / 8; w += kThreads)
+      reinterpret_cast<u32x4*>(sh.scales[to])[w] = reinterpret_cast<const u32x4*>(p.scales)[w];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const int token = (i * kGroups + group) / NB, b = (i * kGroups + group) % NB;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 32 + token, slot = sh.slot[token], own = slot >> 5;
+    if (t >= a.tokens) continue;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (slot >= 0) {
+      if (own == tile[0] || own == tile[1]) {
+        const int to = own == tile[0] ? 0 : 1;
+        v = get<FMT, NB, VALUE>(sh.codes[to], sh.scales[to], static_cast<int>(slot & 31), b, lane8);
+      } else {
+        const Plane p = at_unit<FMT, NB>(plane, unit_of(a.c, own, h));
+        v = get<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8);
+      }
+    }
+    store4<TYPE>(a.x[VALUE], ((t * a.c.heads + h) * NB + b) * 32 + lane8 * 4, v);
+  }
+}
+
+template <int KF, int VF, int NB, int TYPE, bool MANY>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
+  if constexpr (MANY) {
+    constexpr size_t bytes = sizeof(Tiles<KF, NB>) > sizeof(Tiles<VF, NB>) ? sizeof(Tiles<KF, NB>) : sizeof(Tiles<VF, NB>);
+    __shared__ __attribute__((aligned(16))) unsigned char shared[bytes];
+    if (blockIdx.z == 0) read_many<KF, NB, TYPE, false>(a, *reinterpret_cast<Tiles<KF, NB>*>(shared));
+    else read_many<VF, NB, TYPE, true>(a, *reinterpret_cast<Tiles<VF, NB>*>(shared));
+  } else {
+    if (blockIdx.z == 0) read_few<KF, NB, TYPE, false>(a);
+    else read_few<VF, NB, TYPE, true>(a);
+  }
+}
+
+// Workgroups of one call: `per` tokens of one head each, keys and values apart.
+dim3 grid_of(int64_t tokens, int per, int heads) {
+  return dim3(static_cast<unsigned>((tokens + per - 1) / per), static_cast<unsigned>(heads), 2);
+}
+
+// The kernels of 32-token tiles, from the size on where they fill the CUs.
+bool many_tokens(int64_t tokens, int heads) { return tokens * heads >= 32 * 512; }
+
 template <typename F, typename A>
-hipError_t launch(F kern, int64_t lanes, hipStream_t stream, const A& a) {
-  const dim3 grid(static_cast<unsigned>((lanes + kThreads - 1) / kThreads), 2);
+hipError_t launch(F kern, const dim3& grid, hipStream_t stream, const A& a) {
   const Timing tm = timing_slot(KIND_PROBE);
   if (tm.on) {
     hipExtLaunchKernelGGL(kern, grid, dim3(kThreads), 0, stream, tm.start, tm.stop, 0, a);
@@ -257,7 +435,7 @@ hipError_t launch_kv_write(const KvWriteCall& w, hipStream_t stream) {
   WriteArgs a;
   a.c = w.cache;
   a.slots = w.slots;
-  a.lanes = w.tokens * w.cache.heads * (w.cache.dim / 4);
+  a.tokens = w.tokens;
   const int size = w.type == KV_F32 ? 4 : 2;
   for (int i = 0; i < 2; ++i) {
     a.x[i] = i ? w.v : w.k;
@@ -266,7 +444,10 @@ hipError_t launch_kv_write(const KvWriteCall& w, hipStream_t stream) {
     a.wide[i] = reinterpret_cast<uintptr_t>(a.x[i]) % (4 * size) == 0 && w.stride_t[i] % 4 == 0 && w.stride_h[i] % 4 == 0;
   }
   return with_constants(w.cache, w.type, [&](auto kf, auto vf, auto nb, auto type) {
-    return launch(kv_write_kernel<kf.value, vf.value, nb.value, type.value>, a.lanes, stream, a);
+    constexpr int KF = kf.value, VF = vf.value, NB = nb.value, TYPE = type.value;
+    if (many_tokens(a.tokens, a.c.heads))
+      return launch(kv_write_kernel<KF, VF, NB, TYPE, true>, grid_of(a.tokens, 32, a.c.heads), stream, a);
+    return launch(kv_write_kernel<KF, VF, NB, TYPE, false>, grid_of(a.tokens, kGroups / NB, a.c.heads), stream, a);
   });
 }
 
@@ -274,11 +455,14 @@ hipError_t launch_kv_read(const KvReadCall& r, hipStream_t stream) {
   ReadArgs a;
   a.c = r.cache;
   a.slots = r.slots;
-  a.lanes = r.tokens * r.cache.heads * (r.cache.dim / 4);
+  a.tokens = r.tokens;
   a.x[0] = r.k;
   a.x[1] = r.v;
   return with_constants(r.cache, r.type, [&](auto kf, auto vf, auto nb, auto type) {
-    return launch(kv_read_kernel<kf.value, vf.value, nb.value, type.value>, a.lanes, stream, a);
+    constexpr int KF = kf.value, VF = vf.value, NB = nb.value, TYPE = type.value;
+    if (many_tokens(a.tokens, a.c.heads))
+      return launch(kv_read_kernel<KF, VF, NB, TYPE, true>, grid_of(a.tokens, 32, a.c.heads), stream, a);
+    return launch(kv_read_kernel<KF, VF, NB, TYPE, false>, grid_of(a.tokens, kGroups / NB, a.c.heads), stream, a);
   });
 }
 
