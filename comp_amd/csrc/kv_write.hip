@@ -6,6 +6,7 @@
 #include <hip/hip_ext.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "komp_device.h"
 #include "komp_internal.h"
@@ -13,6 +14,16 @@
 
 namespace komp {
 namespace {
+
+// f(integral_constant<int, 0>{}) .. f(integral_constant<int, N - 1>{})
+template <typename F, int... I>
+__device__ __forceinline__ void each_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  each_impl(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
+}
 
 constexpr int kThreads = 256, kGroups = kThreads / 8;
 
@@ -62,46 +73,62 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t i, bool wide) {
 
 __device__ __forceinline__ uint16_t f16_bits(float v) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v)); }
 
-// One block of 32 held by 8 aligned lanes of 4 values: the lane's four codes as unsigned bytes (Q4_0: 0..15, Q8_0:
-// value + 128), and the block's scale bits in every lane.
-template <int FMT>
-__device__ __forceinline__ unsigned quantize8(f32x4 v, int lane8, uint16_t& scale) {
+// Blocks of 32, each held by 8 aligned lanes of 4 values, N of them: the lane's four codes of each as unsigned bytes (Q4_0:
+// 0..15, Q8_0: value + 128).  The divisions of N blocks are shared out: lane n of each four does block n's, and holds its
+// scale's bits afterwards (N = 1: every lane).
+template <int FMT, int N>
+__device__ __forceinline__ void quantize8(const f32x4 (&v)[N], int lane8, unsigned (&packed)[N], uint16_t& scale) {
 #pragma clang fp contract(off)
-  // |x|'s bits order like the floats, and a NaN's are above infinity's
-  int a[4];
+  static_assert(N == 1 || N == 4, "blocks of a quad of lanes");
+  float d[N];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) a[e] = __float_as_int(v[e]) & 0x7FFFFFFF;
-  int top = max(max(a[0], a[1]), max(a[2], a[3]));
-  top = max(top, dpp_i<KOMP_DPP_XOR1>(top));
-  top = max(top, dpp_i<KOMP_DPP_XOR2>(top));
-  top = max(top, dpp_i<KOMP_DPP_HALF_MIRROR>(top));
-  float d;
-  if constexpr (FMT == KV_Q8_0) {
-    d = __int_as_float(top) / 127.0f;
-  } else {
-    int first = 64;  // 2 * index + sign of the first value of that magnitude
+  for (int n = 0; n < N; ++n) {
+    // |x|'s bits order like the floats, and a NaN's are above infinity's
+    int a[4];
 #pragma unroll
-    for (int e = 3; e >= 0; --e) first = a[e] == top ? 2 * (4 * lane8 + e) + (__float_as_uint(v[e]) >> 31) : first;
-    first = min(first, dpp_i<KOMP_DPP_XOR1>(first));
-    first = min(first, dpp_i<KOMP_DPP_XOR2>(first));
-    first = min(first, dpp_i<KOMP_DPP_HALF_MIRROR>(first));
-    d = __int_as_float(top) * ((first & 1) ? 0.125f : -0.125f);
-  }
-  const float id = d != 0.0f ? 1.0f / d : 0.0f;
-  scale = f16_bits(d);
-  unsigned packed = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float y = v[e] * id;
-    int q;
+    for (int e = 0; e < 4; ++e) a[e] = __float_as_int(v[n][e]) & 0x7FFFFFFF;
+    int top = max(max(a[0], a[1]), max(a[2], a[3]));
+    top = max(top, dpp_i<KOMP_DPP_XOR1>(top));
+    top = max(top, dpp_i<KOMP_DPP_XOR2>(top));
+    top = max(top, dpp_i<KOMP_DPP_HALF_MIRROR>(top));
     if constexpr (FMT == KV_Q8_0) {
-      q = max(0, min(255, static_cast<int>(round_half_away(y)) + 128));
+      d[n] = __int_as_float(top);
     } else {
-      q = max(0, min(15, static_cast<int>(floorf(y + 8.5f))));
+      int first = 64;  // 2 * index + sign of the first value of that magnitude
+#pragma unroll
+      for (int e = 3; e >= 0; --e) first = a[e] == top ? 2 * (4 * lane8 + e) + (__float_as_uint(v[n][e]) >> 31) : first;
+      first = min(first, dpp_i<KOMP_DPP_XOR1>(first));
+      first = min(first, dpp_i<KOMP_DPP_XOR2>(first));
+      first = min(first, dpp_i<KOMP_DPP_HALF_MIRROR>(first));
+      d[n] = __int_as_float(top) * ((first & 1) ? 0.125f : -0.125f);
     }
-    packed |= static_cast<unsigned>(q) << (8 * e);
   }
-  return packed;
+  float own = d[0];
+  if constexpr (N == 4) {
+    const int q = lane8 & 3;
+    own = q == 0 ? d[0] : q == 1 ? d[1] : q == 2 ? d[2] : d[3];
+  }
+  if constexpr (FMT == KV_Q8_0) own = own / 127.0f;
+  scale = f16_bits(own);
+  float id = own != 0.0f ? 1.0f / own : 0.0f;
+  if constexpr (FMT == KV_Q8_0) id = id + id;
+  each<N>([&](auto nc) __attribute__((always_inline)) {
+    constexpr int n = nc.value;
+    // quad_perm [n, n, n, n]: lane n of each four
+    const float f = N == 1 ? id : __int_as_float(dpp_i<N == 1 ? 0 : n * 0x55>(__float_as_int(id)));
+    unsigned q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (FMT == KV_Q8_0) {
+        // t = trunc(2 y), y = x * id (2 id is exact): roundf(y) is (t + 1) >> 1 for t >= 0, t >> 1 below; and 128 more
+        const int t = static_cast<int>(v[n][e] * f);
+        q[e] = static_cast<unsigned>(t + (t >> 31) + 257) >> 1 & 255;
+      } else {
+        q[e] = min(15u, static_cast<unsigned>(v[n][e] * f + 8.5f));
+      }
+    }
+    packed[n] = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+  });
 }
 
 // where a tile of 32 tokens of a page and head lies, in units of such tiles
@@ -109,6 +136,8 @@ __device__ __forceinline__ int64_t unit_of(const KvCache& c, int64_t tile, int h
   const int log2 = c.page_log2 - 5;
   return (((tile >> log2) * c.heads + h) << log2) + (tile & ((int64_t{1} << log2) - 1));
 }
+
+constexpr int kNext4 = 0x104;  // row_shl:4, lane + 4 of a row
 
 // A block's codes, four of eight lanes each, into the 32-token tile at `codes` and `scales` (global or shared memory).
 // Only this token's bytes are written.
@@ -126,7 +155,7 @@ __device__ __forceinline__ void put(uint8_t* codes, uint16_t* scales, int token3
     }
     if (lane8 == 0) scales[(token32 >> 4) * (16 * NB) + kv_k_scale(NB, token16, b)] = scale;
   } else {
-    if constexpr (FMT == KV_Q4_0) q |= __shfl_xor(static_cast<int>(q), 4, 64) << 4;  // used by lanes 0..3: channels + 16
+    if constexpr (FMT == KV_Q4_0) q |= static_cast<unsigned>(dpp_i<kNext4>(static_cast<int>(q))) << 4;  // lanes 0..3: channels + 16
     if (FMT == KV_Q8_0 || lane8 < 4) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -184,85 +213,136 @@ __device__ __forceinline__ Plane at_unit(const Plane& p, int64_t unit) {
 // Few tokens: eight lanes a block, a workgroup's blocks those of `tokens` tokens of one head.
 template <int FMT, int NB, int TYPE, bool VALUE>
 __device__ __forceinline__ void write_few(const WriteArgs& a) {
-  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.y;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kGroups / NB) + group / NB;
+  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.x % a.c.heads;
+  const int64_t t = static_cast<int64_t>(blockIdx.x / a.c.heads) * (kGroups / NB) + group / NB;
   const int b = group % NB;
   if (group >= kGroups / NB * NB || t >= a.tokens) return;  // in groups of 8 lanes
   const int64_t slot = a.slots[t];
   if (slot < 0 || slot >= a.c.pages << a.c.page_log2) return;
-  const f32x4 v = load4<TYPE>(a.x[VALUE], t * a.stride_t[VALUE] + h * a.stride_h[VALUE] + b * 32 + lane8 * 4, a.wide[VALUE]);
+  const f32x4 v[1] = {load4<TYPE>(a.x[VALUE], t * a.stride_t[VALUE] + h * a.stride_h[VALUE] + b * 32 + lane8 * 4, a.wide[VALUE])};
   uint16_t scale;
-  const unsigned q = quantize8<FMT>(v, lane8, scale);
+  unsigned q[1];
+  quantize8<FMT>(v, lane8, q, scale);
   const Plane p = at_unit<FMT, NB>(plane_of<VALUE>(a.c), unit_of(a.c, slot >> 5, h));
-  put<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8, q, scale);
+  put<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8, q[0], scale);
 }
 
-// Many tokens: a workgroup has 32 tokens of the list and one head.  Consecutive slots fall into two tiles of 32 at most,
-// which it puts together in shared memory and stores by dwords where all the tokens of a dword are its own (four for value
-// codes, two for their scales); tokens of further tiles go one by one.
+// Four tokens' codes of a block, four channels a lane, as four channels' codes, four tokens each, and back.
+__device__ __forceinline__ void transpose4(unsigned (&q)[4]) {
+  const unsigned a = __builtin_amdgcn_perm(q[1], q[0], 0x05010400u), b = __builtin_amdgcn_perm(q[1], q[0], 0x07030602u);
+  const unsigned c = __builtin_amdgcn_perm(q[3], q[2], 0x05010400u), d = __builtin_amdgcn_perm(q[3], q[2], 0x07030602u);
+  q[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  q[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  q[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  q[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// Many tokens: a workgroup has 32 tokens of the list and one head.  Consecutive slots fall into two tiles of 32 at most (one
+// where the list begins at a tile's start, which the first tokens are left out of the first workgroup for); a group of
+// eight lanes takes a block of four neighbouring places of a tile at a time, and the workgroup puts the tiles together in
+// shared memory and moves them by dwords, four tokens of value codes in one.  Tokens of further tiles go one by one.
 template <int FMT, int NB>
 struct Tiles {
   static constexpr int CODES = 32 * NB * kv_code_bytes(FMT), SCALES = 32 * NB;
   uint8_t codes[2][CODES];
   uint16_t scales[2][SCALES];
-  int64_t slot[32];
-  unsigned mask[2];  // tokens of the tiles that are written or read here
+  int64_t slot[32];  // of the tokens of further tiles; -1 for the others
+  int token[2][32];  // which of the 32 a place of a tile belongs to; -1: none
+  int quads[16];     // the fours of places that have a token, 8 * tile + four
+  unsigned mask[2];  // the places that have one
+  int further;       // whether there are tokens of further tiles
 };
-// Fills slot[] and mask[] and finds the two tiles, the first and the last valid slot's; -1 for none.
+// What lies where; the two tiles are the first and the last valid slot's (-1 for none).  Returns the list's index of the
+// first token, and in `count` how many fours of places there are.
 template <int FMT, int NB>
-__device__ __forceinline__ void find_tiles(const KvCache& c, const int64_t* slots, int64_t tokens, Tiles<FMT, NB>& sh, int64_t (&tile)[2]) {
+__device__ __forceinline__ int64_t find_tiles(const KvCache& c, const int64_t* slots, int64_t tokens, Tiles<FMT, NB>& sh, int64_t (&tile)[2], int& count) {
   const int lane = threadIdx.x & 63;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 32 + (lane & 31);
-  int64_t slot = t < tokens ? slots[t] : -1;
+  const int64_t first = static_cast<int64_t>(blockIdx.x / c.heads) * 32 - (slots[0] & 31), t = first + (lane & 31);
+  int64_t slot = t >= 0 && t < tokens ? slots[t] : -1;
   if (slot < 0 || slot >= c.pages << c.page_log2) slot = -1;
   const unsigned there = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(slot >= 0 && lane < 32));
   tile[0] = tile[1] = -1;
+  const int64_t own = slot >> 5;
   if (there) {
-    const int64_t own = slot >> 5;
     tile[0] = __shfl(own, __builtin_ctz(there), 64);
     tile[1] = __shfl(own, 31 - __builtin_clz(there), 64);
     if (tile[1] == tile[0]) tile[1] = -1;
   }
+  if (threadIdx.x < 64) (&sh.token[0][0])[threadIdx.x] = -1;
   if (threadIdx.x < 2) sh.mask[threadIdx.x] = 0;
+  const int to = slot < 0 || lane >= 32 ? -1 : own == tile[0] ? 0 : own == tile[1] ? 1 : -2;
+  const bool further = __builtin_amdgcn_ballot_w64(to == -2) != 0;
   __syncthreads();
   if (threadIdx.x < 32) {
-    sh.slot[threadIdx.x] = slot;
-    if (slot >= 0 && (slot >> 5) == tile[0]) atomicOr(&sh.mask[0], 1u << (slot & 31));
-    if (slot >= 0 && (slot >> 5) == tile[1]) atomicOr(&sh.mask[1], 1u << (slot & 31));
+    sh.slot[threadIdx.x] = to == -2 ? slot : -1;
+    if (to >= 0) {
+      sh.token[to][slot & 31] = threadIdx.x;
+      atomicOr(&sh.mask[to], 1u << (slot & 31));
+    }
   }
+  if (threadIdx.x == 0) sh.further = further;
   __syncthreads();
+  unsigned fours = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) fours |= (sh.mask[i >> 3] >> ((i & 7) * 4) & 15) ? 1u << i : 0u;
+  count = __builtin_popcount(fours);
+  if (threadIdx.x < 16 && (fours >> threadIdx.x & 1)) sh.quads[__builtin_popcount(fours & ((1u << threadIdx.x) - 1))] = threadIdx.x;
+  __syncthreads();
+  return first;
 }
 
 template <int FMT, int NB, int TYPE, bool VALUE>
 __device__ __forceinline__ void write_many(const WriteArgs& a, Tiles<FMT, NB>& sh) {
-  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.y;
+  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.x % a.c.heads;
   int64_t tile[2];
-  find_tiles(a.c, a.slots, a.tokens, sh, tile);
+  int count;
+  const int64_t first = find_tiles(a.c, a.slots, a.tokens, sh, tile, count);
   const Plane plane = plane_of<VALUE>(a.c);
-  // all loads first: a token left out loads nothing
-  f32x4 v[NB];
+  auto row = [&](int token, int b) {
+    return load4<TYPE>(a.x[VALUE], (first + token) * a.stride_t[VALUE] + h * a.stride_h[VALUE] + b * 32 + lane8 * 4, a.wide[VALUE]);
+  };
+  for (int task = group; task < count * NB; task += kGroups) {
+    const int quad = sh.quads[task / NB], b = task % NB, to = quad >> 3, at = (quad & 7) * 4;
+    f32x4 v[4];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const int token = (i * kGroups + group) / NB, b = (i * kGroups + group) % NB;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 32 + token;
-    v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (sh.slot[token] >= 0)
-      v[i] = load4<TYPE>(a.x[VALUE], t * a.stride_t[VALUE] + h * a.stride_h[VALUE] + b * 32 + lane8 * 4, a.wide[VALUE]);
-  }
-#pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const int token = (i * kGroups + group) / NB, b = (i * kGroups + group) % NB;
-    const int64_t slot = sh.slot[token];
+    for (int n = 0; n < 4; ++n) {
+      const int token = sh.token[to][at + n];
+      v[n] = f32x4{0.f, 0.f, 0.f, 0.f};  // (a place without a token: what becomes of it is not stored)
+      if (token >= 0) v[n] = row(token, b);
+    }
+    unsigned q[4];
     uint16_t scale;
-    const unsigned q = quantize8<FMT>(v[i], lane8, scale);
-    if (slot < 0) continue;
-    const int64_t own = slot >> 5;
-    if (own == tile[0] || own == tile[1]) {
-      const int to = own == tile[0] ? 0 : 1;
-      put<FMT, NB, VALUE>(sh.codes[to], sh.scales[to], static_cast<int>(slot & 31), b, lane8, q, scale);
+    quantize8<FMT>(v, lane8, q, scale);
+    if constexpr (VALUE) {
+      if constexpr (FMT == KV_Q4_0) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) q[n] |= static_cast<unsigned>(dpp_i<kNext4>(static_cast<int>(q[n]))) << 4;
+      }
+      if (FMT == KV_Q8_0 || lane8 < 4) {
+        transpose4(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<unsigned*>(&sh.codes[to][kv_v_byte(NB, FMT, at, b, (lane8 & 3) * 4 + e, lane8 >> 2)]) = q[e];
+      }
+      if (lane8 < 4) sh.scales[to][kv_v_scale(NB, at + lane8, b)] = scale;
     } else {
-      const Plane p = at_unit<FMT, NB>(plane, unit_of(a.c, own, h));
-      put<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8, q, scale);
+      each<4>([&](auto nc) __attribute__((always_inline)) {
+        constexpr int n = nc.value;
+        put<FMT, NB, VALUE>(sh.codes[to], sh.scales[to], at + n, b, lane8, q[n], static_cast<uint16_t>(dpp_i<n * 0x55>(scale)));
+      });
+    }
+  }
+  if (sh.further) {
+    for (int task = group; task < 32 * NB; task += kGroups) {
+      const int64_t slot = sh.slot[task / NB];
+      const int b = task % NB;
+      if (slot < 0) continue;
+      const f32x4 v[1] = {row(task / NB, b)};
+      unsigned q[1];
+      uint16_t scale;
+      quantize8<FMT>(v, lane8, q, scale);
+      const Plane p = at_unit<FMT, NB>(plane, unit_of(a.c, slot >> 5, h));
+      put<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8, q[0], scale);
     }
   }
   __syncthreads();
@@ -271,14 +351,21 @@ __device__ __forceinline__ void write_many(const WriteArgs& a, Tiles<FMT, NB>& s
     if (tile[to] < 0) continue;
     const unsigned mask = sh.mask[to];
     const Plane p = at_unit<FMT, NB>(plane, unit_of(a.c, tile[to], h));
+    if (mask == 0xFFFFFFFFu) {  // the whole tile
+      for (int w = threadIdx.x; w < Tiles<FMT, NB>::CODES / 16; w += kThreads)
+        reinterpret_cast<u32x4*>(p.codes)[w] = reinterpret_cast<const u32x4*>(sh.codes[to])[w];
+      for (int w = threadIdx.x; w < Tiles<FMT, NB>::SCALES / 8; w += kThreads)
+        reinterpret_cast<u32x4*>(p.scales)[w] = reinterpret_cast<const u32x4*>(sh.scales[to])[w];
+      continue;
+    }
     const unsigned* codes = reinterpret_cast<const unsigned*>(sh.codes[to]);
     for (int w = threadIdx.x; w < Tiles<FMT, NB>::CODES / 4; w += kThreads) {
       if constexpr (!VALUE) {
-        constexpr int each = kv_kb(NB, FMT) * (FMT == KV_Q8_0 ? 2 : 1), half = 4 * NB * kv_code_bytes(FMT);
-        if (mask >> (w / half * 16 + w / each % 16) & 1) reinterpret_cast<unsigned*>(p.codes)[w] = codes[w];
+        constexpr int lane_words = kv_kb(NB, FMT) * (FMT == KV_Q8_0 ? 2 : 1), half = 4 * NB * kv_code_bytes(FMT);
+        if (mask >> (w / half * 16 + w / lane_words % 16) & 1) reinterpret_cast<unsigned*>(p.codes)[w] = codes[w];
       } else {
-        constexpr int each = kv_vb(NB, FMT) * (FMT == KV_Q8_0 ? 4 : 2);  // dwords a lane
-        const unsigned own = mask >> ((w & 1) * 16 + (w / each >> 4 & 3) * 4) & 15;
+        constexpr int lane_words = kv_vb(NB, FMT) * (FMT == KV_Q8_0 ? 4 : 2);
+        const unsigned own = mask >> ((w & 1) * 16 + (w / lane_words >> 4 & 3) * 4) & 15;
         if (own == 15) {
           reinterpret_cast<unsigned*>(p.codes)[w] = codes[w];
         } else {
@@ -300,10 +387,10 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const WriteArgs a) {
   if constexpr (MANY) {
     constexpr size_t bytes = sizeof(Tiles<KF, NB>) > sizeof(Tiles<VF, NB>) ? sizeof(Tiles<KF, NB>) : sizeof(Tiles<VF, NB>);
     __shared__ __attribute__((aligned(16))) unsigned char shared[bytes];
-    if (blockIdx.z == 0) write_many<KF, NB, TYPE, false>(a, *reinterpret_cast<Tiles<KF, NB>*>(shared));
+    if (blockIdx.y == 0) write_many<KF, NB, TYPE, false>(a, *reinterpret_cast<Tiles<KF, NB>*>(shared));
     else write_many<VF, NB, TYPE, true>(a, *reinterpret_cast<Tiles<VF, NB>*>(shared));
   } else {
-    if (blockIdx.z == 0) write_few<KF, NB, TYPE, false>(a);
+    if (blockIdx.y == 0) write_few<KF, NB, TYPE, false>(a);
     else write_few<VF, NB, TYPE, true>(a);
   }
 }
@@ -324,8 +411,8 @@ __device__ __forceinline__ void store4(void* p, int64_t i, f32x4 v) {
 
 template <int FMT, int NB, int TYPE, bool VALUE>
 __device__ __forceinline__ void read_few(const ReadArgs& a) {
-  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.y;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kGroups / NB) + group / NB;
+  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.x % a.c.heads;
+  const int64_t t = static_cast<int64_t>(blockIdx.x / a.c.heads) * (kGroups / NB) + group / NB;
   const int b = group % NB;
   if (group >= kGroups / NB * NB || t >= a.tokens) return;
   const int64_t slot = a.slots[t];
@@ -340,9 +427,10 @@ __device__ __forceinline__ void read_few(const ReadArgs& a) {
 // (a tile is loaded whole, 16 bytes a lane, whatever part of it is read)
 template <int FMT, int NB, int TYPE, bool VALUE>
 __device__ __forceinline__ void read_many(const ReadArgs& a, Tiles<FMT, NB>& sh) {
-  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.y;
+  const int lane8 = threadIdx.x & 7, group = threadIdx.x >> 3, h = blockIdx.x % a.c.heads;
   int64_t tile[2];
-  find_tiles(a.c, a.slots, a.tokens, sh, tile);
+  int count;
+  const int64_t first = find_tiles(a.c, a.slots, a.tokens, sh, tile, count);
   const Plane plane = plane_of<VALUE>(a.c);
 #pragma unroll
   for (int to = 0; to < 2; ++to) {
@@ -354,22 +442,53 @@ __device__ __forceinline__ void read_many(const ReadArgs& a, Tiles<FMT, NB>& sh)
       reinterpret_cast<u32x4*>(sh.scales[to])[w] = reinterpret_cast<const u32x4*>(p.scales)[w];
   }
   __syncthreads();
+  auto store = [&](int token, int b, f32x4 v) {
+    store4<TYPE>(a.x[VALUE], (((first + token) * a.c.heads + h) * NB + b) * 32 + lane8 * 4, v);
+  };
+  for (int task = group; task < count * NB; task += kGroups) {
+    const int quad = sh.quads[task / NB], b = task % NB, to = quad >> 3, at = (quad & 7) * 4;
+    f32x4 v[4];
+    if constexpr (VALUE) {
+      unsigned q[4];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const int token = (i * kGroups + group) / NB, b = (i * kGroups + group) % NB;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 32 + token, slot = sh.slot[token], own = slot >> 5;
-    if (t >= a.tokens) continue;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (slot >= 0) {
-      if (own == tile[0] || own == tile[1]) {
-        const int to = own == tile[0] ? 0 : 1;
-        v = get<FMT, NB, VALUE>(sh.codes[to], sh.scales[to], static_cast<int>(slot & 31), b, lane8);
-      } else {
+      for (int e = 0; e < 4; ++e) {
+        q[e] = *reinterpret_cast<const unsigned*>(&sh.codes[to][kv_v_byte(NB, FMT, at, b, (lane8 & 3) * 4 + e, lane8 >> 2)]);
+        if constexpr (FMT == KV_Q4_0) q[e] = (lane8 < 4 ? q[e] : q[e] >> 4) & 0x0F0F0F0Fu;
+      }
+      transpose4(q);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float d = f16_bits_to_f32(static_cast<int16_t>(sh.scales[to][kv_v_scale(NB, at + n, b)]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[n][e] = (static_cast<float>(q[n] >> (8 * e) & 255u) - (FMT == KV_Q8_0 ? 128.f : 8.f)) * d;
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v[n] = get<FMT, NB, VALUE>(sh.codes[to], sh.scales[to], at + n, b, lane8);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int token = sh.token[to][at + n];
+      if (token >= 0) store(token, b, v[n]);
+    }
+  }
+  // tokens of further tiles, and those without a slot (or a second time the same one): one by one
+  const int left = static_cast<int>(min(int64_t{32}, a.tokens - first));
+  if (__builtin_popcount(sh.mask[0]) + __builtin_popcount(sh.mask[1]) < left - static_cast<int>(max(int64_t{0}, -first))) {
+    for (int task = group; task < 32 * NB; task += kGroups) {
+      const int token = task / NB, b = task % NB;
+      const int64_t t = first + token;
+      if (t < 0 || t >= a.tokens) continue;
+      const int64_t slot = a.slots[t], own = slot >> 5;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (slot >= 0 && slot < a.c.pages << a.c.page_log2) {
+        const int to = own == tile[0] ? 0 : own == tile[1] ? 1 : -1;
+        if (to >= 0 && sh.token[to][slot & 31] == token) continue;
         const Plane p = at_unit<FMT, NB>(plane, unit_of(a.c, own, h));
         v = get<FMT, NB, VALUE>(p.codes, p.scales, static_cast<int>(slot & 31), b, lane8);
       }
+      store(token, b, v);
     }
-    store4<TYPE>(a.x[VALUE], ((t * a.c.heads + h) * NB + b) * 32 + lane8 * 4, v);
   }
 }
 
@@ -378,20 +497,21 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
   if constexpr (MANY) {
     constexpr size_t bytes = sizeof(Tiles<KF, NB>) > sizeof(Tiles<VF, NB>) ? sizeof(Tiles<KF, NB>) : sizeof(Tiles<VF, NB>);
     __shared__ __attribute__((aligned(16))) unsigned char shared[bytes];
-    if (blockIdx.z == 0) read_many<KF, NB, TYPE, false>(a, *reinterpret_cast<Tiles<KF, NB>*>(shared));
+    if (blockIdx.y == 0) read_many<KF, NB, TYPE, false>(a, *reinterpret_cast<Tiles<KF, NB>*>(shared));
     else read_many<VF, NB, TYPE, true>(a, *reinterpret_cast<Tiles<VF, NB>*>(shared));
   } else {
-    if (blockIdx.z == 0) read_few<KF, NB, TYPE, false>(a);
+    if (blockIdx.y == 0) read_few<KF, NB, TYPE, false>(a);
     else read_few<VF, NB, TYPE, true>(a);
   }
 }
 
-// Workgroups of one call: `per` tokens of one head each, keys and values apart.
+// Workgroups of one call: `per` tokens of one head each, keys and values apart.  The heads of the same tokens follow one
+// another, so that a token's rows are read and written together.
 dim3 grid_of(int64_t tokens, int per, int heads) {
-  return dim3(static_cast<unsigned>((tokens + per - 1) / per), static_cast<unsigned>(heads), 2);
+  return dim3(static_cast<unsigned>((tokens + per - 1) / per * heads), 2);
 }
 
-// The kernels of 32-token tiles, from the size on where they fill the CUs.
+// The kernels of 32-token tiles, from the size on where they fill the CUs (and their lists begin 0 to 31 tokens early).
 bool many_tokens(int64_t tokens, int heads) { return tokens * heads >= 32 * 512; }
 
 template <typename F, typename A>
@@ -446,7 +566,7 @@ hipError_t launch_kv_write(const KvWriteCall& w, hipStream_t stream) {
   return with_constants(w.cache, w.type, [&](auto kf, auto vf, auto nb, auto type) {
     constexpr int KF = kf.value, VF = vf.value, NB = nb.value, TYPE = type.value;
     if (many_tokens(a.tokens, a.c.heads))
-      return launch(kv_write_kernel<KF, VF, NB, TYPE, true>, grid_of(a.tokens, 32, a.c.heads), stream, a);
+      return launch(kv_write_kernel<KF, VF, NB, TYPE, true>, grid_of(a.tokens + 31, 32, a.c.heads), stream, a);
     return launch(kv_write_kernel<KF, VF, NB, TYPE, false>, grid_of(a.tokens, kGroups / NB, a.c.heads), stream, a);
   });
 }
@@ -461,7 +581,7 @@ hipError_t launch_kv_read(const KvReadCall& r, hipStream_t stream) {
   return with_constants(r.cache, r.type, [&](auto kf, auto vf, auto nb, auto type) {
     constexpr int KF = kf.value, VF = vf.value, NB = nb.value, TYPE = type.value;
     if (many_tokens(a.tokens, a.c.heads))
-      return launch(kv_read_kernel<KF, VF, NB, TYPE, true>, grid_of(a.tokens, 32, a.c.heads), stream, a);
+      return launch(kv_read_kernel<KF, VF, NB, TYPE, true>, grid_of(a.tokens + 31, 32, a.c.heads), stream, a);
     return launch(kv_read_kernel<KF, VF, NB, TYPE, false>, grid_of(a.tokens, kGroups / NB, a.c.heads), stream, a);
   });
 }

@@ -27,6 +27,8 @@ import torch
 from . import _abi
 from .host import _current_device, _need, _raw_stream
 
+_Tensor, _I64, _I32 = torch.Tensor, torch.int64, torch.int32
+
 HEAD_DIMS = (64, 96, 128, 256)
 FORMATS = {"q4_0": 0, "q8_0": 2}  # the weight formats' numbers; 16 and 32 code bytes a block of 32
 PAIRS = (("q4_0", "q4_0"), ("q8_0", "q4_0"), ("q8_0", "q8_0"))  # (keys, values)
@@ -66,6 +68,8 @@ class KVCache:
                                           FORMATS[k_format], FORMATS[v_format])  # fmt: skip
         self._ref = ctypes.addressof(self._struct)
         self._device = self.kq.get_device()
+        self._scale = 1.0 / math.sqrt(head_dim)
+        self._work = {}  # workspace bytes of attention calls by their sizes
 
     @property
     def device(self):
@@ -117,69 +121,91 @@ def _need_ints(t, name, cache, dtype, shape):
         raise _BAD(f"{name} is on {t.device}, the cache on {cache.device}")
 
 
+# An eager call is mostly host time, so each checks its arguments in one chain of cheap attribute reads first, which implies
+# the full checks; those run, and name the fault, when any of it fails.
+def _rows_fit(t, cache, heads):
+    """True for a tensor that passes _need_rows(t, ..., cache, heads, ...)."""
+    if isinstance(t, _Tensor) and t.is_cuda and t.dtype in TYPES and t.dim() == 3:
+        shape = t.shape
+        return (shape[1] == heads and shape[2] == cache.head_dim and t.stride(2) == 1 and t.get_device() == cache._device)  # fmt: skip
+    return False
+
+
+def _ints_fit(t, cache, dtype, n):
+    """True for a contiguous one-dimensional tensor of n elements of this type on the cache's device."""
+    return (isinstance(t, _Tensor) and t.is_cuda and t.dtype is dtype and t.dim() == 1 and t.shape[0] == n
+            and t.is_contiguous() and t.get_device() == cache._device)  # fmt: skip
+
+
 def write(cache, k, v, slots):
     """Quantize k, v [T][kv_heads][head_dim] (f32, f16 or bf16; rows contiguous, any strides between them) into the cache's
     slots int64 [T].  A negative slot leaves its token out; slots of one call are to differ.  Returns the cache."""
-    _need_cache(cache)
-    _need_rows(k, "k", cache, cache.kv_heads, "T")
-    _need_rows(v, "v", cache, cache.kv_heads, "T")
-    if v.shape[0] != k.shape[0] or v.dtype is not k.dtype:
-        raise _BAD(f"k and v must have as many tokens and one type: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
-    _need_ints(slots, "slots", cache, torch.int64, (k.shape[0],))
-    _launch("komp_kv_write", cache, k.data_ptr(), v.data_ptr(), TYPES[k.dtype], slots.data_ptr(), k.shape[0], k.stride(0),
-            k.stride(1), v.stride(0), v.stride(1))  # fmt: skip
+    if not (type(cache) is KVCache and _rows_fit(k, cache, cache.kv_heads) and _rows_fit(v, cache, cache.kv_heads)
+            and v.shape[0] == k.shape[0] and v.dtype is k.dtype and _ints_fit(slots, cache, _I64, k.shape[0])):  # fmt: skip
+        _need_cache(cache)
+        _need_rows(k, "k", cache, cache.kv_heads, "T")
+        _need_rows(v, "v", cache, cache.kv_heads, "T")
+        if v.shape[0] != k.shape[0] or v.dtype is not k.dtype:
+            raise _BAD(f"k and v must have as many tokens and one type: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
+        _need_ints(slots, "slots", cache, torch.int64, (k.shape[0],))
+    ks, vs = k.stride(), v.stride()
+    _launch("komp_kv_write", cache, k.data_ptr(), v.data_ptr(), TYPES[k.dtype], slots.data_ptr(), k.shape[0], ks[0], ks[1],
+            vs[0], vs[1])  # fmt: skip
     return cache
+
+
+def _need_slots(slots, cache):
+    n = slots.shape[0] if isinstance(slots, torch.Tensor) and slots.dim() else 0
+    if not (type(cache) is KVCache and _ints_fit(slots, cache, _I64, n)):
+        _need_cache(cache)
+        _need_ints(slots, "slots", cache, torch.int64, (n,))
+    return n
 
 
 def read_into(cache, slots, k, v):
     """read() into preallocated contiguous k, v [T][kv_heads][head_dim] of one type."""
-    _need_cache(cache)
-    _need_ints(slots, "slots", cache, torch.int64, (slots.shape[0] if isinstance(slots, torch.Tensor) and slots.dim() else 0,))
+    n = _need_slots(slots, cache)
     for t, name in ((k, "k"), (v, "v")):
         _need_rows(t, name, cache, cache.kv_heads, "T")
-        if t.shape[0] != slots.shape[0] or not t.is_contiguous() or t.dtype is not k.dtype:
-            raise _BAD(f"{name} must be contiguous [{slots.shape[0]}][{cache.kv_heads}][{cache.head_dim}], k and v of one type")
-    _launch("komp_kv_read", cache, slots.data_ptr(), slots.shape[0], k.data_ptr(), v.data_ptr(), TYPES[k.dtype])
+        if t.shape[0] != n or not t.is_contiguous() or t.dtype is not k.dtype:
+            raise _BAD(f"{name} must be contiguous [{n}][{cache.kv_heads}][{cache.head_dim}], k and v of one type")
+    _launch("komp_kv_read", cache, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), TYPES[k.dtype])
 
 
 def read(cache, slots, dtype=torch.float32):
     """The keys and values that the cache holds at slots int64 [T], as (k, v) [T][kv_heads][head_dim] of dtype: each the
     product of its code and its block's scale, rounded once.  A slot outside the cache gives zeros."""
-    _need_cache(cache)
-    _need_ints(slots, "slots", cache, torch.int64, (slots.shape[0] if isinstance(slots, torch.Tensor) and slots.dim() else 0,))
+    n = _need_slots(slots, cache)
     if dtype not in TYPES:
         raise _BAD(f"dtype must be f32, f16 or bf16, got {dtype}")
-    shape = (slots.shape[0], cache.kv_heads, cache.head_dim)
-    k, v = (torch.empty(shape, dtype=dtype, device=slots.device) for _ in "kv")
-    _launch("komp_kv_read", cache, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(), TYPES[dtype])
+    shape = (n, cache.kv_heads, cache.head_dim)
+    k, v = cache.kq.new_empty(shape, dtype=dtype), cache.kq.new_empty(shape, dtype=dtype)
+    _launch("komp_kv_read", cache, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), TYPES[dtype])
     return k, v
 
 
-def attend_into(cache, q, out, tables, lengths, starts=None, *, max_queries=None, max_length=None, scale=None, softcap=0.0,
-                window=0, prefix=None, slopes=None, lse=None):  # fmt: skip
-    """attend() into a preallocated out [T][heads][head_dim] of q's type (rows contiguous, any strides between them) and,
-    when given, lse f32 [T][heads].  (A call over few rows and many keys still takes a workspace from torch.)"""
+def _check_attend(cache, q, out, tables, lengths, starts, max_queries, prefix, slopes, lse):
+    """Every check of an attention call's tensors, with its message."""
     _need_cache(cache)
     _need_rows(q, "q", cache, None, "T")
     t, heads = q.shape[0], q.shape[1]
     if heads < 1 or heads % cache.kv_heads:
         raise _BAD(f"q has {heads} heads, which must be a multiple of the cache's {cache.kv_heads}")
-    _need_rows(out, "out", cache, heads, t)
-    if out.shape[0] != t or out.dtype is not q.dtype:
-        raise _BAD(f"out must be {list(q.shape)} {q.dtype}, got {list(out.shape)} {out.dtype}")
+    if out is not None:
+        _need_rows(out, "out", cache, heads, t)
+        if out.shape[0] != t or out.dtype is not q.dtype:
+            raise _BAD(f"out must be {list(q.shape)} {q.dtype}, got {list(out.shape)} {out.dtype}")
     _need(tables, "tables", torch.int32, 2)
-    batch, cols = tables.shape
+    batch = tables.shape[0]
     if tables.get_device() != cache._device or (tables.numel() and tables.stride(1) != 1):
         raise _BAD("tables must be [sequences][pages] on the cache's device with contiguous rows")
     _need_ints(lengths, "lengths", cache, torch.int32, (batch,))
     if starts is None:
         if t != batch:
             raise _BAD(f"q has {t} rows for {batch} sequences: give starts, or one row a sequence")
-        max_queries = 1 if t else 0
     else:
         _need_ints(starts, "starts", cache, torch.int32, (batch + 1,))
-        max_queries = t if max_queries is None else max_queries
-        if not 0 <= max_queries <= t:
+        if max_queries is not None and not 0 <= max_queries <= t:
             raise _BAD(f"max_queries={max_queries} must be from 0 to q's {t} rows")
     if prefix is not None:
         _need_ints(prefix, "prefix", cache, torch.int32, (batch,))
@@ -187,20 +213,62 @@ def attend_into(cache, q, out, tables, lengths, starts=None, *, max_queries=None
         _need_ints(slopes, "slopes", cache, torch.float32, (heads,))
     if lse is not None:
         _need_ints(lse, "lse", cache, torch.float32, (t, heads))
-    scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
-    if not math.isfinite(scale):
+
+
+def _attend_fits(cache, q, tables, lengths, starts, max_queries, prefix, slopes):
+    """True for tensors that pass _check_attend (out and lse aside)."""
+    if not (type(cache) is KVCache and isinstance(q, _Tensor) and q.dim() == 3 and isinstance(tables, _Tensor)
+            and tables.is_cuda and tables.dtype is _I32 and tables.dim() == 2):  # fmt: skip
+        return False
+    t, heads = q.shape[0], q.shape[1]
+    batch = tables.shape[0]
+    return (heads > 0 and heads % cache.kv_heads == 0 and _rows_fit(q, cache, heads) and tables.stride(1) == 1
+            and tables.get_device() == cache._device and _ints_fit(lengths, cache, _I32, batch)
+            and (t == batch if starts is None else _ints_fit(starts, cache, _I32, batch + 1)
+                 and (max_queries is None or 0 <= max_queries <= t))
+            and (prefix is None or _ints_fit(prefix, cache, _I32, batch))
+            and (slopes is None or _ints_fit(slopes, cache, torch.float32, heads)))  # fmt: skip
+
+
+def _attend(cache, q, out, tables, lengths, starts, max_queries, max_length, scale, softcap, window, prefix, slopes, lse):
+    """Launch an attention call of checked tensors."""
+    t, heads = q.shape[0], q.shape[1]
+    batch, cols = tables.shape
+    if starts is None:
+        max_queries = 1 if t else 0
+    elif max_queries is None:
+        max_queries = t
+    if scale is None:
+        scale = cache._scale
+    elif not math.isfinite(scale):
         raise _BAD(f"scale={scale} must be finite")
     most = cols * cache.page
     max_length = most if max_length is None else max(0, min(int(max_length), most))
-    args = (TYPES[q.dtype], t, batch, heads, max_queries, max_length)
-    need = ctypes.c_int64()
-    _abi.call("komp_kv_attend_workspace", cache._ref, *args, ctypes.byref(need))
-    work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-    ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
-    _launch("komp_kv_attend", cache, q.data_ptr(), out.data_ptr(), ptr(lse), args[0], tables.data_ptr(), lengths.data_ptr(),
-            ptr(starts), ptr(prefix), ptr(slopes), t, batch, heads, q.stride(0), q.stride(1), out.stride(0), out.stride(1),
-            tables.stride(0), cols, max_queries, max_length, scale, float(softcap), window, ptr(work),
-            need.value)  # fmt: skip
+    key = (TYPES[q.dtype], t, batch, heads, max_queries, max_length)
+    need = cache._work.get(key)
+    if need is None:
+        v = ctypes.c_int64()
+        _abi.call("komp_kv_attend_workspace", cache._ref, *key, ctypes.byref(v))
+        if len(cache._work) >= 4096:
+            cache._work.clear()
+        need = cache._work[key] = v.value
+    work = None
+    if need:  # kept until the call is on the stream; torch hands the memory to later work of this stream only
+        work = cache.kq.new_empty(need)
+    qs, os, ts = q.stride(), out.stride(), tables.stride(0)
+    _launch("komp_kv_attend", cache, q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), key[0],
+            tables.data_ptr(), lengths.data_ptr(), None if starts is None else starts.data_ptr(),
+            None if prefix is None else prefix.data_ptr(), None if slopes is None else slopes.data_ptr(), t, batch, heads,
+            qs[0], qs[1], os[0], os[1], ts, cols, max_queries, max_length, scale, softcap, window,
+            None if work is None else work.data_ptr(), need)  # fmt: skip
+
+
+def attend_into(cache, q, out, tables, lengths, starts=None, *, max_queries=None, max_length=None, scale=None, softcap=0.0,
+                window=0, prefix=None, slopes=None, lse=None):  # fmt: skip
+    """attend() into a preallocated out [T][heads][head_dim] of q's type (rows contiguous, any strides between them) and,
+    when given, lse f32 [T][heads].  (A call over few rows and many keys still takes a workspace from torch.)"""
+    _check_attend(cache, q, out, tables, lengths, starts, max_queries, prefix, slopes, lse)
+    _attend(cache, q, out, tables, lengths, starts, max_queries, max_length, scale, softcap, window, prefix, slopes, lse)
 
 
 def attend(cache, q, tables, lengths, starts=None, *, max_queries=None, max_length=None, scale=None, softcap=0.0, window=0,
@@ -219,10 +287,9 @@ def attend(cache, q, tables, lengths, starts=None, *, max_queries=None, max_leng
 
     max_queries: the most rows of one sequence (T by default); rows past it are not computed.  max_length: an upper bound of
     the lengths that the launch is planned for (the tables' width by default); any value gives the right result."""
-    _need_cache(cache)
-    _need_rows(q, "q", cache, None, "T")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    attend_into(cache, q, out, tables, lengths, starts, max_queries=max_queries, max_length=max_length, scale=scale,
-                softcap=softcap, window=window, prefix=prefix, slopes=slopes, lse=lse)  # fmt: skip
+    if not _attend_fits(cache, q, tables, lengths, starts, max_queries, prefix, slopes):
+        _check_attend(cache, q, None, tables, lengths, starts, max_queries, prefix, slopes, None)
+    out = cache.kq.new_empty(q.shape, dtype=q.dtype)
+    lse = cache.kq.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
+    _attend(cache, q, out, tables, lengths, starts, max_queries, max_length, scale, softcap, window, prefix, slopes, lse)
     return (out, lse) if return_lse else out
