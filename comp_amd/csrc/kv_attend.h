@@ -417,7 +417,7 @@ struct Columns {
       }
       const float unit = __builtin_ldexpf(fabsf(a.scale), (SIGNED ? 0 : 24) - up);
       raw[ct] = a.cap > 0.f ? 2.f * unit / a.cap : unit;
-      fx[ct] = a.cap > 0.f || a.slopes ? 1.f : unit;
+      fx[ct] = a.cap > 0.f || a.slopes ? 1.f : fmaxf(unit, 0x1p-126f);
       neg[ct] = 0.f;
       lim[ct] = NONE;
       l[ct] = 0.f;
@@ -427,14 +427,14 @@ struct Columns {
   }
 
   // capped and biased scores from raw ones
-  __device__ __forceinline__ void shape(const AttendArgs& a, int ct, int key0, float (&y)[2][4]) const {
+  __device__ __forceinline__ void shape(const AttendArgs& a, int ct, int key0, float unit, float (&y)[2][4]) const {
     const float cap = a.cap * kLog2e;
-    const float back = static_cast<float>(pos[ct] - key0);
+    const float back = static_cast<float>(pos[ct] - key0), to = raw[ct] * unit;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float x = y[t][r] * raw[ct];
+        float x = y[t][r] * to;
         // cap tanh(s / cap), tanh u = 1 - 2 / (e^2u + 1)
         if (a.cap > 0.f) x = cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.f);
         y[t][r] = fmaf(-slope[ct], fabsf(back - (16 * t + r)), x);
@@ -442,7 +442,7 @@ struct Columns {
   }
 
   // M moves to the largest score so far, and what was summed with it
-  __device__ __forceinline__ void move(int off_now, const float (&y)[CT][2][4]) {
+  __device__ __forceinline__ void move(int off_now, float unit, const float (&y)[CT][2][4]) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float top = y[ct][0][0];
@@ -450,7 +450,7 @@ struct Columns {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, y[ct][t][r]);
-      top = quarters_max(top * fx[ct]);
+      top = quarters_max(top * (fx[ct] * unit));
       const float before = reference(ct);
       top = fmaxf(top, before + off);
       const float now = top - off_now;
@@ -460,20 +460,19 @@ struct Columns {
 #pragma unroll
       for (int i = 0; i < OT; ++i) acc[ct][i] *= by;
       neg[ct] = now == NONE ? 0.f : -now;
-      lim[ct] = now == NONE ? NONE : fx[ct] > 0.f ? (top + 8.f) / fx[ct] : __builtin_inff();
+      lim[ct] = now == NONE ? NONE : (top + 8.f) / fx[ct];
     }
     off = off_now;
   }
 
-  // Raw scores to probabilities 2^(x - M + ev), and the sums of 2^(x - M).
-  template <bool MASKED>
-  __device__ __forceinline__ void soften(const AttendArgs& a, int key0, int off_now, int ev, float (&y)[CT][2][4]) {
+  // Raw scores (in the tile's unit) to probabilities 2^(x - M + ev), and the sums of 2^(x - M).
+  __device__ __forceinline__ void soften(const AttendArgs& a, bool masked, int key0, int off_now, float unit, int ev, float (&y)[CT][2][4]) {
     const bool shaped = a.cap > 0.f || a.slopes != nullptr;
     bool go = off_now < off;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      if (shaped) shape(a, ct, key0, y[ct]);
-      if constexpr (MASKED) {
+      if (shaped) shape(a, ct, key0, unit, y[ct]);
+      if (masked) {  // (2^(-inf fx - M) is 0: fx is not)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -483,27 +482,23 @@ struct Columns {
           }
       }
     }
+    if (shaped) unit = 1.f;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const float top = fmaxf(fmaxf(fmaxf(y[ct][0][0], y[ct][0][1]), fmaxf(y[ct][0][2], y[ct][0][3])),
                               fmaxf(fmaxf(y[ct][1][0], y[ct][1][1]), fmaxf(y[ct][1][2], y[ct][1][3])));
-      go |= top > lim[ct];
+      go |= top * unit > lim[ct];
     }
-    if (__builtin_amdgcn_ballot_w64(go) != 0) move(off_now, y);
+    if (__builtin_amdgcn_ballot_w64(go) != 0) move(off_now, unit, y);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const float n = neg[ct] + ev;
+      const float f = fx[ct] * unit, n = neg[ct] + ev;
       float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float x = fmaf(y[ct][t][r], fx[ct], n);
-          if constexpr (MASKED) {
-            const int j = key0 + 16 * t + r;
-            if (j < span[ct].lo || j >= span[ct].hi) x = NONE;
-          }
-          y[ct][t][r] = __builtin_amdgcn_exp2f(x);
+          y[ct][t][r] = __builtin_amdgcn_exp2f(fmaf(y[ct][t][r], f, n));
           sum += y[ct][t][r];
         }
       l[ct] += __builtin_ldexpf(sum, -ev);
@@ -534,10 +529,9 @@ struct Columns {
     }
   }
 
-  // A tile of 32 keys from key `first` on.  MASKED: some column does not see some of them; a key that a column does not
+  // A tile of 32 keys from key `first` on.  masked: some column does not see some of them; a key that a column does not
   // see gets a P' of 0 there whatever its scale holds.
-  template <bool MASKED>
-  __device__ __forceinline__ void step(const AttendArgs& a, const KvTile<NB, KF, VF>& kv, int first, int lane) {
+  __device__ __forceinline__ void step(const AttendArgs& a, const KvTile<NB, KF, VF>& kv, bool masked, int first, int lane) {
     const int quarter = lane >> 4, key0 = first + quarter * 4;
     float y[CT][2][4];
     each<2>([&](auto tc) {
@@ -572,7 +566,7 @@ struct Columns {
 #pragma unroll
     for (int i = 0; i < KvTile<NB, KF, VF>::SW; ++i) {
       vs[i] = kv.vs[i];
-      if constexpr (MASKED) {
+      if (masked) {
         const int pair = min(i * 16 + (lane & 15), 4 * NB - 1) & 3, j = key0 + 16 * (pair >> 1) + (pair & 1);
         vs[i] &= (j >= all.lo && j < all.hi ? 0xFFFFu : 0u) | (j + 2 >= all.lo && j + 2 < all.hi ? 0xFFFF0000u : 0u);
       }
@@ -591,12 +585,12 @@ struct Columns {
       for (int o = 32; o > 0; o >>= 1) e = max(e, static_cast<unsigned>(__shfl_xor(static_cast<int>(e), o, 64)));
       off_now = __builtin_amdgcn_readfirstlane(min(off, 21 - static_cast<int>(max(e, 1u))));
     }
-    soften<MASKED>(a, key0, off_now, 0, y);
+    soften(a, masked, key0, off_now, 1.f, 0, y);
     unsigned ph[CT][4], keep[CT][4];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       if constexpr (MODE == KV_BF16) pack(y[ct], ph[ct]);
-      if constexpr (MASKED) seen_pairs(ct, key0, keep[ct]);
+      if (masked) seen_pairs(ct, key0, keep[ct]);
     }
     each<NB>([&](auto bc) {
       constexpr int b = bc.value;
@@ -611,7 +605,7 @@ struct Columns {
           } else {
             weigh(y[ct][i >> 1][i & 1], y[ct][i >> 1][2 + (i & 1)], d, w[ct], i);
           }
-          if constexpr (MASKED) {
+          if (masked) {
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) w[ct][part][i] &= keep[ct][i];
           }
@@ -669,8 +663,8 @@ struct Pages {
       : table(a.tables + seq * a.table_stride), pages(a.c.pages), heads(a.c.heads), h(h), log2(a.c.page_log2 - 5) {}
   __device__ __forceinline__ int64_t unit(int tile) const {
     const int page = table[tile >> log2];
-    if (page < 0 || page >= pages) return -1;
-    return ((static_cast<int64_t>(page) * heads + h) << log2) + (tile & ((1 << log2) - 1));
+    const int64_t u = ((static_cast<int64_t>(page) * heads + h) << log2) + (tile & ((1 << log2) - 1));
+    return ((page < 0) | (page >= pages)) ? -1 : u;
   }
 };
 
@@ -718,7 +712,7 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {
       const int now = tile + i * W, next = now + DEEP * W;
-      if (unit[i] >= 0) cols.template step<false>(a, kv[i], now * 32, lane);
+      if (unit[i] >= 0) cols.step(a, kv[i], false, now * 32, lane);
       unit[i] = next < full1 ? pages.unit(next) : -1;
       if (unit[i] >= 0) kv[i].load(a.c, unit[i], lane);
     }
@@ -731,7 +725,7 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
     if (u < 0) continue;
     KvTile<NB, KF, VF> one;
     one.load(a.c, u, lane);
-    cols.template step<true>(a, one, tile * 32, lane);
+    cols.step(a, one, true, tile * 32, lane);
   }
 
   // join the waves, a column tile at a time: the upper half hands its sums to the lower half, then wave 1 to wave 0

@@ -20,7 +20,13 @@ hipError_t launch_attend_mode(const AttendArgs& a, const AttendPlan& plan, int b
     }
     return hipGetLastError();
   };
-  if (plan.many) return launch_attend_many<NB, KF, VF, MODE>(a, dim3(grid.y, grid.z, grid.x), stream);
+  if (plan.many) {
+    const dim3 heads_first(grid.y, grid.z, grid.x);
+    if constexpr (MODE == KV_BF16) {
+      if (a.lse == nullptr) return launch_attend_many<NB, KF, VF, MODE, true>(a, heads_first, stream);
+    }
+    return launch_attend_many<NB, KF, VF, MODE, false>(a, heads_first, stream);
+  }
   return run(kv_attend_few_kernel<NB, KF, VF, MODE>, kAttendWaves * 64);
 }
 template <int NB, int KF, int VF>

@@ -6,18 +6,19 @@
 // KEYS keys, one barrier a buffer: while a wave computes with one, it unpacks its share of the next and has the codes
 // after that in flight.
 //
-// Key operands hold the codes, exact; their scales lie beside them and multiply the partial dots as in Columns::step.  So do
-// value operands for f16 and f32 queries.  For bf16 queries value operands hold d * code, rounded to f16 after a power of
-// two that brings the tile's largest scale to [1, 2) and that the probabilities' exponent takes back: 2^-12 of a value, an
-// eighth of what bf16 keeps of the result, for a quarter of the instructions a column.  A value block whose scale is no
-// number is held as zeros then, and makes NaN of its channels in the columns that see it.
+// f16 and f32 queries: the operands hold the codes, exact; the scales lie beside them and are used as in Columns::step.
+// bf16 queries: the operands hold d * code, rounded to f16 after a power of two that brings the tile's largest scale to
+// [1, 2) and that the scores' factor or the probabilities' exponent takes back.  2^-12 of a key or value is an eighth of
+// what bf16 keeps of the result, and saves the f32 products of the partial dots and of the probabilities, half of a
+// column's instructions.  (Where the logarithms of the sums are asked for, in f32, keys stay exact: KEYS_SCALED.)  A value
+// block whose scale is no number is held as zeros then, and makes NaN of its channels in the columns that see it.
 #pragma once
 
 #include "kv_attend.h"
 
 namespace komp {
 
-template <int NB, int KF, int VF, int MODE>
+template <int NB, int KF, int VF, int MODE, bool KEYS_SCALED>
 struct Many {
   // two column tiles a wave halve the operand reads and the unpacking a column, where the registers (of two waves a SIMD)
   // hold their queries and sums: not f32 queries, in two parts, nor 256 channels
@@ -32,14 +33,13 @@ struct Many {
   static constexpr int TURNS = (CHUNKS + WAVES - 1) / WAVES;  // chunks of one wave
   static constexpr int SW = (16 * NB + 63) / 64;              // dwords a lane of a half's scales, in a wave
   using Cols = Columns<NB, KF, VF, MODE, CT, true>;
-  using Units = int64_t[HALVES];  // where the halves of a tile lie, -1 for nowhere
 
   struct Shared {
     f16x8 k[2][HALVES * 2 * NB][64];  // [16 tokens][block]
     f16x8 v[2][HALVES * NB * 2][64];  // [32 tokens][block][channels 0..15, 16..31]
-    unsigned ks[2][HALVES][16 * NB];
-    unsigned vs[2][SCALED ? 1 : HALVES][16 * NB];
-    unsigned most[4];                          // of the values' scales: the largest exponent field
+    unsigned ks[2][KEYS_SCALED ? 1 : HALVES][KEYS_SCALED ? 1 : 16 * NB];
+    unsigned vs[2][SCALED ? 1 : HALVES][SCALED ? 1 : 16 * NB];
+    unsigned most[4][2];                       // the largest exponent field of the values' and the keys' scales
     unsigned bad[4][SCALED ? 1 + HALVES * NB : 1];  // whether there are, and which, tokens of a half and block whose value
                                                     // scale is no number
   };
@@ -54,23 +54,28 @@ struct Many {
 
   static __device__ __forceinline__ int half_of(int c) { return c < KCHUNKS ? c / KG >> 1 : (c - KCHUNKS) / VG; }
 
-  __device__ __forceinline__ void load(const KvCache& cache, const Units& unit, int wave, int lane) {
-    auto of = [&](int half) {
-      int64_t u = unit[0];
-#pragma unroll
-      for (int j = 1; j < HALVES; ++j) u = half == j ? unit[j] : u;
-      return u;
-    };
+  // `unit(half)`: where a half of the tile lies, -1 for nowhere
+  template <typename F>
+  __device__ __forceinline__ void load(const KvCache& cache, F&& unit, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
       const int c = i * WAVES + wave;
-      const int64_t u = c < CHUNKS ? of(half_of(c)) : -1;
+      const int64_t u = c < CHUNKS ? unit(half_of(c)) : -1;
       there[i] = u >= 0;
       if (!there[i]) continue;
       if (c < KCHUNKS) {
         const int t16 = c / KG & 1, g = c % KG;
         load_words<KD, KD>(cache.kq + u * (NB * 32 * kv_code_bytes(KF)) + t16 * (NB * 16 * kv_code_bytes(KF)) + (g * 64 + lane) * (KD * 4),
                            chunk[i].code);
+        if constexpr (KEYS_SCALED) {
+          const uint16_t* sp = cache.ks + u * (32 * NB) + (t16 * 16 + (lane & 15)) * NB + g * KB;
+          if constexpr (KB % 2 == 0) {
+            load_words<KB / 2, KB / 2>(reinterpret_cast<const uint8_t*>(sp), chunk[i].scale);
+          } else {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) chunk[i].scale[b] = sp[b];
+          }
+        }
       } else {
         const int g = (c - KCHUNKS) % VG;
         load_words<VD, VD>(cache.vq + u * (NB * 32 * kv_code_bytes(VF)) + (g * 64 + lane) * (VD * 4), chunk[i].code);
@@ -80,12 +85,12 @@ struct Many {
         }
       }
     }
-    if (wave < HALVES) {
-      const int64_t u = of(wave);
+    if (!(KEYS_SCALED && SCALED) && wave < HALVES) {
+      const int64_t u = unit(wave);
 #pragma unroll
       for (int i = 0; i < SW; ++i) {
         const int at = min(i * 64 + lane, 16 * NB - 1);
-        ks[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.ks)[u * (16 * NB) + at];
+        if constexpr (!KEYS_SCALED) ks[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.ks)[u * (16 * NB) + at];
         if constexpr (!SCALED) vs[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.vs)[u * (16 * NB) + at];
       }
     }
@@ -98,15 +103,27 @@ struct Many {
     return (token < left ? 0xFFFFu : 0u) | (token + 2 < left ? 0xFFFF0000u : 0u);
   }
 
-  // The loaded value scales: those of keys from `length` on become 0, and so do such as are no numbers, which go into
-  // bad[slot]; the largest exponent goes to most[slot].  (f16 and f32 queries: their products stay numbers by the masks.)
+  // The loaded scales: those of keys from `length` on become 0, and so do values' that are no numbers, which go into
+  // bad[slot]; the largest exponents go to most[slot].  (Scales beside the operands: the masks keep the products numbers.)
   __device__ __forceinline__ void look(Shared& sh, int slot, int first, int length, int wave, int lane) {
-    unsigned e = 0;
+    unsigned e = 0, ek = 0;
     if constexpr (SCALED) {
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int c = i * WAVES + wave;
-        if (c < KCHUNKS || !there[i]) continue;
+        if (!there[i]) continue;
+        if (c < KCHUNKS) {
+          if constexpr (KEYS_SCALED) {
+            const bool in = (c / KG & 1) * 16 + (lane & 15) < length - first - half_of(c) * 32;
+#pragma unroll
+            for (int b = 0; b < (KB % 2 == 0 ? KB / 2 : KB); ++b) {
+              chunk[i].scale[b] = in ? chunk[i].scale[b] : 0u;
+              const unsigned lo = chunk[i].scale[b] & 0x7C00u, hi = chunk[i].scale[b] >> 16 & 0x7C00u;
+              ek = max(ek, max(lo == 0x7C00u ? 0u : lo, hi == 0x7C00u ? 0u : hi));
+            }
+          }
+          continue;
+        }
         const int left = length - first - half_of(c) * 32;
         unsigned worst = 0;
 #pragma unroll
@@ -145,16 +162,22 @@ struct Many {
     int top = static_cast<int>(e);
     if constexpr (!SCALED) top = row16_max_i(top);  // (value operands: a row's lanes have the same scales)
     top = static_cast<int>(quarters_max(static_cast<float>(top)));
-    if (top && lane == 0) atomicMax(&sh.most[slot], static_cast<unsigned>(top));
+    if (top && lane == 0) atomicMax(&sh.most[slot][0], static_cast<unsigned>(top));
+    if constexpr (KEYS_SCALED) {
+      const int k = row16_max_i(static_cast<int>(ek >> 10));  // (the quarters have the same keys)
+      if (k && lane == 0) atomicMax(&sh.most[slot][1], static_cast<unsigned>(k));
+    }
   }
 
   // the loaded codes as operands in buffer `buf`
   __device__ __forceinline__ void unpack(Shared& sh, int buf, int slot, int wave, int lane) {
-    f16x2 fv = {};
-    if constexpr (SCALED) {  // 2^(15 - field)
-      const _Float16 v = static_cast<_Float16>(__builtin_ldexpf(1.f, 15 - static_cast<int>(max(sh.most[slot], 1u))));
-      fv = f16x2{v, v};
-    }
+    f16x2 fv = {}, fk = {};  // 2^(15 - field)
+    auto power = [&](int which) {
+      const _Float16 f = static_cast<_Float16>(__builtin_ldexpf(1.f, 15 - static_cast<int>(max(sh.most[slot][which], 1u))));
+      return f16x2{f, f};
+    };
+    if constexpr (SCALED) fv = power(0);
+    if constexpr (KEYS_SCALED) fk = power(1);
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
       const int c = i * WAVES + wave;
@@ -163,8 +186,15 @@ struct Many {
         f16x8* to = &sh.k[buf][c / KG * NB + c % KG * KB][lane];
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-          if constexpr (KF == KV_Q4_0) to[b * 64] = key_codes<true, KF>(chunk[i].code[b], 0u);
-          else to[b * 64] = key_codes<true, KF>(chunk[i].code[2 * b], chunk[i].code[2 * b + 1]);
+          f16x8 x;
+          if constexpr (KF == KV_Q4_0) x = key_codes<true, KF>(chunk[i].code[b], 0u);
+          else x = key_codes<true, KF>(chunk[i].code[2 * b], chunk[i].code[2 * b + 1]);
+          if constexpr (KEYS_SCALED) {
+            const _Float16 d = KB % 2 == 0 ? as_f16x2(chunk[i].scale[b >> 1])[b & 1] : as_f16x2(chunk[i].scale[b])[0];
+            const f16x2 dd = f16x2{d, d} * fk;
+            x *= f16x8{dd[0], dd[0], dd[0], dd[0], dd[0], dd[0], dd[0], dd[0]};
+          }
+          to[b * 64] = x;
         }
       } else {
         f16x8* to = &sh.v[buf][(c - KCHUNKS) * VB * 2][lane];
@@ -186,28 +216,27 @@ struct Many {
         }
       }
     }
-    if (wave < HALVES) {
+    if (!(KEYS_SCALED && SCALED) && wave < HALVES) {
 #pragma unroll
       for (int i = 0; i < SW; ++i) {
         const int at = min(i * 64 + lane, 16 * NB - 1);
-        sh.ks[buf][wave][at] = ks[i];
+        if constexpr (!KEYS_SCALED) sh.ks[buf][wave][at] = ks[i];
         if constexpr (!SCALED) sh.vs[buf][wave][at] = vs[i];
       }
     }
   }
 
   // a wave's columns over half `half` of the tile in `buf`, its keys from `first` on
-  template <bool MASKED>
-  static __device__ __forceinline__ void step(Cols& cols, const AttendArgs& a, const Shared& sh, int buf, int slot, int half,
-                                              int first, int lane) {
+  static __device__ __forceinline__ void step(Cols& cols, const AttendArgs& a, const Shared& sh, bool masked, int buf, int slot,
+                                              int half, int first, int lane) {
     constexpr int ROWS = (4 * NB + 15) / 16;  // a quarter's scales: dwords a lane of its 16
     const int quarter = lane >> 4, key0 = first + quarter * 4;
-    const int e = __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot], 1u)));
-    unsigned ks[ROWS];
+    const int e = __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][0], 1u)));
+    unsigned ks[ROWS] = {};
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const int at = min(i * 16 + (lane & 15), 4 * NB - 1), t = at / (2 * NB);
-      ks[i] = sh.ks[buf][half][t * 8 * NB + quarter * 2 * NB + at - t * 2 * NB];
+      if constexpr (!KEYS_SCALED) ks[i] = sh.ks[buf][half][t * 8 * NB + quarter * 2 * NB + at - t * 2 * NB];
     }
     float y[CT][2][4];
     each<2>([&](auto tc) {
@@ -218,12 +247,18 @@ struct Many {
         const f16x8 k = sh.k[buf][(half * 2 + t) * NB + b][lane];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          c[ct][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+          f32x4& x = c[ct][KEYS_SCALED ? 0 : b];
+          if (!KEYS_SCALED || b == 0) x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int p = 0; p < Cols::PARTS; ++p) c[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, cols.qf[ct][b][p], c[ct][b], 0, 0, 0);
+          for (int p = 0; p < Cols::PARTS; ++p) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, cols.qf[ct][b][p], x, 0, 0, 0);
         }
       }
-      each<2 * NB>([&](auto jc) {
+      if constexpr (KEYS_SCALED) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[ct][t][r] = c[ct][0][r];
+      } else each<2 * NB>([&](auto jc) {
         constexpr int j = jc.value, at = t * 2 * NB + j;
         const f16x2 d = as_f16x2(row_lane<at % 16>(ks[at / 16]));
 #pragma unroll
@@ -235,7 +270,10 @@ struct Many {
         }
       });
     });
-    cols.template soften<MASKED>(a, key0, min(cols.off, 21 - e), SCALED ? e - 15 : 0, y);
+    float unit = 1.f;
+    if constexpr (KEYS_SCALED)
+      unit = __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][1], 1u))) - 15);
+    cols.soften(a, masked, key0, min(cols.off, 21 - e), unit, SCALED ? e - 15 : 0, y);
     if constexpr (SCALED) {
       unsigned w[CT][4];
 #pragma unroll
@@ -252,7 +290,7 @@ struct Many {
       unsigned vs[ROWS], keep[CT][4];
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) vs[i] = sh.vs[buf][half][quarter * 4 * NB + min(i * 16 + (lane & 15), 4 * NB - 1)];
-      if constexpr (MASKED) {
+      if (masked) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) cols.seen_pairs(ct, key0, keep[ct]);
       }
@@ -265,7 +303,7 @@ struct Many {
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
             Cols::weigh(y[ct][i >> 1][i & 1], y[ct][i >> 1][2 + (i & 1)], d, w[ct], i);
-            if constexpr (MASKED) {
+            if (masked) {
 #pragma unroll
               for (int p = 0; p < Cols::PARTS; ++p) w[ct][p][i] &= keep[ct][i];
             }
@@ -304,12 +342,14 @@ struct Many {
   }
 };
 
-template <int NB, int KF, int VF, int MODE>
-__global__ void __launch_bounds__((64 * Many<NB, KF, VF, MODE>::WAVES), (Many<NB, KF, VF, MODE>::WAVES / 4)) kv_attend_many_kernel(const AttendArgs a) {
-  using M = Many<NB, KF, VF, MODE>;
+template <int NB, int KF, int VF, int MODE, bool KEYS_SCALED>
+__global__ void __launch_bounds__((64 * Many<NB, KF, VF, MODE, KEYS_SCALED>::WAVES), (Many<NB, KF, VF, MODE, KEYS_SCALED>::WAVES / 4))
+kv_attend_many_kernel(const AttendArgs a) {
+  using M = Many<NB, KF, VF, MODE, KEYS_SCALED>;
   extern __shared__ __attribute__((aligned(16))) unsigned char shared_bytes[];
   typename M::Shared& sh = *reinterpret_cast<typename M::Shared*>(shared_bytes);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __builtin_assume(wave >= 0 && wave < M::WAVES);
   const int h = blockIdx.x, seq = blockIdx.y, split = blockIdx.z / a.groups;
   // the groups of the latest positions, which see the most keys, begin first, those of all heads and sequences together
   const int group0 = (a.groups - 1 - (static_cast<int>(blockIdx.z) - split * a.groups)) * (M::WAVES * M::COLS);
@@ -328,62 +368,62 @@ __global__ void __launch_bounds__((64 * Many<NB, KF, VF, MODE>::WAVES), (Many<NB
   const Span w0 = s.seen(a, any ? col0 / a.group : 0), w1 = s.seen(a, any ? (min(s.cols, col0 + M::COLS) - 1) / a.group : 0);
 
   const Pages pages(a, seq, h);
-  auto units = [&](int tile, typename M::Units& u) {  // -> a bit for each half that lies somewhere
+  auto unit = [&](int tile, int half) -> int64_t {
+    // (no branch, so that a tile's table entries are loaded together; there is a first key where there is a tile)
+    const int at = tile * M::HALVES + half, last = (s.length - 1) >> 5;
+    const int64_t u = pages.unit(min(at, last));
+    return ((tile < tile1) & (at <= last)) ? u : -1;
+  };
+  auto halves = [&](int tile) {  // a bit for each half that lies somewhere
     unsigned there = 0;
 #pragma unroll
-    for (int i = 0; i < M::HALVES; ++i) {
-      const int at = tile * M::HALVES + i;
-      u[i] = tile < tile1 && at * 32 < s.length ? pages.unit(at) : -1;
-      there |= u[i] < 0 ? 0u : 1u << i;
-    }
+    for (int i = 0; i < M::HALVES; ++i) there |= unit(tile, i) < 0 ? 0u : 1u << i;
     return there;
   };
-  M m;
-  typename M::Units unit;
-  if (threadIdx.x < 4) sh.most[threadIdx.x] = 0;
-  constexpr int BAD = M::SCALED ? 1 + M::HALVES * NB : 0;
-  if (threadIdx.x < 4 * BAD) (&sh.bad[0][0])[threadIdx.x] = 0;
-  unsigned now = units(tile0, unit);
-  m.load(a.c, unit, wave, lane);
   typename M::Cols cols;
   cols.all = Span{w0.lo, w1.hi};
   cols.begin(a, s, h, col0, lane);
-  __syncthreads();
-  m.look(sh, 0, tile0 * M::KEYS, s.length, wave, lane);
-  __syncthreads();
-  m.unpack(sh, 0, 0, wave, lane);
-  unsigned next = units(tile0 + 1, unit);
-  m.load(a.c, unit, wave, lane);
-  m.look(sh, 1, (tile0 + 1) * M::KEYS, s.length, wave, lane);
-  __syncthreads();
-  for (int tile = tile0; tile < tile1; ++tile) {
-    // most[] and bad[]: this tile's are in slot i, the next one's in i + 1, the one after's are filled in i + 2, and i + 3,
-    // last read a turn ago, is cleared for the turn to come
-    const int i = tile - tile0, buf = i & 1;
-    if (threadIdx.x == 0) sh.most[(i + 3) & 3] = 0;
-    if (threadIdx.x < BAD) sh.bad[(i + 3) & 3][threadIdx.x] = 0;
-    m.unpack(sh, buf ^ 1, (i + 1) & 3, wave, lane);
-    const unsigned after = units(tile + 2, unit);
-    m.load(a.c, unit, wave, lane);
-    const bool spoilt = M::SCALED && __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) != 0;
-#pragma unroll 1
-    for (int half = 0; half < M::HALVES; ++half) {
-      const int first = tile * M::KEYS + half * 32;
-      if (!any || first >= w1.hi || first + 32 <= w0.lo || !(now >> half & 1)) continue;
-      if (first >= w1.lo && first + 32 <= w0.hi)
-        M::template step<false>(cols, a, sh, buf, i & 3, half, first, lane);
-      else
-        M::template step<true>(cols, a, sh, buf, i & 3, half, first, lane);
-    }
-    if (spoilt) {
-#pragma unroll 1
-      for (int half = 0; half < M::HALVES; ++half)
-        if (any && (now >> half & 1)) M::spoil(cols, sh, i & 3, half, tile * M::KEYS + half * 32);
-    }
-    m.look(sh, (i + 2) & 3, (tile + 2) * M::KEYS, s.length, wave, lane);
-    now = next;
-    next = after;
+  if (tile0 < tile1) {
+    M m;
+    if (threadIdx.x < 8) sh.most[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    constexpr int BAD = M::SCALED ? 1 + M::HALVES * NB : 0;
+    if (threadIdx.x < 4 * BAD) (&sh.bad[0][0])[threadIdx.x] = 0;
+    unsigned now = halves(tile0);
+    m.load(a.c, [&](int half) { return unit(tile0, half); }, wave, lane);
     __syncthreads();
+    m.look(sh, 0, tile0 * M::KEYS, s.length, wave, lane);
+    __syncthreads();
+    m.unpack(sh, 0, 0, wave, lane);
+    unsigned next = halves(tile0 + 1);
+    m.load(a.c, [&](int half) { return unit(tile0 + 1, half); }, wave, lane);
+    m.look(sh, 1, (tile0 + 1) * M::KEYS, s.length, wave, lane);
+    __syncthreads();
+    for (int tile = tile0; tile < tile1; ++tile) {
+      // most[] and bad[]: this tile's are in slot i, the next one's in i + 1, the one after's are filled in i + 2, and i + 3,
+      // last read a turn ago, is cleared for the turn to come
+      const int i = tile - tile0, buf = i & 1;
+      if (threadIdx.x < 2) sh.most[(i + 3) & 3][threadIdx.x] = 0;
+      if (threadIdx.x < BAD) sh.bad[(i + 3) & 3][threadIdx.x] = 0;
+      m.unpack(sh, buf ^ 1, (i + 1) & 3, wave, lane);
+      const unsigned after = halves(tile + 2);
+      m.load(a.c, [&](int half) { return unit(tile + 2, half); }, wave, lane);
+      const bool spoilt = M::SCALED && __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) != 0;
+#pragma unroll 1
+      for (int half = 0; half < M::HALVES; ++half) {
+        const int first = tile * M::KEYS + half * 32;
+        if (!any || first >= w1.hi || first + 32 <= w0.lo || !(now >> half & 1)) continue;
+        M::step(cols, a, sh, first < w1.lo || first + 32 > w0.hi, buf, i & 3, half, first, lane);
+      }
+      if (spoilt) {
+#pragma unroll 1
+        for (int half = 0; half < M::HALVES; ++half)
+          if (any && (now >> half & 1)) M::spoil(cols, sh, i & 3, half, tile * M::KEYS + half * 32);
+      }
+      m.look(sh, (i + 2) & 3, (tile + 2) * M::KEYS, s.length, wave, lane);
+      now = next;
+      next = after;
+      __syncthreads();
+    }
   }
   if (!any) return;
 #pragma unroll
@@ -391,18 +431,19 @@ __global__ void __launch_bounds__((64 * Many<NB, KF, VF, MODE>::WAVES), (Many<NB
   cols.store(a, s, h, col0, split, lane);
 }
 
-template <int NB, int KF, int VF, int MODE>
+template <int NB, int KF, int VF, int MODE, bool KEYS_SCALED>
 hipError_t launch_attend_many(const AttendArgs& a, const dim3& grid, hipStream_t stream) {
+  using M = Many<NB, KF, VF, MODE, KEYS_SCALED>;
   static std::atomic<unsigned> limit[kMaxDevices];
-  const auto kern = kv_attend_many_kernel<NB, KF, VF, MODE>;
-  constexpr size_t bytes = sizeof(typename Many<NB, KF, VF, MODE>::Shared);
+  const auto kern = kv_attend_many_kernel<NB, KF, VF, MODE, KEYS_SCALED>;
+  constexpr size_t bytes = sizeof(typename M::Shared);
   const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), bytes, limit);
   if (e != hipSuccess) return e;
   const Timing tm = timing_slot(KIND_PROBE);
   if (tm.on) {
-    hipExtLaunchKernelGGL(kern, grid, dim3(64 * Many<NB, KF, VF, MODE>::WAVES), bytes, stream, tm.start, tm.stop, 0, a);
+    hipExtLaunchKernelGGL(kern, grid, dim3(64 * M::WAVES), bytes, stream, tm.start, tm.stop, 0, a);
   } else {
-    hipLaunchKernelGGL(kern, grid, dim3(64 * Many<NB, KF, VF, MODE>::WAVES), bytes, stream, a);
+    hipLaunchKernelGGL(kern, grid, dim3(64 * M::WAVES), bytes, stream, a);
   }
   return hipGetLastError();
 }
