@@ -256,12 +256,6 @@ __device__ constexpr int key_place(int e) {
   return KF == KV_Q4_0 ? n4[e] : n8[e];
 }
 
-__device__ __forceinline__ float load_query(const void* q, int type, int64_t i) {
-  if (type == KV_F32) return static_cast<const float*>(q)[i];
-  const uint16_t u = static_cast<const uint16_t*>(q)[i];
-  return type == KV_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, u)) : __uint_as_float(static_cast<unsigned>(u) << 16);
-}
-
 // four consecutive channels of an output row
 __device__ __forceinline__ void store_out(void* out, int type, bool wide, int64_t i, f32x4 o) {
   typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
@@ -348,8 +342,40 @@ struct Columns {
   // M of column ct (-inf before anything was seen)
   __device__ __forceinline__ float reference(int ct) const { return lim[ct] == NONE ? NONE : -neg[ct]; }
 
-  __device__ __forceinline__ void begin(const AttendArgs& a, const Sequence& s, int h, int col0, int lane) {
+  // a lane's query channels, as they are in memory: the loads are under way before the keys', which take longer
+  struct Raw {
+    u32x4 w[CT][NB][PREC ? 2 : 1];
+  };
+  __device__ __forceinline__ void fetch(const AttendArgs& a, const Sequence& s, int h, int col0, int lane, Raw& q) const {
     const int quarter = lane >> 4;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      int64_t row;
+      int head;
+      const bool live = place(a, s, h, col0, ct, lane, row, head);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int64_t at = row * a.q_stride_t + head * a.q_stride_h + b * 32 + quarter * 8;
+#pragma unroll
+        for (int i = 0; i < (PREC ? 2 : 1); ++i) q.w[ct][b][i] = u32x4{0, 0, 0, 0};
+        if (!live) continue;
+        if (a.wide_q) {
+          const u32x4* p = PREC ? reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + at)
+                                : reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
+#pragma unroll
+          for (int i = 0; i < (PREC ? 2 : 1); ++i) q.w[ct][b][i] = p[i];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if constexpr (PREC) q.w[ct][b][e >> 2][e & 3] = static_cast<const unsigned*>(a.q)[at + e];
+            else q.w[ct][b][0][e >> 1] |= static_cast<unsigned>(static_cast<const uint16_t*>(a.q)[at + e]) << (16 * (e & 1));
+          }
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void begin(const AttendArgs& a, const Sequence& s, int h, int col0, int lane, const Raw& q) {
     off = PREC ? 20 : 6;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -365,33 +391,15 @@ struct Columns {
       const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const int64_t at = row * a.q_stride_t + head * a.q_stride_h + b * 32 + quarter * 8;
-        if (!live) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[b][e] = 0.f;
-        } else if (a.wide_q) {
-          if constexpr (PREC) {
-            const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at);
-            const f32x4 x = p[0], y = p[1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[b][e] = x[e], v[b][4 + e] = y[e];
-          } else {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const unsigned u = e & 1 ? x[e >> 1] >> 16 : x[e >> 1] & 0xFFFFu;
-              v[b][e] = MODE == KV_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u)))
-                                       : __uint_as_float(u << 16);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[b][e] = load_query(a.q, MODE, at + e);
-        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          top = fmaxf(top, fabsf(v[b][e]));
-          v[b][e] *= sign;
+          const unsigned w = PREC ? q.w[ct][b][PREC ? e >> 2 : 0][e & 3] : q.w[ct][b][0][e >> 1];
+          const unsigned u = e & 1 ? w >> 16 : w & 0xFFFFu;
+          const float x = PREC            ? __uint_as_float(w)
+                          : MODE == KV_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u)))
+                                           : __uint_as_float(u << 16);
+          top = fmaxf(top, fabsf(x));
+          v[b][e] = x * sign;
         }
       }
       top = quarters_max(top);
@@ -683,16 +691,22 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
   using Cols = Columns<NB, KF, VF, MODE, CT, (Few<NB, KF, VF, MODE>::SIGNED || MODE == KV_F32)>;
   constexpr int COLS = Cols::COLS, OT = Cols::OT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y, seq = blockIdx.z, split = blockIdx.x / a.groups, col0 = (blockIdx.x - split * a.groups) * COLS;
+  const int h = blockIdx.y, seq = blockIdx.z, split = a.groups == 1 ? blockIdx.x : blockIdx.x / a.groups;
+  const int col0 = (blockIdx.x - split * a.groups) * COLS;
   const Sequence s(a, seq);
   if (col0 >= s.cols) return;
+  Cols cols;
+  typename Cols::Raw query;
+  cols.fetch(a, s, h, col0, lane, query);
   const Span s0 = s.seen(a, col0 / a.group), s1 = s.seen(a, (min(s.cols, col0 + COLS) - 1) / a.group);
   // the workgroup's tiles, and those of them that all columns see
   int tile0 = s0.lo >> 5, tile1 = (s1.hi + 31) >> 5;
   if (tile0 > tile1) tile0 = tile1 = 0;
-  const int per = (tile1 - tile0 + a.splits - 1) / a.splits;
-  tile0 = min(tile1, tile0 + split * per);
-  tile1 = min(tile1, tile0 + per);
+  if (a.splits > 1) {
+    const int per = (tile1 - tile0 + a.splits - 1) / a.splits;
+    tile0 = min(tile1, tile0 + split * per);
+    tile1 = min(tile1, tile0 + per);
+  }
   int full0 = max(tile0, (s1.lo + 31) >> 5), full1 = min(tile1, s0.hi >> 5);
   if (full0 >= full1) full0 = full1 = tile1;
 
@@ -705,9 +719,8 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
     unit[i] = tile < full1 ? pages.unit(tile) : -1;
     if (unit[i] >= 0) kv[i].load(a.c, unit[i], lane);
   }
-  Cols cols;
   cols.all = Span{s0.lo, s1.hi};
-  cols.begin(a, s, h, col0, lane);
+  cols.begin(a, s, h, col0, lane, query);
   for (int tile = full0 + wave; tile < full1; tile += DEEP * W) {
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {

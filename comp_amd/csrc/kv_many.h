@@ -382,7 +382,9 @@ kv_attend_many_kernel(const AttendArgs a) {
   };
   typename M::Cols cols;
   cols.all = Span{w0.lo, w1.hi};
-  cols.begin(a, s, h, col0, lane);
+  typename M::Cols::Raw query;
+  cols.fetch(a, s, h, col0, lane, query);
+  cols.begin(a, s, h, col0, lane, query);
   if (tile0 < tile1) {
     M m;
     if (threadIdx.x < 8) sh.most[threadIdx.x >> 1][threadIdx.x & 1] = 0;
