@@ -1228,6 +1228,9 @@ int kv_attend_call(const char* name, const komp_kv_cache* C, int type, int64_t T
   if (T < 0 || T > most) return fail(KOMP_EINVAL, "%s: T=%lld rows (0 to %lld)", name, static_cast<long long>(T), static_cast<long long>(most));
   if (max_queries < 0 || max_queries > T)
     return fail(KOMP_EINVAL, "%s: max_queries=%lld (0 to T=%lld)", name, static_cast<long long>(max_queries), static_cast<long long>(T));
+  if (max_queries * (heads / c.cache.heads) > INT64_C(1) << 23)
+    return fail(KOMP_EINVAL, "%s: max_queries=%lld rows of %lld heads a kv head (2^23 columns at most)", name,
+                static_cast<long long>(max_queries), static_cast<long long>(heads / c.cache.heads));
   if (max_length < 0 || max_length > INT64_C(0x7FFFFFFF) - 65536)
     return fail(KOMP_EINVAL, "%s: max_length=%lld", name, static_cast<long long>(max_length));
   c.type = type;

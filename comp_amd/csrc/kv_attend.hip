@@ -13,15 +13,23 @@ AttendPlan plan_of(const KvAttendCall& c) {
   const int64_t cols = c.max_queries * group;
   const int64_t units = static_cast<int64_t>(c.batch) * c.cache.heads;
   AttendPlan p;
-  p.many = cols > 32;
+  // The many-column kernel unpacks a key once for 256 columns rather than 16, but starts slower and fills a CU with one
+  // workgroup: 8 sequences of 4096 keys, 8 kv heads, bf16, 96 columns 70 us (few) and 59, 128 columns 70 and 74, f32 83 and
+  // 80, 91 and 86; 48 columns 37 and 65.
+  p.many = cols > 96;
   const int wide = p.many ? many_cols(c.cache.dim, c.type) : 16;
   p.groups = static_cast<int>((cols + wide - 1) / wide);
-  // Enough workgroups to fill the CUs (one of many columns each, four of the others), eight where unlike lengths have to
-  // even out (64 sequences of up to 8192 keys, 8 kv heads, bf16: 106 us with 1024 workgroups, 97 with 2048, 103 with
-  // 4096), and no split of less than two tiles a wave or two buffers.
-  const int64_t aim = p.many ? 256 : units * p.groups >= 256 ? 2048 : 1024;
+  // Enough workgroups to fill the CUs once (one of many columns each, three of few: 16 sequences of up to 8192 keys and 1-5
+  // rows, f32: 59 us with 512 workgroups, 50 with 768 and 1024), or where there are many sequences more, so that unlike
+  // lengths even out (64 sequences of up to 8192 keys, bf16: 106 us with 1024, 97 with 2048, 103 with 4096); and no split
+  // of less than two tiles a wave or two buffers.
+  const int64_t aim = p.many ? 256 : units * p.groups >= 256 ? 2048 : 768;
   const int64_t want = (aim + units * p.groups - 1) / (units * p.groups);
   const int64_t most = p.many ? c.max_length / 256 : (c.max_length + 31) / 32 / (2 * kAttendWaves);
+  if (c.rows * c.heads > 1 << 22) {  // rows that no sequence holds, most likely: the join has a workgroup for each row and head
+    p.splits = 1;
+    return p;
+  }
   p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits})));
   return p;
 }

@@ -261,8 +261,8 @@ typedef struct komp_kv_cache {
 } komp_kv_cache;
 
 /* Quantize K, V [T][heads][head_dim] into the T slots of SLOTS.  Codes and scales are ggml's (Q8_0 as komp_quant_q8_0, Q4_0
- * as ggml's quantize_row_q4_0_ref); a block that holds a NaN reads back as NaN.  A slot below 0 or past the cache leaves
- * its token out; of equal slots in one call, either token's bytes may stay, also in part. */
+ * as ggml's quantize_row_q4_0_ref); a block that holds a NaN reads back as NaN.  T * heads * head_dim is at most 2^32.  A slot
+ * below 0 or past the cache leaves its token out; of equal slots in one call, either token's bytes may stay, also in part. */
 int komp_kv_write(const komp_kv_cache* C, const void* K, const void* V, int type, const int64_t* SLOTS, int64_t T,
                   int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, void* stream);
 
@@ -279,7 +279,8 @@ int komp_kv_read(const komp_kv_cache* C, const int64_t* SLOTS, int64_t T, void* 
  *   OUT [T][heads][head_dim] = softmax over the visible keys times their values, 0 where none is visible
  *   LSE f32 [T][heads] (or NULL) = the natural logarithm of the sum of exp(score), -inf where none is visible
  * A page number that the cache does not have hides its keys; lengths past table_cols pages end there.  max_queries: at
- * least the most rows a sequence has (at most T); max_length: the longest length, for the plan alone (any value is right).
+ * least the most rows a sequence has (at most T, and
+ * 2^23 with the query heads of a kv head counted); max_length: the longest length, for the plan alone (any value is right).
  * WORK: komp_kv_attend_workspace bytes for the same arguments (0: may be NULL), 16-byte aligned, free again when the call
  * has run.  Rows of Q that no sequence holds get unspecified results. */
 int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE, int type, const int32_t* TABLES,
