@@ -459,3 +459,82 @@ def test_refusals():
         kv.write(None, k, k, slots)
     with pytest.raises(TypeError):
         kv.attend(cache, np.zeros((2, 4, 64)), tables, lengths)
+
+
+# ---- many columns, and what only their kernel does -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", kv.HEAD_DIMS)
+@pytest.mark.parametrize("kf,vf", PAIRS)
+@pytest.mark.parametrize("opts", [dict(), dict(softcap=20.0, window=130), dict(slopes=True, prefix=[150, 20])], ids=["plain", "cap", "bias"])
+def test_attend_many_bf16_without_lse(kf, vf, dim, opts):
+    """bf16 without the sums' logarithms scales the keys in the operands too."""
+    p = Problem([333, 75], [90, 60], 4, 2, dim, kf, vf, "bf16", seed=12)
+    opts = dict(opts)
+    if opts.get("slopes"):
+        opts["slopes"] = np.array([0.5, 0.125, 0.01, 0.0], np.float32)
+    dev = {k: p.dev(np.asarray(v, np.int32 if k == "prefix" else np.float32)) if k in ("prefix", "slopes") else v
+           for k, v in opts.items()}  # fmt: skip
+    p.check(kv.attend(*p.args(), max_queries=90, **dev), **opts)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kf,vf", PAIRS)
+@pytest.mark.parametrize("kind", ["tiny", "large", "mixed", "rising", "keys"])
+def test_attend_many_value_ranges(dtype, kf, vf, kind):
+    """Scales near f16's ends, far apart from token to token, and large and tiny keys, for many columns."""
+    scales = {"tiny": lambda r, n: np.full(n, 3e-4), "large": lambda r, n: np.full(n, 3000.0),
+              "mixed": lambda r, n: np.exp(r.uniform(-6, 8, n)), "rising": lambda r, n: np.exp(np.linspace(-6, 8, n)),
+              "keys": lambda r, n: np.ones(n)}  # fmt: skip
+    p = Problem([300, 90], [70, 70], 4, 2, 64, kf, vf, dtype, seed=13, v_scale=lambda r, n: scales[kind](r, n).astype(np.float32),
+                k_scale=2000.0 if kind == "keys" else 1.0)  # fmt: skip
+    scale = 0.125 / 2000 if kind == "keys" else 0.125
+    p.check(kv.attend(*p.args(), max_queries=70, scale=scale), scale=scale)
+    p.check(kv.attend(*p.args(), max_queries=70, scale=-scale), scale=-scale)
+    p.check(kv.attend(*p.args(), max_queries=70, scale=0.0), scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attend_many_nonfinite(dtype, dim):
+    """A token without numbers reaches the rows that see it, in the channels of its block, and no others."""
+    n, rows, at = 200, 80, 150  # the rows are positions 120 .. 199
+    p = Problem([n], [rows], 4, 2, dim, "q8_0", "q4_0", dtype, seed=14)
+    want = kv.attend(*p.args(), max_queries=rows)
+    bad_k, bad_v = normal((1, 2, dim), 15, dtype), normal((1, 2, dim), 16, dtype)
+    bad_v[0, :, 40] = float("nan")
+    kv.write(p.cache, bad_k, bad_v, p.slots[0][at : at + 1])
+    out = kv.attend(*p.args(), max_queries=rows)
+    sees = at - (n - rows)
+    assert torch.equal(out[:sees], want[:sees])
+    assert torch.isnan(out[sees:, :, 32:64]).all()
+    assert torch.isfinite(out[sees:, :, :32]).all() and torch.isfinite(out[sees:, :, 64:]).all()
+    bad_k[0, :, 3] = float("nan")
+    kv.write(p.cache, bad_k, bad_v, p.slots[0][at : at + 1])
+    out = kv.attend(*p.args(), max_queries=rows)
+    assert torch.equal(out[:sees], want[:sees]) and torch.isnan(out[sees:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [96, 128])
+def test_attend_many_splits_and_pages(dtype, dim):
+    """Splits of the keys, pages that the cache does not have, rows of no sequence, pages of 32 and 256 tokens."""
+    for page in (32, 256):
+        p = Problem([3000, 700], [60, 50], 4, 2, dim, "q4_0", "q4_0", dtype, page=page, seed=15)
+        for lse in (True, False):
+            got = kv.attend(*p.args(), max_queries=60, return_lse=lse)
+            p.check(*(got if lse else (got,)))
+    tables = p.tables.copy()
+    tables[0, 1], tables[0, 3] = -1, 2**31 - 1  # of 256 tokens
+    args = list(p.args())
+    args[2] = p.dev(tables)
+    out = kv.attend(*args, max_queries=60, prefix=p.dev(np.array([3000, 700], np.int32)))
+    left = np.r_[0:256, 512:768, 1024:3000]
+    prefix = [10**6, 10**6]
+    want, _ = R.attend(p.q.double().cpu().numpy(), [p.keys[0][left], p.keys[1]], [p.values[0][left], p.values[1]], p.counts, prefix=prefix)
+    assert np.abs(out.double().cpu().numpy() - want).max() <= TOL[dtype] * np.abs(p.values[0]).max()
+    # rows before and after those that `starts` gives to the sequences
+    more = torch.cat([p.q[:3], p.q, p.q[:5]])
+    args = list(p.args())
+    args[1], args[4] = more, p.dev(p.starts + 3)
+    p.check(kv.attend(*args, max_queries=60)[3:-5])
