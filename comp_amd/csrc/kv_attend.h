@@ -62,6 +62,8 @@ struct AttendArgs {
   bool wide_q;   // query rows may be loaded 16 bytes at a time
   bool wide_out; // output rows stored four elements at a time
   int splits;
+  int least;     // splits of any sequence with as many tiles
+  int per;       // tiles a split of longer ones
   int groups;    // column groups a sequence may have
   float* part_o;   // [split][row][head][dim]
   float2* part_m;  // [split][row][head]: M and l
@@ -72,6 +74,8 @@ struct AttendPlan {
   bool many;
   int groups;
   int splits;
+  int least;
+  int per;
 };
 
 hipError_t launch_attend_q4_q4(const AttendArgs& a, const AttendPlan& plan, int batch, hipStream_t stream);
@@ -632,6 +636,16 @@ struct Columns {
     });
   }
 
+  // the parts of a split without keys
+  __device__ __forceinline__ void store_none(const AttendArgs& a, const Sequence& s, int h, int col0, int split, int lane) const {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      int64_t row;
+      int head;
+      if (place(a, s, h, col0, ct, lane, row, head)) a.part_m[(split * a.rows + row) * a.heads + head] = float2{NONE, 0.f};
+    }
+  }
+
   // the columns' results, or their part of a split
   __device__ __forceinline__ void store(const AttendArgs& a, const Sequence& s, int h, int col0, int split, int lane) const {
     constexpr int D = NB * 32;
@@ -691,22 +705,30 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
   using Cols = Columns<NB, KF, VF, MODE, CT, (Few<NB, KF, VF, MODE>::SIGNED || MODE == KV_F32)>;
   constexpr int COLS = Cols::COLS, OT = Cols::OT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y, seq = blockIdx.z, split = a.groups == 1 ? blockIdx.x : blockIdx.x / a.groups;
-  const int col0 = (blockIdx.x - split * a.groups) * COLS;
+  const int h = blockIdx.y, seq = blockIdx.z, place = a.groups == 1 ? blockIdx.x : blockIdx.x / a.groups;
+  const int col0 = (blockIdx.x - place * a.groups) * COLS;
+  // workgroups go round the XCDs in order; so that the first splits, which are never empty, do not all meet on the same one,
+  // a sequence and head begins with a split of its own
+  const int split = a.splits == 1 ? 0 : (place + h + seq) % a.splits;
   const Sequence s(a, seq);
   if (col0 >= s.cols) return;
   Cols cols;
-  typename Cols::Raw query;
-  cols.fetch(a, s, h, col0, lane, query);
   const Span s0 = s.seen(a, col0 / a.group), s1 = s.seen(a, (min(s.cols, col0 + COLS) - 1) / a.group);
   // the workgroup's tiles, and those of them that all columns see
   int tile0 = s0.lo >> 5, tile1 = (s1.hi + 31) >> 5;
   if (tile0 > tile1) tile0 = tile1 = 0;
   if (a.splits > 1) {
-    const int per = (tile1 - tile0 + a.splits - 1) / a.splits;
+    // pieces of a length that the plan sets, but `least` of a sequence, and no more than there are splits
+    const int n = tile1 - tile0, per = max((n + a.splits - 1) / a.splits, min((n + a.least - 1) / a.least, a.per));
     tile0 = min(tile1, tile0 + split * per);
     tile1 = min(tile1, tile0 + per);
+    if (tile0 == tile1) {  // nothing for this one
+      if (wave == 0 && lane < 16) cols.store_none(a, s, h, col0, split, lane);
+      return;
+    }
   }
+  typename Cols::Raw query;
+  cols.fetch(a, s, h, col0, lane, query);
   int full0 = max(tile0, (s1.lo + 31) >> 5), full1 = min(tile1, s0.hi >> 5);
   if (full0 >= full1) full0 = full1 = tile1;
 

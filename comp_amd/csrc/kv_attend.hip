@@ -20,10 +20,13 @@ AttendPlan plan_of(const KvAttendCall& c) {
   const int wide = p.many ? many_cols(c.cache.dim, c.type) : 16;
   p.groups = static_cast<int>((cols + wide - 1) / wide);
   // Enough workgroups to fill the CUs once (one of many columns each, three of few: 16 sequences of up to 8192 keys and 1-5
-  // rows, f32: 59 us with 512 workgroups, 50 with 768 and 1024), or where there are many sequences more, so that unlike
-  // lengths even out (64 sequences of up to 8192 keys, bf16: 106 us with 1024, 97 with 2048, 103 with 4096); and no split
-  // of less than two tiles a wave or two buffers.
-  const int64_t aim = p.many ? 256 : units * p.groups >= 256 ? 2048 : 768;
+  // rows, f32: 59 us with 512 workgroups, 51 with 768, 50 with 1024), or where there are many sequences more, so that unlike
+  // lengths even out (64 sequences of up to 8192 keys, bf16: 106 us with 1024, 92 with 2048, 94 with 4096); and no split
+  // of less than two tiles a wave or two buffers.  Pieces of few columns have the longest length's share of the splits,
+  // so that shorter sequences are cut into fewer, but enough (`least`) to fill the CUs once if all are that short.
+  const int64_t fill = p.many ? 256 : 768, aim = !p.many && units * p.groups >= 256 ? 2048 : fill;
+  p.least = static_cast<int>((fill + units * p.groups - 1) / (units * p.groups));
+  p.per = 1;
   const int64_t want = (aim + units * p.groups - 1) / (units * p.groups);
   const int64_t most = p.many ? c.max_length / 256 : (c.max_length + 31) / 32 / (2 * kAttendWaves);
   if (c.rows * c.heads > 1 << 22) {  // rows that no sequence holds, most likely: the join has a workgroup for each row and head
@@ -31,6 +34,8 @@ AttendPlan plan_of(const KvAttendCall& c) {
     return p;
   }
   p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits})));
+  p.least = std::min(p.least, p.splits);
+  p.per = static_cast<int>(((c.max_length + 31) / 32 + p.splits - 1) / p.splits);
   return p;
 }
 
@@ -125,6 +130,8 @@ hipError_t launch_kv_attend(const KvAttendCall& c, hipStream_t stream) {
   a.wide_q = fits(c.q, c.q_stride_t, c.q_stride_h, 16);
   a.wide_out = fits(c.out, c.out_stride_t, c.out_stride_h, 4 * size);
   a.splits = p.splits;
+  a.least = p.least;
+  a.per = p.per;
   a.groups = p.groups;
   a.part_o = static_cast<float*>(c.work);
   const int64_t n = p.splits * c.rows * c.heads;
