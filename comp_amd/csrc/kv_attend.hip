@@ -19,12 +19,13 @@ AttendPlan plan_of(const KvAttendCall& c) {
   p.many = cols > 96;
   const int wide = p.many ? many_cols(c.cache.dim, c.type) : 16;
   p.groups = static_cast<int>((cols + wide - 1) / wide);
-  // Enough workgroups to fill the CUs once (one of many columns each, three of few: 16 sequences of up to 8192 keys and 1-5
-  // rows, f32: 59 us with 512 workgroups, 51 with 768, 50 with 1024), or where there are many sequences more, so that unlike
-  // lengths even out (64 sequences of up to 8192 keys, bf16: 106 us with 1024, 92 with 2048, 94 with 4096); and no split
-  // of less than two tiles a wave or two buffers.  Pieces of few columns have the longest length's share of the splits,
-  // so that shorter sequences are cut into fewer, but enough (`least`) to fill the CUs once if all are that short.
-  const int64_t fill = p.many ? 256 : 768, aim = !p.many && units * p.groups >= 256 ? 2048 : fill;
+  // Workgroups to fill the CUs (one of many columns each; of few three fit, and a fourth evens out what masks and short
+  // sequences leave empty: 16 sequences of up to 8192 keys and 1-5 rows, f32, 60 us with 512 workgroups, 64 with 768, 41
+  // with 1024, 44 with 1536), twice that where there are many sequences of unlike lengths (64 of up to 8192 keys, bf16: 106
+  // us with 1024, 92 with 2048, 94 with 4096); and no split of less than two tiles a wave or two buffers.  Pieces of few
+  // columns have the longest length's share of the splits, so that shorter sequences are cut into fewer, but enough
+  // (`least`) to fill the CUs if all are that short.
+  const int64_t fill = p.many ? 256 : 1024, aim = !p.many && units * p.groups >= 256 ? 2 * fill : fill;
   p.least = static_cast<int>((fill + units * p.groups - 1) / (units * p.groups));
   p.per = 1;
   const int64_t want = (aim + units * p.groups - 1) / (units * p.groups);
