@@ -9,11 +9,16 @@
 // Both products run transposed, S^T = K Q^T and O^T = V^T P^T, with the cache's codes as operand A in f16:
 //   * a nibble (or byte) n, masked out of its dword, IS an f16: the subnormal n * 2^-24.  Key codes are used that way: the
 //     product is exact, 2^-24 goes into the score's factor and the offset (code = n - 8) into the product's initial
-//     accumulator, -8 * 2^-24 * sum(q) over the block (one column).  Several columns share the unpacking and take
-//     signed codes ((n | 0x6400) - 1032, exact) instead, which needs no accumulators kept for it, and so do f32 queries:
+//     accumulator, -8 * 2^-24 * sum(q) over the block.  Where registers are short, or many columns share the unpacking,
+//     keys are signed codes ((n | 0x6400) - 1032, exact) instead, which needs no accumulators kept for it, and so do f32 queries:
 //     the matrix unit sums products of subnormals with some 20 bits.
 //   * a block's key scale multiplies its 32-channel partial dot in f32, so keys are not rounded at all;
 //   * value codes are exact signed f16, and the value scale of (token, block) goes onto the probability: P' = P * d.
+// What bounds it: few columns, by bytes (18 or 34 a block of keys and of values, once a kv head) and by the some 270
+// vector instructions a 32-key tile of 128 4-bit channels takes (400 with f32 queries), which a CU's memory rate leaves
+// room for about twice; many columns, by the softmax's instructions beside the products (kv_many.h).  Measured, 32 query
+// heads over 8 of 128 channels, 4-bit, bf16: 64 sequences of up to 8192 keys 88 us (4.1 TB/s), one of 131072 38 us (4.0
+// TB/s), where a read of as many bytes takes 53 and 22 us.
 // What is rounded: queries to f16 after a power of two that puts a column's largest at 2^13 (f16 and bf16 queries are
 // exact, except values 2^-27 of the largest), P and P' to f16 (2^-12 each, to nearest).  f32 queries (PREC) are held in
 // two f16 parts and P' in two, 22 bits each, two matrix instructions for one.  Scores, sums and accumulators are f32.
@@ -100,10 +105,6 @@ __device__ __forceinline__ float quarters_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-template <int N>
-struct Words {
-  unsigned w[N];
-};
 // N dwords of a 16-, 12-, 8- or 4-byte aligned address, in loads of W
 template <int N, int W>
 __device__ __forceinline__ void load_words(const uint8_t* p, unsigned* out) {
@@ -181,16 +182,6 @@ __device__ __forceinline__ f16x8 value_codes(unsigned w0, unsigned w1, int half)
     return as_f16x8(signed_low(w0 & 0x00FF00FFu, 128.f), signed_low(w0 >> 8 & 0x00FF00FFu, 128.f),
                     signed_low(w1 & 0x00FF00FFu, 128.f), signed_low(w1 >> 8 & 0x00FF00FFu, 128.f));
   }
-}
-
-// f(integral_constant<int, 0>{}) .. f(integral_constant<int, N - 1>{})
-template <typename F, int... I>
-__device__ __forceinline__ void each_impl(F&& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void each(F&& f) {
-  each_impl(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
 }
 
 // lane I of each 16 lanes, in all of them

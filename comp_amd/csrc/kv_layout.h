@@ -21,7 +21,20 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+#include <utility>
+
 namespace komp {
+
+// f(integral_constant<int, 0>{}) .. f(integral_constant<int, N - 1>{})
+template <typename F, int... I>
+__device__ __forceinline__ void each_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  each_impl(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
+}
 
 enum KvFmt { KV_Q4_0 = 0, KV_Q8_0 = 2 };  // Fmt's values
 enum KvType { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };

@@ -12,6 +12,9 @@
 // what bf16 keeps of the result, and saves the f32 products of the partial dots and of the probabilities, half of a
 // column's instructions.  (Where the logarithms of the sums are asked for, in f32, keys stay exact: KEYS_SCALED.)  A value
 // block whose scale is no number is held as zeros then, and makes NaN of its channels in the columns that see it.
+// Measured, 32 query heads over 8 of 128 channels, 4-bit, bf16: a prompt of 4096 tokens 275 us, 570 TFLOP/s where every key
+// is seen (f16 450, f32 210, twice the products), where a large library product reaches 1160: the vector unit is busy 46%
+// of the time, the matrix unit 20%.
 #pragma once
 
 #include "kv_attend.h"

