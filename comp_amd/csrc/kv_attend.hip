@@ -18,7 +18,7 @@ AttendPlan plan_of(const KvAttendCall& c) {
   // 80, 91 and 86; 48 columns 37 and 65.
   p.many = cols > 96;
   const int wide = p.many ? many_cols(c.cache.dim, c.type) : 16;
-  p.groups = static_cast<int>((cols + wide - 1) / wide);
+  p.groups = std::max(1, static_cast<int>((cols + wide - 1) / wide));  // (none without query rows: such a call launches nothing)
   // Workgroups to fill the CUs (one of many columns each; of few three fit, and a fourth evens out what masks and short
   // sequences leave empty: 16 sequences of up to 8192 keys and 1-5 rows, f32, 60 us with 512 workgroups, 64 with 768, 41
   // with 1024, 44 with 1536), twice that where there are many sequences of unlike lengths (64 of up to 8192 keys, bf16: 106
@@ -92,7 +92,7 @@ int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 }  // namespace
 
 int64_t kv_attend_work_bytes(const KvAttendCall& c) {
-  if (c.batch == 0 || c.rows == 0) return 0;
+  if (c.batch == 0 || c.rows == 0 || c.max_queries == 0) return 0;
   const AttendPlan p = plan_of(c);
   if (p.splits == 1) return 0;
   const int64_t n = p.splits * c.rows * c.heads;

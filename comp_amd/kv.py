@@ -285,8 +285,9 @@ def attend(cache, q, tables, lengths, starts=None, *, max_queries=None, max_leng
     j <= i or j < prefix[s] (int32 [B]), of the past only the nearest `window` ones (itself among them) with window > 0.
     A row that sees nothing gives zeros and an lse of -inf.
 
-    max_queries: the most rows of one sequence (T by default); rows past it are not computed.  max_length: an upper bound of
-    the lengths that the launch is planned for (the tables' width by default); any value gives the right result."""
+    max_queries: the most rows of one sequence (T by default); the results' places of rows past it hold anything (with 0 nothing
+    is computed at all).  max_length: an upper bound of the lengths that the launch is planned for (the tables' width by
+    default); any value gives the right result."""
     if not _attend_fits(cache, q, tables, lengths, starts, max_queries, prefix, slopes):
         _check_attend(cache, q, None, tables, lengths, starts, max_queries, prefix, slopes, None)
     out = cache.kq.new_empty(q.shape, dtype=q.dtype)

@@ -279,8 +279,8 @@ int komp_kv_read(const komp_kv_cache* C, const int64_t* SLOTS, int64_t T, void* 
  *   OUT [T][heads][head_dim] = softmax over the visible keys times their values, 0 where none is visible
  *   LSE f32 [T][heads] (or NULL) = the natural logarithm of the sum of exp(score), -inf where none is visible
  * A page number that the cache does not have hides its keys; lengths past table_cols pages end there.  max_queries: at
- * least the most rows a sequence has (at most T, and
- * 2^23 with the query heads of a kv head counted); max_length: the longest length, for the plan alone (any value is right).
+ * least the most rows a sequence has (at most T, and 2^23 with the query heads of a kv head counted; 0: nothing is computed
+ * and OUT and LSE stay as they are); max_length: the longest length, for the plan alone (any value is right).
  * WORK: komp_kv_attend_workspace bytes for the same arguments (0: may be NULL), 16-byte aligned, free again when the call
  * has run.  Rows of Q that no sequence holds get unspecified results. */
 int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE, int type, const int32_t* TABLES,
