@@ -64,6 +64,7 @@ struct AttendArgs {
   int window;
   float scale;   // times log2(e)
   float cap;     // softcap, or 0
+  float twice;   // 2 / softcap
   bool wide_q;   // query rows may be loaded 16 bytes at a time
   bool wide_out; // output rows stored four elements at a time
   int splits;
@@ -316,7 +317,7 @@ struct Columns {
   f16x8 qf[CT][NB][PARTS];
   f32x4 init[SIGNED ? 1 : NB];
   float fx[CT];       // of y, the raw or capped and biased score, to log2 units
-  float raw[CT];      // of the raw score, when it is capped or biased
+  float raw[CT];      // of the raw score to log2 units, when it is capped or biased
   float slope[CT];
   f32x4 acc[CT][OT];
   float neg[CT];      // -M, or 0 before anything was seen
@@ -419,7 +420,7 @@ struct Columns {
         }
       }
       const float unit = __builtin_ldexpf(fabsf(a.scale), (SIGNED ? 0 : 24) - up);
-      raw[ct] = a.cap > 0.f ? 2.f * unit / a.cap : unit;
+      raw[ct] = unit;
       fx[ct] = a.cap > 0.f || a.slopes ? 1.f : fmaxf(unit, 0x1p-126f);
       neg[ct] = 0.f;
       lim[ct] = NONE;
@@ -429,17 +430,38 @@ struct Columns {
     }
   }
 
-  // capped and biased scores from raw ones
+  // Capped and biased scores from raw ones.  With s the score in log2 units and v = 2 s / cap, tanh(score / cap) = tanh(v ln2 /
+  // 2) is 1 - 2 / (2^v + 1), whose two terms cancel where |v| is small; there the capped score is s (1 + z P(z)), z = v^2, P
+  // fitted to tanh(u) / u on |u| <= 1/2 (relative error 2^-25.9, coefficients times (ln2 / 2)^2k).  A wave whose scores are
+  // all that small, as with most caps in use, computes nothing else.
   __device__ __forceinline__ void shape(const AttendArgs& a, int ct, int key0, float unit, float (&y)[2][4]) const {
-    const float cap = a.cap * kLog2e;
+    constexpr float BEND = kLog2e;  // |v| of |u| = 1/2
     const float back = static_cast<float>(pos[ct] - key0), to = raw[ct] * unit;
+    bool bent = false;
+    if (a.cap > 0.f) {
+      float most = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(y[t][r]));
+      bent = __builtin_amdgcn_ballot_w64(most * to * a.twice > BEND) != 0;
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float x = y[t][r] * to;
-        // cap tanh(s / cap), tanh u = 1 - 2 / (e^2u + 1)
-        if (a.cap > 0.f) x = cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.f);
+        if (a.cap > 0.f) {
+          const float v = x * a.twice, z = v * v;
+          const float p = fmaf(fmaf(fmaf(0x1.e1ab3p-19f, z, -0x1.818ceap-14f), z, 0x1.f7fc2cp-10f), z, -0x1.47fcc6p-5f);
+          const float low = fmaf(x * z, p, x);
+          if (bent) {
+            const float one = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v) + 1.f), 1.f);
+            x = fabsf(v) > BEND ? a.cap * one * kLog2e : low;
+          } else {
+            x = low;
+          }
+        }
         y[t][r] = fmaf(-slope[ct], fabsf(back - (16 * t + r)), x);
       }
   }

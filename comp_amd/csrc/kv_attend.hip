@@ -124,6 +124,7 @@ hipError_t launch_kv_attend(const KvAttendCall& c, hipStream_t stream) {
   a.window = c.window;
   a.scale = c.scale * kLog2e;
   a.cap = c.softcap;
+  a.twice = c.softcap > 0.f ? std::min(2.f / c.softcap, 3.0e38f) : 0.f;  // (a number for the smallest caps too)
   const int size = c.type == KV_F32 ? 4 : 2;
   auto fits = [&](const void* p, int64_t st, int64_t sh, int bytes) {
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && st * size % bytes == 0 && sh * size % bytes == 0;
