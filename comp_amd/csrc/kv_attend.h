@@ -310,6 +310,10 @@ struct Columns {
   static constexpr int PARTS = PREC ? 2 : 1;
   static constexpr int OT = 2 * NB;  // 16-channel tiles of the output
   static constexpr float NONE = -__builtin_inff();
+  static constexpr float UNSEEN = 0x1p127f;  // neg before anything was seen: any score is above its reference, and masked ones give 0
+  // M moves to a column's largest score less this, and moves again when a score is 8 above that: P is 2^(ROOM + 8) at most,
+  // and P' = P d below 2^15 for value scales of exponent fields up to 21 - ROOM.  Keys with larger ones leave less room.
+  static constexpr int ROOM = PREC ? 20 : 6;
 
   Span all;           // keys that some column sees
   Span span[CT];      // of the lane's columns
@@ -320,10 +324,9 @@ struct Columns {
   float raw[CT];      // of the raw score to log2 units, when it is capped or biased
   float slope[CT];
   f32x4 acc[CT][OT];
-  float neg[CT];      // -M, or 0 before anything was seen
-  float lim[CT];      // y above which M moves
+  float neg[CT];      // -M, or UNSEEN
   float l[CT];
-  int off;
+  int room;           // of the tiles so far (Columns::step)
 
   // the lane's column ct: its query row and head; false where there is none
   __device__ __forceinline__ bool place(const AttendArgs& a, const Sequence& s, int h, int col0, int ct, int lane,
@@ -336,7 +339,7 @@ struct Columns {
   }
 
   // M of column ct (-inf before anything was seen)
-  __device__ __forceinline__ float reference(int ct) const { return lim[ct] == NONE ? NONE : -neg[ct]; }
+  __device__ __forceinline__ float reference(int ct) const { return neg[ct] == UNSEEN ? NONE : -neg[ct]; }
 
   // a lane's query channels, as they are in memory: the loads are under way before the keys', which take longer
   struct Raw {
@@ -372,7 +375,7 @@ struct Columns {
   }
 
   __device__ __forceinline__ void begin(const AttendArgs& a, const Sequence& s, int h, int col0, int lane, const Raw& q) {
-    off = PREC ? 20 : 6;
+    room = ROOM;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       int64_t row;
@@ -422,8 +425,7 @@ struct Columns {
       const float unit = __builtin_ldexpf(fabsf(a.scale), (SIGNED ? 0 : 24) - up);
       raw[ct] = unit;
       fx[ct] = a.cap > 0.f || a.slopes ? 1.f : fmaxf(unit, 0x1p-126f);
-      neg[ct] = 0.f;
-      lim[ct] = NONE;
+      neg[ct] = UNSEEN;
       l[ct] = 0.f;
 #pragma unroll
       for (int i = 0; i < OT; ++i) acc[ct][i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -466,8 +468,32 @@ struct Columns {
       }
   }
 
-  // M moves to the largest score so far, and what was summed with it
-  __device__ __forceinline__ void move(int off_now, float unit, const float (&y)[CT][2][4]) {
+  // The columns' room over 32 keys of which some are masked, whose value scales lie as in KvTile::vs: of each column, by the
+  // finite scales that it sees, so that a large one that it does not see takes no bits from it.
+  __device__ __forceinline__ void settle(const unsigned (&vs)[(4 * NB + 15) / 16], int key0, int (&own)[CT]) const {
+    unsigned keep[CT][4];
+    int top[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      seen_pairs(ct, key0, keep[ct]);
+      top[ct] = 21 - ROOM;
+    }
+    each<4 * NB>([&](auto nc) {
+      constexpr int at = nc.value;
+      const unsigned d = row_lane<at % 16>(vs[at / 16]);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const unsigned w = d & keep[ct][at & 3];
+        const int lo = w >> 10 & 31, hi = w >> 26 & 31;
+        top[ct] = max(top[ct], max(lo == 31 ? 0 : lo, hi == 31 ? 0 : hi));
+      }
+    });
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) own[ct] = 21 - static_cast<int>(quarters_max(static_cast<float>(top[ct])));
+  }
+
+  // Where a column's largest score has left its room, M moves there, and what was summed with it.
+  __device__ __forceinline__ void move(const int (&own)[CT], float unit, const float (&y)[CT][2][4]) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float top = y[ct][0][0];
@@ -476,24 +502,23 @@ struct Columns {
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, y[ct][t][r]);
       top = quarters_max(top * (fx[ct] * unit));
-      const float before = reference(ct);
-      top = fmaxf(top, before + off);
-      const float now = top - off_now;
+      const float to = top + neg[ct] > own[ct] + 8 ? own[ct] - top : neg[ct];
       // (nothing seen yet: nothing to rescale)
-      const float by = before == NONE ? 0.f : __builtin_amdgcn_exp2f(before - now);
+      const float by = neg[ct] == UNSEEN ? 0.f : __builtin_amdgcn_exp2f(to - neg[ct]);
       l[ct] *= by;
 #pragma unroll
       for (int i = 0; i < OT; ++i) acc[ct][i] *= by;
-      neg[ct] = now == NONE ? 0.f : -now;
-      lim[ct] = now == NONE ? NONE : (top + 8.f) / fx[ct];
+      neg[ct] = to;
     }
-    off = off_now;
   }
 
-  // Raw scores (in the tile's unit) to probabilities 2^(x - M + ev), and the sums of 2^(x - M).
-  __device__ __forceinline__ void soften(const AttendArgs& a, bool masked, int key0, int off_now, float unit, int ev, float (&y)[CT][2][4]) {
+  // Raw scores (in the tile's unit) to probabilities 2^(x - M + ev), and the sums of 2^(x - M).  `left`: the room that the
+  // tile's value scales leave, seen or not.  `scales`: them, or nothing where they are in the operands.
+  template <typename S>
+  __device__ __forceinline__ void soften(const AttendArgs& a, bool masked, int key0, int left, float unit, int ev, float (&y)[CT][2][4],
+                                         S&& scales) {
     const bool shaped = a.cap > 0.f || a.slopes != nullptr;
-    bool go = off_now < off;
+    bool go = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       if (shaped) shape(a, ct, key0, unit, y[ct]);
@@ -512,9 +537,17 @@ struct Columns {
     for (int ct = 0; ct < CT; ++ct) {
       const float top = fmaxf(fmaxf(fmaxf(y[ct][0][0], y[ct][0][1]), fmaxf(y[ct][0][2], y[ct][0][3])),
                               fmaxf(fmaxf(y[ct][1][0], y[ct][1][1]), fmaxf(y[ct][1][2], y[ct][1][3])));
-      go |= top * unit > lim[ct];
+      go |= fmaf(top, fx[ct] * unit, neg[ct]) > left + 8;
     }
-    if (__builtin_amdgcn_ballot_w64(go) != 0) move(off_now, unit, y);
+    if (__builtin_amdgcn_ballot_w64(go) != 0) {
+      int own[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) own[ct] = left;
+      if constexpr (!std::is_same_v<std::decay_t<S>, std::nullptr_t>) {
+        if (masked) settle(scales(), key0, own);
+      }
+      move(own, unit, y);
+    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const float f = fx[ct] * unit, n = neg[ct] + ev;
@@ -585,7 +618,7 @@ struct Columns {
         }
       });
     });
-    // larger value scales may need a lower `off`; the scales of keys that no column sees are not looked at
+    // larger value scales may leave less room; the scales of keys that no column sees are not looked at
     unsigned vs[KvTile<NB, KF, VF>::SW];
     bool above = false;
 #pragma unroll
@@ -595,10 +628,9 @@ struct Columns {
         const int pair = min(i * 16 + (lane & 15), 4 * NB - 1) & 3, j = key0 + 16 * (pair >> 1) + (pair & 1);
         vs[i] &= (j >= all.lo && j < all.hi ? 0xFFFFu : 0u) | (j + 2 >= all.lo && j + 2 < all.hi ? 0xFFFF0000u : 0u);
       }
-      const unsigned lo = vs[i] & 0x7C00u, hi = vs[i] >> 16 & 0x7C00u, most = static_cast<unsigned>(21 - off) << 10;
+      const unsigned lo = vs[i] & 0x7C00u, hi = vs[i] >> 16 & 0x7C00u, most = static_cast<unsigned>(21 - room) << 10;
       above |= (lo > most && lo != 0x7C00u) || (hi > most && hi != 0x7C00u);
     }
-    int off_now = off;
     if (__builtin_amdgcn_ballot_w64(above) != 0) {
       unsigned e = 0;  // the largest finite scale's exponent field
 #pragma unroll
@@ -608,9 +640,9 @@ struct Columns {
       }
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) e = max(e, static_cast<unsigned>(__shfl_xor(static_cast<int>(e), o, 64)));
-      off_now = __builtin_amdgcn_readfirstlane(min(off, 21 - static_cast<int>(max(e, 1u))));
+      room = __builtin_amdgcn_readfirstlane(min(room, 21 - static_cast<int>(max(e, 1u))));
     }
-    soften(a, masked, key0, off_now, 1.f, 0, y);
+    soften(a, masked, key0, room, 1.f, 0, y, [&]() -> auto& { return vs; });
     unsigned ph[CT][4], keep[CT][4];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -804,8 +836,7 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
       }
       __syncthreads();
     }
-    cols.neg[ct] = -M;
-    cols.lim[ct] = M == Cols::NONE ? Cols::NONE : 0.f;
+    cols.neg[ct] = M == Cols::NONE ? Cols::UNSEEN : -M;
   }
   if (wave == 0) cols.store(a, s, h, col0, split, lane);
 }

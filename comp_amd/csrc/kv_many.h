@@ -35,6 +35,8 @@ struct Many {
   static constexpr int KCHUNKS = KEYS / 16 * KG, VCHUNKS = HALVES * VG, CHUNKS = KCHUNKS + VCHUNKS;
   static constexpr int TURNS = (CHUNKS + WAVES - 1) / WAVES;  // chunks of one wave
   static constexpr int SW = (16 * NB + 63) / 64;              // dwords a lane of a half's scales, in a wave
+  // the largest exponent fields of a tile: of the values' and the keys' scales (SCALED), or of each half's values' scales
+  static constexpr int MOST = SCALED ? 2 : HALVES;
   using Cols = Columns<NB, KF, VF, MODE, CT, true>;
 
   struct Shared {
@@ -42,7 +44,7 @@ struct Many {
     f16x8 v[2][HALVES * NB * 2][64];  // [32 tokens][block][channels 0..15, 16..31]
     unsigned ks[2][KEYS_SCALED ? 1 : HALVES][KEYS_SCALED ? 1 : 16 * NB];
     unsigned vs[2][SCALED ? 1 : HALVES][SCALED ? 1 : 16 * NB];
-    unsigned most[4][2];                       // the largest exponent field of the values' and the keys' scales
+    unsigned most[4][MOST];
     unsigned bad[4][SCALED ? 1 + HALVES * NB : 1];  // whether there are, and which, tokens of a half and block whose value
                                                     // scale is no number
   };
@@ -165,7 +167,11 @@ struct Many {
     int top = static_cast<int>(e);
     if constexpr (!SCALED) top = row16_max_i(top);  // (value operands: a row's lanes have the same scales)
     top = static_cast<int>(quarters_max(static_cast<float>(top)));
-    if (top && lane == 0) atomicMax(&sh.most[slot][0], static_cast<unsigned>(top));
+    if constexpr (SCALED) {
+      if (top && lane == 0) atomicMax(&sh.most[slot][0], static_cast<unsigned>(top));
+    } else {
+      if (wave < HALVES && lane == 0) sh.most[slot][wave] = static_cast<unsigned>(top);
+    }
     if constexpr (KEYS_SCALED) {
       const int k = row16_max_i(static_cast<int>(ek >> 10));  // (the quarters have the same keys)
       if (k && lane == 0) atomicMax(&sh.most[slot][1], static_cast<unsigned>(k));
@@ -234,7 +240,7 @@ struct Many {
                                               int half, int first, int lane) {
     constexpr int ROWS = (4 * NB + 15) / 16;  // a quarter's scales: dwords a lane of its 16
     const int quarter = lane >> 4, key0 = first + quarter * 4;
-    const int e = __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][0], 1u)));
+    const int e = __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][SCALED ? 0 : half], 1u)));
     unsigned ks[ROWS] = {};
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
@@ -276,7 +282,18 @@ struct Many {
     float unit = 1.f;
     if constexpr (KEYS_SCALED)
       unit = __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][1], 1u))) - 15);
-    cols.soften(a, masked, key0, min(cols.off, 21 - e), unit, SCALED ? e - 15 : 0, y);
+    const int left = min(Cols::ROOM, 21 - e);
+    if constexpr (SCALED) {
+      // (the power of two is the whole tile's, and so is what P may reach)
+      cols.soften(a, masked, key0, left, unit, e - 15, y, nullptr);
+    } else {
+      unsigned own[ROWS];
+      cols.soften(a, masked, key0, left, unit, 0, y, [&]() -> auto& {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) own[i] = sh.vs[buf][half][quarter * 4 * NB + min(i * 16 + (lane & 15), 4 * NB - 1)];
+        return own;
+      });
+    }
     if constexpr (SCALED) {
       unsigned w[CT][4];
 #pragma unroll
@@ -390,7 +407,7 @@ kv_attend_many_kernel(const AttendArgs a) {
   cols.begin(a, s, h, col0, lane, query);
   if (tile0 < tile1) {
     M m;
-    if (threadIdx.x < 8) sh.most[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    if (M::SCALED && threadIdx.x < 4 * M::MOST) (&sh.most[0][0])[threadIdx.x] = 0;
     constexpr int BAD = M::SCALED ? 1 + M::HALVES * NB : 0;
     if (threadIdx.x < 4 * BAD) (&sh.bad[0][0])[threadIdx.x] = 0;
     unsigned now = halves(tile0);
@@ -407,7 +424,7 @@ kv_attend_many_kernel(const AttendArgs a) {
       // most[] and bad[]: this tile's are in slot i, the next one's in i + 1, the one after's are filled in i + 2, and i + 3,
       // last read a turn ago, is cleared for the turn to come
       const int i = tile - tile0, buf = i & 1;
-      if (threadIdx.x < 2) sh.most[(i + 3) & 3][threadIdx.x] = 0;
+      if (M::SCALED && threadIdx.x < M::MOST) sh.most[(i + 3) & 3][threadIdx.x] = 0;
       if (threadIdx.x < BAD) sh.bad[(i + 3) & 3][threadIdx.x] = 0;
       m.unpack(sh, buf ^ 1, (i + 1) & 3, wave, lane);
       const unsigned after = halves(tile + 2);
