@@ -587,12 +587,47 @@ struct Columns {
     }
   }
 
+  // Queries of 8 blocks in shared memory (one column tile, the same for all waves): 32 registers, or 64 in two parts, that a
+  // wave beside its tile and sums does not have.
+  static constexpr bool SHARED_QUERIES = NB == 8 && CT == 1;
+  typedef f16x8 Queries[NB * PARTS][64];
+  __device__ __forceinline__ void share(Queries& to, int lane) const {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) to[b * PARTS + p][lane] = qf[0][b][p];
+  }
+
   // A tile of 32 keys from key `first` on.  masked: some column does not see some of them; a key that a column does not
   // see gets a P' of 0 there whatever its scale holds.
-  __device__ __forceinline__ void step(const AttendArgs& a, const KvTile<NB, KF, VF>& kv, bool masked, int first, int lane) {
+  __device__ __forceinline__ void step(const AttendArgs& a, const KvTile<NB, KF, VF>& kv, const Queries* shared, bool masked, int first,
+                                       int lane) {
     const int quarter = lane >> 4, key0 = first + quarter * 4;
     float y[CT][2][4];
-    each<2>([&](auto tc) {
+    if constexpr (SHARED_QUERIES) {
+      static_assert(SIGNED, "the accumulators begin at zero");
+      int at = lane;
+      asm volatile("" : "+v"(at));  // (read here, a tile at a time: held over the loop they would take their registers again)
+      each<NB / 2>([&](auto gc) {
+        constexpr int g = gc.value;
+        f32x4 c[2][2] = {};
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) {
+            const f16x8 q = (*shared)[(2 * g + b) * PARTS + p][at];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              c[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv.template key<SIGNED>(t, 2 * g + b), q, c[t][b], 0, 0, 0);
+          }
+        each<8>([&](auto rc) {
+          constexpr int t = rc.value / 4, r = rc.value % 4, i = t * 2 * NB + r * NB / 2 + g;  // (dword of row r, blocks 2 g and 2 g + 1)
+          const f16x2 d = as_f16x2(row_lane<i % 16>(kv.ks[i / 16]));
+          y[0][t][r] = g == 0 ? static_cast<float>(d[0]) * c[t][0][r] : fmaf(static_cast<float>(d[0]), c[t][0][r], y[0][t][r]);
+          y[0][t][r] = fmaf(static_cast<float>(d[1]), c[t][1][r], y[0][t][r]);
+        });
+      });
+    } else each<2>([&](auto tc) {
       constexpr int t = tc.value;
       f32x4 c[CT][NB];
 #pragma unroll
@@ -738,6 +773,8 @@ struct Pages {
 // Few columns over many keys: the waves of a workgroup have the same 16 columns and share its keys out among them, a tile
 // each in turn; they join their sums in shared memory.  Registers decide how it hides the memory's latency: 3 waves a SIMD
 // (4 of 64 channels, 2 of 256, or 1 with f32 queries) with one tile in flight each, or for 8-bit tiles, twice as large, 2 waves with two.
+// No kernel may spill registers (the compiler has stored a spilled one where only some lanes were on, and all lanes read it
+// again: wild addresses): 256 channels have their queries in shared memory.
 template <int NB, int KF, int VF, int MODE>
 struct Few {
   static constexpr int DEEP = KF == KV_Q8_0 && VF == KV_Q8_0 && NB <= 4 ? 2 : 1;
@@ -778,6 +815,16 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
   int full0 = max(tile0, (s1.lo + 31) >> 5), full1 = min(tile1, s0.hi >> 5);
   if (full0 >= full1) full0 = full1 = tile1;
 
+  __shared__ f32x4 so[W / 2][OT][64];  // the waves' sums on their way to each other; until then, the queries
+  __shared__ float2 sm[W / 2][16];
+  auto* const queries = reinterpret_cast<typename Cols::Queries*>(so);
+  cols.all = Span{s0.lo, s1.hi};
+  if constexpr (Cols::SHARED_QUERIES) {
+    static_assert(sizeof(typename Cols::Queries) <= sizeof(so), "the queries fit");
+    cols.begin(a, s, h, col0, lane, query);
+    if (wave == 0) cols.share(*queries, lane);
+    __syncthreads();
+  }
   const Pages pages(a, seq, h);
   KvTile<NB, KF, VF> kv[DEEP];
   int64_t unit[DEEP];
@@ -787,13 +834,12 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
     unit[i] = tile < full1 ? pages.unit(tile) : -1;
     if (unit[i] >= 0) kv[i].load(a.c, unit[i], lane);
   }
-  cols.all = Span{s0.lo, s1.hi};
-  cols.begin(a, s, h, col0, lane, query);
+  if constexpr (!Cols::SHARED_QUERIES) cols.begin(a, s, h, col0, lane, query);
   for (int tile = full0 + wave; tile < full1; tile += DEEP * W) {
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {
       const int now = tile + i * W, next = now + DEEP * W;
-      if (unit[i] >= 0) cols.step(a, kv[i], false, now * 32, lane);
+      if (unit[i] >= 0) cols.step(a, kv[i], queries, false, now * 32, lane);
       unit[i] = next < full1 ? pages.unit(next) : -1;
       if (unit[i] >= 0) kv[i].load(a.c, unit[i], lane);
     }
@@ -806,12 +852,11 @@ __global__ void __launch_bounds__(kAttendWaves * 64, (Few<NB, KF, VF, MODE>::WAV
     if (u < 0) continue;
     KvTile<NB, KF, VF> one;
     one.load(a.c, u, lane);
-    cols.step(a, one, true, tile * 32, lane);
+    cols.step(a, one, queries, true, tile * 32, lane);
   }
 
   // join the waves, a column tile at a time: the upper half hands its sums to the lower half, then wave 1 to wave 0
-  __shared__ f32x4 so[W / 2][OT][64];
-  __shared__ float2 sm[W / 2][16];
+  if constexpr (Cols::SHARED_QUERIES) __syncthreads();
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     float M = cols.reference(ct);

@@ -7,11 +7,11 @@
 // after that in flight.
 //
 // f16 and f32 queries: the operands hold the codes, exact; the scales lie beside them and are used as in Columns::step.
-// bf16 queries: the operands hold d * code, rounded to f16 after a power of two that brings the tile's largest scale to
-// [1, 2) and that the scores' factor or the probabilities' exponent takes back.  2^-12 of a key or value is an eighth of
+// bf16 queries (SCALED): the operands hold d * code, rounded to f16 after a power of two that brings the tile's largest scale
+// to [1, 2) and that the scores' factor or the probabilities' exponent takes back.  2^-12 of a key or value is an eighth of
 // what bf16 keeps of the result, and saves the f32 products of the partial dots and of the probabilities, half of a
-// column's instructions.  (Where the logarithms of the sums are asked for, in f32, keys stay exact: KEYS_SCALED.)  A value
-// block whose scale is no number is held as zeros then, and makes NaN of its channels in the columns that see it.
+// column's instructions.  (Where the logarithms of the sums are asked for, in f32, the operands stay exact.)  A value block
+// whose scale is no number is held as zeros then, and makes NaN of its channels in the columns that see it.
 // Measured, 32 query heads over 8 of 128 channels, 4-bit, bf16: a prompt of 4096 tokens 275 us, 570 TFLOP/s where every key
 // is seen (f16 450, f32 210, twice the products), where a large library product reaches 1160: the vector unit is busy 46%
 // of the time, the matrix unit 20%.
@@ -21,16 +21,17 @@
 
 namespace komp {
 
-template <int NB, int KF, int VF, int MODE, bool KEYS_SCALED>
+template <int NB, int KF, int VF, int MODE, bool SCALED>
 struct Many {
+  static constexpr bool IN_OPERANDS = SCALED;
   // two column tiles a wave halve the operand reads and the unpacking a column, where the registers (of two waves a SIMD)
   // hold their queries and sums: not f32 queries, in two parts, nor 256 channels
   static constexpr bool PAIR = NB <= 4 && MODE != KV_F32;
   static constexpr int CT = PAIR ? 2 : 1, WAVES = PAIR || NB == 8 ? 8 : 12, COLS = 16 * CT;
   static constexpr int HALVES = NB == 8 ? 2 : PAIR ? 4 : 3, KEYS = 32 * HALVES;  // (a "half" is 32 keys: two key tiles)
-  static constexpr bool SCALED = MODE == KV_BF16;  // value operands
   static constexpr int KB = kv_kb(NB, KF), VB = kv_vb(NB, VF);
   static constexpr int KD = KB * kv_code_bytes(KF) / 16, VD = VB * kv_code_bytes(VF) / 8;  // code dwords of a lane's chunk
+  static constexpr int MD = KD > VD ? KD : VD;
   static constexpr int KG = NB / KB, VG = NB / VB;                                         // chunks a 16- or 32-token tile
   static constexpr int KCHUNKS = KEYS / 16 * KG, VCHUNKS = HALVES * VG, CHUNKS = KCHUNKS + VCHUNKS;
   static constexpr int TURNS = (CHUNKS + WAVES - 1) / WAVES;  // chunks of one wave
@@ -42,7 +43,7 @@ struct Many {
   struct Shared {
     f16x8 k[2][HALVES * 2 * NB][64];  // [16 tokens][block]
     f16x8 v[2][HALVES * NB * 2][64];  // [32 tokens][block][channels 0..15, 16..31]
-    unsigned ks[2][KEYS_SCALED ? 1 : HALVES][KEYS_SCALED ? 1 : 16 * NB];
+    unsigned ks[2][SCALED ? 1 : HALVES][SCALED ? 1 : 16 * NB];
     unsigned vs[2][SCALED ? 1 : HALVES][SCALED ? 1 : 16 * NB];
     unsigned most[4][MOST];
     unsigned bad[4][SCALED ? 1 + HALVES * NB : 1];  // whether there are, and which, tokens of a half and block whose value
@@ -50,12 +51,12 @@ struct Many {
   };
   // a wave's chunks on their way from the cache to shared memory, and for the first waves the scales of a half
   struct Chunk {
-    unsigned code[KD > VD ? KD : VD];
+    unsigned code[MD];
     unsigned scale[SCALED ? 4 * VB : 1];
   };
   Chunk chunk[TURNS];
   bool there[TURNS];
-  unsigned ks[SW], vs[SCALED ? 1 : SW];
+  unsigned ks[SCALED ? 1 : SW], vs[SCALED ? 1 : SW];
 
   static __device__ __forceinline__ int half_of(int c) { return c < KCHUNKS ? c / KG >> 1 : (c - KCHUNKS) / VG; }
 
@@ -68,11 +69,15 @@ struct Many {
       const int64_t u = c < CHUNKS ? unit(half_of(c)) : -1;
       there[i] = u >= 0;
       if (!there[i]) continue;
+      if constexpr (KD != VD) {  // (a length that depends on the kind would put the codes into scratch memory)
+#pragma unroll
+        for (int j = KD < VD ? KD : VD; j < MD; ++j) chunk[i].code[j] = 0;
+      }
       if (c < KCHUNKS) {
         const int t16 = c / KG & 1, g = c % KG;
         load_words<KD, KD>(cache.kq + u * (NB * 32 * kv_code_bytes(KF)) + t16 * (NB * 16 * kv_code_bytes(KF)) + (g * 64 + lane) * (KD * 4),
                            chunk[i].code);
-        if constexpr (KEYS_SCALED) {
+        if constexpr (SCALED) {
           const uint16_t* sp = cache.ks + u * (32 * NB) + (t16 * 16 + (lane & 15)) * NB + g * KB;
           if constexpr (KB % 2 == 0) {
             load_words<KB / 2, KB / 2>(reinterpret_cast<const uint8_t*>(sp), chunk[i].scale);
@@ -90,13 +95,13 @@ struct Many {
         }
       }
     }
-    if (!(KEYS_SCALED && SCALED) && wave < HALVES) {
+    if constexpr (!SCALED) if (wave < HALVES) {
       const int64_t u = unit(wave);
 #pragma unroll
       for (int i = 0; i < SW; ++i) {
         const int at = min(i * 64 + lane, 16 * NB - 1);
-        if constexpr (!KEYS_SCALED) ks[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.ks)[u * (16 * NB) + at];
-        if constexpr (!SCALED) vs[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.vs)[u * (16 * NB) + at];
+        ks[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.ks)[u * (16 * NB) + at];
+        vs[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.vs)[u * (16 * NB) + at];
       }
     }
   }
@@ -118,14 +123,12 @@ struct Many {
         const int c = i * WAVES + wave;
         if (!there[i]) continue;
         if (c < KCHUNKS) {
-          if constexpr (KEYS_SCALED) {
-            const bool in = (c / KG & 1) * 16 + (lane & 15) < length - first - half_of(c) * 32;
+          const bool in = (c / KG & 1) * 16 + (lane & 15) < length - first - half_of(c) * 32;
 #pragma unroll
-            for (int b = 0; b < (KB % 2 == 0 ? KB / 2 : KB); ++b) {
-              chunk[i].scale[b] = in ? chunk[i].scale[b] : 0u;
-              const unsigned lo = chunk[i].scale[b] & 0x7C00u, hi = chunk[i].scale[b] >> 16 & 0x7C00u;
-              ek = max(ek, max(lo == 0x7C00u ? 0u : lo, hi == 0x7C00u ? 0u : hi));
-            }
+          for (int b = 0; b < (KB % 2 == 0 ? KB / 2 : KB); ++b) {
+            chunk[i].scale[b] = in ? chunk[i].scale[b] : 0u;
+            const unsigned lo = chunk[i].scale[b] & 0x7C00u, hi = chunk[i].scale[b] >> 16 & 0x7C00u;
+            ek = max(ek, max(lo == 0x7C00u ? 0u : lo, hi == 0x7C00u ? 0u : hi));
           }
           continue;
         }
@@ -167,12 +170,10 @@ struct Many {
     int top = static_cast<int>(e);
     if constexpr (!SCALED) top = row16_max_i(top);  // (value operands: a row's lanes have the same scales)
     top = static_cast<int>(quarters_max(static_cast<float>(top)));
-    if constexpr (SCALED) {
-      if (top && lane == 0) atomicMax(&sh.most[slot][0], static_cast<unsigned>(top));
-    } else {
+    if constexpr (!SCALED) {
       if (wave < HALVES && lane == 0) sh.most[slot][wave] = static_cast<unsigned>(top);
-    }
-    if constexpr (KEYS_SCALED) {
+    } else {
+      if (top && lane == 0) atomicMax(&sh.most[slot][0], static_cast<unsigned>(top));
       const int k = row16_max_i(static_cast<int>(ek >> 10));  // (the quarters have the same keys)
       if (k && lane == 0) atomicMax(&sh.most[slot][1], static_cast<unsigned>(k));
     }
@@ -185,8 +186,7 @@ struct Many {
       const _Float16 f = static_cast<_Float16>(__builtin_ldexpf(1.f, 15 - static_cast<int>(max(sh.most[slot][which], 1u))));
       return f16x2{f, f};
     };
-    if constexpr (SCALED) fv = power(0);
-    if constexpr (KEYS_SCALED) fk = power(1);
+    if constexpr (SCALED) fv = power(0), fk = power(1);
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
       const int c = i * WAVES + wave;
@@ -198,7 +198,7 @@ struct Many {
           f16x8 x;
           if constexpr (KF == KV_Q4_0) x = key_codes<true, KF>(chunk[i].code[b], 0u);
           else x = key_codes<true, KF>(chunk[i].code[2 * b], chunk[i].code[2 * b + 1]);
-          if constexpr (KEYS_SCALED) {
+          if constexpr (SCALED) {
             const _Float16 d = KB % 2 == 0 ? as_f16x2(chunk[i].scale[b >> 1])[b & 1] : as_f16x2(chunk[i].scale[b])[0];
             const f16x2 dd = f16x2{d, d} * fk;
             x *= f16x8{dd[0], dd[0], dd[0], dd[0], dd[0], dd[0], dd[0], dd[0]};
@@ -225,12 +225,12 @@ struct Many {
         }
       }
     }
-    if (!(KEYS_SCALED && SCALED) && wave < HALVES) {
+    if constexpr (!SCALED) if (wave < HALVES) {
 #pragma unroll
       for (int i = 0; i < SW; ++i) {
         const int at = min(i * 64 + lane, 16 * NB - 1);
-        if constexpr (!KEYS_SCALED) sh.ks[buf][wave][at] = ks[i];
-        if constexpr (!SCALED) sh.vs[buf][wave][at] = vs[i];
+        sh.ks[buf][wave][at] = ks[i];
+        sh.vs[buf][wave][at] = vs[i];
       }
     }
   }
@@ -245,7 +245,7 @@ struct Many {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const int at = min(i * 16 + (lane & 15), 4 * NB - 1), t = at / (2 * NB);
-      if constexpr (!KEYS_SCALED) ks[i] = sh.ks[buf][half][t * 8 * NB + quarter * 2 * NB + at - t * 2 * NB];
+      if constexpr (!SCALED) ks[i] = sh.ks[buf][half][t * 8 * NB + quarter * 2 * NB + at - t * 2 * NB];
     }
     float y[CT][2][4];
     each<2>([&](auto tc) {
@@ -256,13 +256,13 @@ struct Many {
         const f16x8 k = sh.k[buf][(half * 2 + t) * NB + b][lane];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          f32x4& x = c[ct][KEYS_SCALED ? 0 : b];
-          if (!KEYS_SCALED || b == 0) x = f32x4{0.f, 0.f, 0.f, 0.f};
+          f32x4& x = c[ct][SCALED ? 0 : b];
+          if (!SCALED || b == 0) x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int p = 0; p < Cols::PARTS; ++p) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, cols.qf[ct][b][p], x, 0, 0, 0);
         }
       }
-      if constexpr (KEYS_SCALED) {
+      if constexpr (SCALED) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -279,16 +279,14 @@ struct Many {
         }
       });
     });
-    float unit = 1.f;
-    if constexpr (KEYS_SCALED)
-      unit = __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][1], 1u))) - 15);
     const int left = min(Cols::ROOM, 21 - e);
     if constexpr (SCALED) {
+      const float unit = __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][1], 1u))) - 15);
       // (the power of two is the whole tile's, and so is what P may reach)
       cols.soften(a, masked, key0, left, unit, e - 15, y, nullptr);
     } else {
       unsigned own[ROWS];
-      cols.soften(a, masked, key0, left, unit, 0, y, [&]() -> auto& {
+      cols.soften(a, masked, key0, left, 1.f, 0, y, [&]() -> auto& {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) own[i] = sh.vs[buf][half][quarter * 4 * NB + min(i * 16 + (lane & 15), 4 * NB - 1)];
         return own;
@@ -362,10 +360,10 @@ struct Many {
   }
 };
 
-template <int NB, int KF, int VF, int MODE, bool KEYS_SCALED>
-__global__ void __launch_bounds__((64 * Many<NB, KF, VF, MODE, KEYS_SCALED>::WAVES), (Many<NB, KF, VF, MODE, KEYS_SCALED>::WAVES / 4))
+template <int NB, int KF, int VF, int MODE, bool SCALED>
+__global__ void __launch_bounds__((64 * Many<NB, KF, VF, MODE, SCALED>::WAVES), (Many<NB, KF, VF, MODE, SCALED>::WAVES / 4))
 kv_attend_many_kernel(const AttendArgs a) {
-  using M = Many<NB, KF, VF, MODE, KEYS_SCALED>;
+  using M = Many<NB, KF, VF, MODE, SCALED>;
   extern __shared__ __attribute__((aligned(16))) unsigned char shared_bytes[];
   typename M::Shared& sh = *reinterpret_cast<typename M::Shared*>(shared_bytes);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -407,8 +405,8 @@ kv_attend_many_kernel(const AttendArgs a) {
   cols.begin(a, s, h, col0, lane, query);
   if (tile0 < tile1) {
     M m;
-    if (M::SCALED && threadIdx.x < 4 * M::MOST) (&sh.most[0][0])[threadIdx.x] = 0;
-    constexpr int BAD = M::SCALED ? 1 + M::HALVES * NB : 0;
+    if (M::IN_OPERANDS && threadIdx.x < 4 * M::MOST) (&sh.most[0][0])[threadIdx.x] = 0;
+    constexpr int BAD = M::IN_OPERANDS ? 1 + M::HALVES * NB : 0;
     if (threadIdx.x < 4 * BAD) (&sh.bad[0][0])[threadIdx.x] = 0;
     unsigned now = halves(tile0);
     m.load(a.c, [&](int half) { return unit(tile0, half); }, wave, lane);
@@ -424,12 +422,12 @@ kv_attend_many_kernel(const AttendArgs a) {
       // most[] and bad[]: this tile's are in slot i, the next one's in i + 1, the one after's are filled in i + 2, and i + 3,
       // last read a turn ago, is cleared for the turn to come
       const int i = tile - tile0, buf = i & 1;
-      if (M::SCALED && threadIdx.x < M::MOST) sh.most[(i + 3) & 3][threadIdx.x] = 0;
+      if (M::IN_OPERANDS && threadIdx.x < M::MOST) sh.most[(i + 3) & 3][threadIdx.x] = 0;
       if (threadIdx.x < BAD) sh.bad[(i + 3) & 3][threadIdx.x] = 0;
       m.unpack(sh, buf ^ 1, (i + 1) & 3, wave, lane);
       const unsigned after = halves(tile + 2);
       m.load(a.c, [&](int half) { return unit(tile + 2, half); }, wave, lane);
-      const bool spoilt = M::SCALED && __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) != 0;
+      const bool spoilt = M::IN_OPERANDS && __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) != 0;
 #pragma unroll 1
       for (int half = 0; half < M::HALVES; ++half) {
         const int first = tile * M::KEYS + half * 32;
@@ -453,11 +451,11 @@ kv_attend_many_kernel(const AttendArgs a) {
   cols.store(a, s, h, col0, split, lane);
 }
 
-template <int NB, int KF, int VF, int MODE, bool KEYS_SCALED>
+template <int NB, int KF, int VF, int MODE, bool SCALED>
 hipError_t launch_attend_many(const AttendArgs& a, const dim3& grid, hipStream_t stream) {
-  using M = Many<NB, KF, VF, MODE, KEYS_SCALED>;
+  using M = Many<NB, KF, VF, MODE, SCALED>;
   static std::atomic<unsigned> limit[kMaxDevices];
-  const auto kern = kv_attend_many_kernel<NB, KF, VF, MODE, KEYS_SCALED>;
+  const auto kern = kv_attend_many_kernel<NB, KF, VF, MODE, SCALED>;
   constexpr size_t bytes = sizeof(typename M::Shared);
   const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), bytes, limit);
   if (e != hipSuccess) return e;
