@@ -11,7 +11,9 @@
 // to [1, 2) and that the scores' factor or the probabilities' exponent takes back.  2^-12 of a key or value is an eighth of
 // what bf16 keeps of the result, and saves the f32 products of the partial dots and of the probabilities, half of a
 // column's instructions.  (Where the logarithms of the sums are asked for, in f32, the operands stay exact.)  A value block
-// whose scale is no number is held as zeros then, and makes NaN of its channels in the columns that see it.
+// whose scale is no number is held as zeros then, and makes NaN of its channels in the columns that see it.  f16 holds a scale
+// times that power whole down to 2^-14 of the largest (or at all, where the largest is below 2); where a tile has a smaller one,
+// of keys that some column sees or not, the workgroup begins again with exact operands.
 // Measured, 32 query heads over 8 of 128 channels, 4-bit, bf16: a prompt of 4096 tokens 275 us, 570 TFLOP/s where every key
 // is seen (f16 450, f32 210, twice the products), where a large library product reaches 1160: the vector unit is busy 46%
 // of the time, the matrix unit 20%.
@@ -24,6 +26,7 @@ namespace komp {
 template <int NB, int KF, int VF, int MODE, bool SCALED>
 struct Many {
   static constexpr bool IN_OPERANDS = SCALED;
+  static constexpr int BLOCKS = NB;
   // two column tiles a wave halve the operand reads and the unpacking a column, where the registers (of two waves a SIMD)
   // hold their queries and sums: not f32 queries, in two parts, nor 256 channels
   static constexpr bool PAIR = NB <= 4 && MODE != KV_F32;
@@ -46,9 +49,11 @@ struct Many {
     unsigned ks[2][SCALED ? 1 : HALVES][SCALED ? 1 : 16 * NB];
     unsigned vs[2][SCALED ? 1 : HALVES][SCALED ? 1 : 16 * NB];
     unsigned most[4][MOST];
-    unsigned bad[4][SCALED ? 1 + HALVES * NB : 1];  // whether there are, and which, tokens of a half and block whose value
-                                                    // scale is no number
+    unsigned bad[4][SCALED ? 1 + HALVES * NB : 1];  // a tile's flags; which tokens of a half and block have a value scale
+                                                    // that is no number
   };
+  // flags: there are value scales that are no numbers; scales too far below the largest
+  static constexpr unsigned SPOILT = 1, SCATTERED = 2;
   // a wave's chunks on their way from the cache to shared memory, and for the first waves the scales of a half
   struct Chunk {
     unsigned code[MD];
@@ -150,7 +155,7 @@ struct Many {
             if ((hi & 0x7C00u) == 0x7C00u) none |= 4u << token, hi = 0;
             if (none && (lane & 15) == 0) {
               atomicOr(&sh.bad[slot][1 + half_of(c) * NB + (c - KCHUNKS) % VG * VB + (j >> 2)], none);
-              sh.bad[slot][0] = 1;
+              atomicOr(&sh.bad[slot][0], SPOILT);
             }
             chunk[i].scale[j] = lo | hi << 16;
             worst = max(worst, max(lo & 0x7C00u, hi & 0x7C00u));
@@ -186,7 +191,31 @@ struct Many {
       const _Float16 f = static_cast<_Float16>(__builtin_ldexpf(1.f, 15 - static_cast<int>(max(sh.most[slot][which], 1u))));
       return f16x2{f, f};
     };
-    if constexpr (SCALED) fv = power(0), fk = power(1);
+    if constexpr (SCALED) {
+      fv = power(0), fk = power(1);
+      // f16 scales (but 0) of exponent fields below this, 2 at least, lose bits to the power
+      auto least = [&](int which) { return __builtin_amdgcn_readfirstlane(static_cast<int>(sh.most[slot][which])) - 14; };
+      auto below = [](unsigned pair, int field) {
+        const unsigned lo = pair & 0x7FFFu, hi = pair >> 16 & 0x7FFFu, to = static_cast<unsigned>(field) << 10;
+        return (lo != 0 && lo < to) || (hi != 0 && hi < to);
+      };
+      const int kl = least(1), vl = least(0);
+      if (kl > 1 || vl > 1) {
+        bool scattered = false;
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+          if (!there[i]) continue;
+          if (i * WAVES + wave < KCHUNKS) {
+#pragma unroll
+            for (int b = 0; b < (KB % 2 == 0 ? KB / 2 : KB); ++b) scattered |= kl > 1 && below(chunk[i].scale[b], kl);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4 * VB; ++j) scattered |= vl > 1 && below(chunk[i].scale[j], vl);
+          }
+        }
+        if (scattered) atomicOr(&sh.bad[slot][0], SCATTERED);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
       const int c = i * WAVES + wave;
@@ -360,19 +389,18 @@ struct Many {
   }
 };
 
-template <int NB, int KF, int VF, int MODE, bool SCALED>
-__global__ void __launch_bounds__((64 * Many<NB, KF, VF, MODE, SCALED>::WAVES), (Many<NB, KF, VF, MODE, SCALED>::WAVES / 4))
-kv_attend_many_kernel(const AttendArgs a) {
-  using M = Many<NB, KF, VF, MODE, SCALED>;
-  extern __shared__ __attribute__((aligned(16))) unsigned char shared_bytes[];
-  typename M::Shared& sh = *reinterpret_cast<typename M::Shared*>(shared_bytes);
+// A workgroup's columns over its keys; false where a tile's scales are scattered, for all of its waves at the same point, and
+// nothing is stored then.
+template <typename M>
+__device__ __forceinline__ bool attend_many(const AttendArgs& a, typename M::Shared& sh) {
+  constexpr int NB = M::BLOCKS;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   __builtin_assume(wave >= 0 && wave < M::WAVES);
   const int h = blockIdx.x, seq = blockIdx.y, split = blockIdx.z / a.groups;
   // the groups of the latest positions, which see the most keys, begin first, those of all heads and sequences together
   const int group0 = (a.groups - 1 - (static_cast<int>(blockIdx.z) - split * a.groups)) * (M::WAVES * M::COLS);
   const Sequence s(a, seq);
-  if (group0 >= s.cols) return;
+  if (group0 >= s.cols) return true;
   const Span g0 = s.seen(a, group0 / a.group), g1 = s.seen(a, (min(s.cols, group0 + M::WAVES * M::COLS) - 1) / a.group);
   int tile0 = g0.lo / M::KEYS, tile1 = (g1.hi + M::KEYS - 1) / M::KEYS;
   if (tile0 > tile1) tile0 = tile1 = 0;
@@ -427,14 +455,15 @@ kv_attend_many_kernel(const AttendArgs a) {
       m.unpack(sh, buf ^ 1, (i + 1) & 3, wave, lane);
       const unsigned after = halves(tile + 2);
       m.load(a.c, [&](int half) { return unit(tile + 2, half); }, wave, lane);
-      const bool spoilt = M::IN_OPERANDS && __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) != 0;
+      const unsigned flags = M::IN_OPERANDS ? __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) : 0u;
+      if (flags & M::SCATTERED) return false;  // (set before the last barrier: every wave sees it here)
 #pragma unroll 1
       for (int half = 0; half < M::HALVES; ++half) {
         const int first = tile * M::KEYS + half * 32;
         if (!any || first >= w1.hi || first + 32 <= w0.lo || !(now >> half & 1)) continue;
         M::step(cols, a, sh, first < w1.lo || first + 32 > w0.hi, buf, i & 3, half, first, lane);
       }
-      if (spoilt) {
+      if (flags & M::SPOILT) {
 #pragma unroll 1
         for (int half = 0; half < M::HALVES; ++half)
           if (any && (now >> half & 1)) M::spoil(cols, sh, i & 3, half, tile * M::KEYS + half * 32);
@@ -445,25 +474,48 @@ kv_attend_many_kernel(const AttendArgs a) {
       __syncthreads();
     }
   }
-  if (!any) return;
+  if (!any) return true;
 #pragma unroll
   for (int ct = 0; ct < M::CT; ++ct) cols.l[ct] = quarters_sum(cols.l[ct]);
   cols.store(a, s, h, col0, split, lane);
+  return true;
+}
+
+template <int NB, int KF, int VF, int MODE, bool SCALED>
+struct ManyKernel {
+  using First = Many<NB, KF, VF, MODE, SCALED>;
+  using Exact = Many<NB, KF, VF, MODE, false>;
+  static constexpr int THREADS = 64 * First::WAVES;
+  static constexpr size_t SHARED = sizeof(typename First::Shared) > sizeof(typename Exact::Shared) ? sizeof(typename First::Shared)
+                                                                                                   : sizeof(typename Exact::Shared);
+  static_assert(First::WAVES == Exact::WAVES && First::COLS == Exact::COLS, "one launch serves both");
+};
+template <int NB, int KF, int VF, int MODE, bool SCALED>
+__global__ void __launch_bounds__((ManyKernel<NB, KF, VF, MODE, SCALED>::THREADS), (ManyKernel<NB, KF, VF, MODE, SCALED>::THREADS / 256))
+kv_attend_many_kernel(const AttendArgs a) {
+  using K = ManyKernel<NB, KF, VF, MODE, SCALED>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char shared_bytes[];
+  const bool done = attend_many<typename K::First>(a, *reinterpret_cast<typename K::First::Shared*>(shared_bytes));
+  if constexpr (SCALED) {
+    if (done) return;
+    __syncthreads();
+    attend_many<typename K::Exact>(a, *reinterpret_cast<typename K::Exact::Shared*>(shared_bytes));
+  }
 }
 
 template <int NB, int KF, int VF, int MODE, bool SCALED>
 hipError_t launch_attend_many(const AttendArgs& a, const dim3& grid, hipStream_t stream) {
-  using M = Many<NB, KF, VF, MODE, SCALED>;
+  using K = ManyKernel<NB, KF, VF, MODE, SCALED>;
   static std::atomic<unsigned> limit[kMaxDevices];
   const auto kern = kv_attend_many_kernel<NB, KF, VF, MODE, SCALED>;
-  constexpr size_t bytes = sizeof(typename M::Shared);
+  constexpr size_t bytes = K::SHARED;
   const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), bytes, limit);
   if (e != hipSuccess) return e;
   const Timing tm = timing_slot(KIND_PROBE);
   if (tm.on) {
-    hipExtLaunchKernelGGL(kern, grid, dim3(64 * M::WAVES), bytes, stream, tm.start, tm.stop, 0, a);
+    hipExtLaunchKernelGGL(kern, grid, dim3(K::THREADS), bytes, stream, tm.start, tm.stop, 0, a);
   } else {
-    hipLaunchKernelGGL(kern, grid, dim3(64 * M::WAVES), bytes, stream, a);
+    hipLaunchKernelGGL(kern, grid, dim3(K::THREADS), bytes, stream, a);
   }
   return hipGetLastError();
 }
