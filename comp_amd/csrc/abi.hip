@@ -1318,6 +1318,8 @@ int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE,
   if (STARTS == nullptr && T != batch)
     return fail(KOMP_EINVAL, "%s: T=%lld rows for batch=%lld without STARTS (one row a sequence)", name,
                 static_cast<long long>(T), static_cast<long long>(batch));
+  // (the kernels take scores in units of log2: scale * log2(e))
+  if (!(scale >= -2.0e38f && scale <= 2.0e38f)) return fail(KOMP_EINVAL, "%s: scale=%g (2e38 at most)", name, static_cast<double>(scale));
   if (!(softcap >= 0.f) || softcap > 3.0e38f) return fail(KOMP_EINVAL, "%s: softcap=%g", name, static_cast<double>(softcap));
   if (window < 0 || window > INT64_C(0x3FFFFFFF)) return fail(KOMP_EINVAL, "%s: window=%lld", name, static_cast<long long>(window));
   if (table_cols < 0 || table_cols > (INT64_C(0x7FFFFFFF) - 65536) / c.cache.page)

@@ -240,8 +240,8 @@ def _attend(cache, q, out, tables, lengths, starts, max_queries, max_length, sca
         max_queries = t
     if scale is None:
         scale = cache._scale
-    elif not math.isfinite(scale):
-        raise _BAD(f"scale={scale} must be finite")
+    elif not abs(scale) <= 2e38:
+        raise _BAD(f"scale={scale}: 2e38 at most in magnitude")
     most = cols * cache.page
     max_length = most if max_length is None else max(0, min(int(max_length), most))
     key = (TYPES[q.dtype], t, batch, heads, max_queries, max_length)

@@ -274,15 +274,17 @@ int komp_kv_read(const komp_kv_cache* C, const int64_t* SLOTS, int64_t T, void* 
  * (row stride table_stride), and the query rows STARTS[s] .. STARTS[s + 1] - 1 of Q [T][heads][head_dim] (STARTS NULL: row
  * s); its n rows are its last n positions, the new tokens' own keys being in the cache already.  `heads` is a multiple
  * of the cache's: each kv head serves heads / C->heads consecutive query heads.  For a row at position i
- *   score_j = scale * q . k_j;  softcap > 0: softcap * tanh(score / softcap);  SLOPES f32 [heads]: - slope * |i - j|
+ *   score_j = scale * q . k_j (|scale| 2e38 at most); softcap > 0: softcap * tanh(score / softcap); SLOPES f32 [heads]:
+ *   - slope * |i - j|
  *   visible: j < LENGTHS[s], j <= i or j < PREFIX[s] (NULL: 0), and with window > 0 also i - j < window
  *   OUT [T][heads][head_dim] = softmax over the visible keys times their values, 0 where none is visible
  *   LSE f32 [T][heads] (or NULL) = the natural logarithm of the sum of exp(score), -inf where none is visible
- * A page number that the cache does not have hides its keys; lengths past table_cols pages end there.  max_queries: at
- * least the most rows a sequence has (at most T, and 2^23 with the query heads of a kv head counted; 0: nothing is computed
- * and OUT and LSE stay as they are); max_length: the longest length, for the plan alone (any value is right).
- * WORK: komp_kv_attend_workspace bytes for the same arguments (0: may be NULL), 16-byte aligned, free again when the call
- * has run.  Rows of Q that no sequence holds get unspecified results. */
+ * A page number that the cache does not have hides its keys, and so does a table that ends before LENGTHS[s] (positions count
+ * from LENGTHS[s] all the same).  max_queries: at least the most rows a sequence has (at most T, and 2^23 with the query heads
+ * of a kv head counted; 0: nothing is computed, OUT and LSE stay as they are); max_length: the longest length, for the plan
+ * alone (any value is right).  WORK: komp_kv_attend_workspace bytes for the same arguments (0: may be NULL), 16-byte aligned,
+ * free again when the call has run.  Rows of Q that no sequence holds get unspecified results.  bf16 OUT is rounded from sums
+ * that differ in their last bits with and without LSE. */
 int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE, int type, const int32_t* TABLES,
                    const int32_t* LENGTHS, const int32_t* STARTS, const int32_t* PREFIX, const float* SLOPES, int64_t T,
                    int64_t batch, int64_t heads, int64_t q_stride_t, int64_t q_stride_h, int64_t out_stride_t,
