@@ -14,14 +14,17 @@
 //     the matrix unit sums products of subnormals with some 20 bits.
 //   * a block's key scale multiplies its 32-channel partial dot in f32, so keys are not rounded at all;
 //   * value codes are exact signed f16, and the value scale of (token, block) goes onto the probability: P' = P * d.
-// What bounds it: few columns, by bytes (18 or 34 a block of keys and of values, once a kv head) and by the some 270
-// vector instructions a 32-key tile of 128 4-bit channels takes (400 with f32 queries), which a CU's memory rate leaves
-// room for about twice; many columns, by the softmax's instructions beside the products (kv_many.h).  Measured, 32 query
-// heads over 8 of 128 channels, 4-bit, bf16: 64 sequences of up to 8192 keys 88 us (4.1 TB/s), one of 131072 38 us (4.0
-// TB/s), where a read of as many bytes takes 53 and 22 us.
+// What bounds it: few columns, by bytes (18 or 34 a block of keys and of values, once a kv head) and by vector
+// instructions: 346 counted a 32-key tile of 128 4-bit channels, bf16 (630 with f32 queries and 8-bit keys), which is 1400
+// cycles of a SIMD, whose share of the rate of a large read (6.85 TB/s) is the tile's bytes in 1650; many columns, by the
+// softmax's instructions beside the products (kv_many.h).  Measured, 32 query heads over 8 of 128 channels, 4-bit, bf16: 64
+// sequences of up to 8192 keys 85-88 us (4.2 TB/s), one of 131072 38 us (4.0 TB/s), where a read of as many bytes takes 53
+// and 22 us.
 // What is rounded: queries to f16 after a power of two that puts a column's largest at 2^13 (f16 and bf16 queries are
-// exact, except values 2^-27 of the largest), P and P' to f16 (2^-12 each, to nearest).  f32 queries (PREC) are held in
-// two f16 parts and P' in two, 22 bits each, two matrix instructions for one.  Scores, sums and accumulators are f32.
+// exact, except values 2^-27 of the largest), P' to f16 (2^-12, to nearest), and for bf16 queries P before it.  f32 queries
+// (PREC) are held in two f16 parts and P' in two, 22 bits each, two matrix instructions for one.  Scores, sums and
+// accumulators are f32.  Relative error against 64 bits, and of f32 operations rounded once: f16 2.4e-4 and 2.1e-4 (many
+// columns 2.9e-4), bf16 1.7e-3 and 1.6e-3, f32 2.8e-7 and 5.3e-7.
 //
 // One wave's keys are a range of tiles that no mask of its columns empties; inside it only the tiles at a mask's edge are
 // masked, and there a masked key's P' is set to 0, so what a masked or unwritten place holds (NaN scales too) is not seen.
@@ -772,7 +775,8 @@ struct Pages {
 
 // Few columns over many keys: the waves of a workgroup have the same 16 columns and share its keys out among them, a tile
 // each in turn; they join their sums in shared memory.  Registers decide how it hides the memory's latency: 3 waves a SIMD
-// (4 of 64 channels, 2 of 256, or 1 with f32 queries) with one tile in flight each, or for 8-bit tiles, twice as large, 2 waves with two.
+// (4 of 64 channels, 2 of 256, or 1 with f32 queries) with one tile in flight each, or for 8-bit tiles, twice as large, 2 waves
+// with two.  256 channels, 64 sequences of up to 8192 keys, 32 heads over 4: 4-bit 102 us (f32 queries 128), 8-bit 138 (209).
 // No kernel may spill registers (the compiler has stored a spilled one where only some lanes were on, and all lanes read it
 // again: wild addresses): 256 channels have their queries in shared memory.
 template <int NB, int KF, int VF, int MODE>

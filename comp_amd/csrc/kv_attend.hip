@@ -14,15 +14,16 @@ AttendPlan plan_of(const KvAttendCall& c) {
   const int64_t units = static_cast<int64_t>(c.batch) * c.cache.heads;
   AttendPlan p;
   // The many-column kernel unpacks a key once for 256 columns rather than 16, but starts slower and fills a CU with one
-  // workgroup: 8 sequences of 4096 keys, 8 kv heads, bf16, 96 columns 70 us (few) and 59, 128 columns 70 and 74, f32 83 and
-  // 80, 91 and 86; 48 columns 37 and 65.
+  // workgroup.  8 sequences of 4096 keys, 8 kv heads of 128 channels, 4-bit, few and many, us: 48 columns bf16 35 and 62, f32
+  // 46 and 59; 96 columns bf16 57 and 67, f16 61 and 72, f32 73 and 80; 128 columns bf16 68 and 69, f16 73 and 76, f32 88 and 84.
   p.many = cols > 96;
   const int wide = p.many ? many_cols(c.cache.dim, c.type) : 16;
   p.groups = std::max(1, static_cast<int>((cols + wide - 1) / wide));  // (none without query rows: such a call launches nothing)
   // Workgroups to fill the CUs (one of many columns each; of few three fit, and a fourth evens out what masks and short
-  // sequences leave empty: 16 sequences of up to 8192 keys and 1-5 rows, f32, 60 us with 512 workgroups, 64 with 768, 41
-  // with 1024, 44 with 1536), twice that where there are many sequences of unlike lengths (64 of up to 8192 keys, bf16: 106
-  // us with 1024, 92 with 2048, 94 with 4096); and no split of less than two tiles a wave or two buffers.  Pieces of few
+  // sequences leave empty: 16 sequences of up to 8192 keys and 1-5 rows, f32, 56 us with 512 workgroups, 45 with 768, 37
+  // with 1024, 39 with 1536; 8 of up to 3000 keys, 12 heads of 96 channels, f16, 18, 20, 20 and 20), twice that where there are
+  // many sequences of unlike lengths (64 of up to 8192 keys, bf16: 100 us with 1024, 89 with 2048, 90 with 4096; 40 of up to
+  // 3000, 20 heads over 5: 24 with each); and no split of less than two tiles a wave or two buffers.  Pieces of few
   // columns have the longest length's share of the splits, so that shorter sequences are cut into fewer, but enough
   // (`least`) to fill the CUs if all are that short.
   const int64_t fill = p.many ? 256 : 1024, aim = !p.many && units * p.groups >= 256 ? 2 * fill : fill;

@@ -14,9 +14,9 @@
 // whose scale is no number is held as zeros then, and makes NaN of its channels in the columns that see it.  f16 holds a scale
 // times that power whole down to 2^-14 of the largest (or at all, where the largest is below 2); where a tile has a smaller one,
 // of keys that some column sees or not, the workgroup begins again with exact operands.
-// Measured, 32 query heads over 8 of 128 channels, 4-bit, bf16: a prompt of 4096 tokens 275 us, 570 TFLOP/s where every key
-// is seen (f16 450, f32 210, twice the products), where a large library product reaches 1160: the vector unit is busy 46%
-// of the time, the matrix unit 20%.
+// Measured, 32 query heads over 8 of 128 channels, 4-bit: a prompt of 4096 tokens 268 us in bf16 (with the sums' logarithms
+// 356, f16 354, f32 516), 600 TFLOP/s where every key is seen (f16 450, f32 283, twice the products), where a large library
+// product reaches 1160: the vector unit is busy 43% of the time, the matrix unit 20%.
 #pragma once
 
 #include "kv_attend.h"

@@ -4,8 +4,8 @@
 // / -8 with max the signed value of largest magnitude (the first of equals), q = min(15, floor(x * (1 / d) + 8.5)); the
 // stored scale is f16(d).  A block that holds a NaN gets a NaN scale, so it reads back as NaN.
 //
-// Bound by bytes: 65536 tokens of 8 heads of 128 channels, f32 and Q8_0, are written in 158-173 us and read in 121-135 (679 MB
-// each way; a copy of as many bytes 141), 49999 tokens read from Q8_0 and Q4_0 as bf16 in 72 us (288 MB; 60).  One token
+// Bound by bytes: 65536 tokens of 8 heads of 128 channels, f32 and Q8_0, are written in 158-173 us and read in 114-146 (679 MB
+// each way; a copy of as many bytes 141), 49999 tokens read from Q8_0 and Q4_0 as bf16 in 71 us (288 MB; 60).  One token
 // each of 64 sequences: 2.8 and 2.7 us, a launch's own time.
 #include <hip/hip_ext.h>
 
@@ -505,7 +505,10 @@ dim3 grid_of(int64_t tokens, int per, int heads) {
   return dim3(static_cast<unsigned>((tokens + per - 1) / per * heads), 2);
 }
 
-// The kernels of 32-token tiles, from the size on where they fill the CUs (and their lists begin 0 to 31 tokens early).
+// The kernels of 32-token tiles, from the size on where they fill the CUs (and their lists begin 0 to 31 tokens early).  Few and
+// tiles, us, 8 heads of 128 channels, of 8192, 16384 and 32768 tokens times heads: write bf16 into Q8_0 keys and Q4_0 values
+// 4.3 and 5.7, 6.1 and 6.9, 10.2 and 10.1; f32 into Q8_0 4.9 and 5.6, 7.9 and 7.0, 14.5 and 10.8; read bf16 from the first 3.7 and
+// 4.4, 5.5 and 5.6, 8.9 and 8.5; f32 from the second 4.6 and 4.8, 7.1 and 6.8, 11.7 and 10.3.
 bool many_tokens(int64_t tokens, int heads) { return tokens * heads >= 32 * 512; }
 
 template <typename F, typename A>

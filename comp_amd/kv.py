@@ -286,8 +286,13 @@ def attend(cache, q, tables, lengths, starts=None, *, max_queries=None, max_leng
     A row that sees nothing gives zeros and an lse of -inf.
 
     max_queries: the most rows of one sequence (T by default); the results' places of rows past it hold anything (with 0 nothing
-    is computed at all).  max_length: an upper bound of the lengths that the launch is planned for (the tables' width by
-    default); any value gives the right result."""
+    is computed at all).  Give it where starts is given and sequences have a few rows each: one plan serves all sequences, and
+    T rows for each of them plan for a prompt.  max_length: an upper bound of the lengths that the launch is planned for (the
+    tables' width by default); any value gives the right result.
+
+    Scores, sums and accumulators are f32.  f32 queries keep 22 bits of queries and probabilities; f16 and bf16 queries hold the
+    probabilities in f16 (2^-12), bf16 ones of many rows also keys and values times their scales (where the logarithms are not
+    asked for: with return_lse their last bits differ)."""
     if not _attend_fits(cache, q, tables, lengths, starts, max_queries, prefix, slopes):
         _check_attend(cache, q, None, tables, lengths, starts, max_queries, prefix, slopes, None)
     out = cache.kq.new_empty(q.shape, dtype=q.dtype)

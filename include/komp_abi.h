@@ -284,7 +284,7 @@ int komp_kv_read(const komp_kv_cache* C, const int64_t* SLOTS, int64_t T, void* 
  * of a kv head counted; 0: nothing is computed, OUT and LSE stay as they are); max_length: the longest length, for the plan
  * alone (any value is right).  WORK: komp_kv_attend_workspace bytes for the same arguments (0: may be NULL), 16-byte aligned,
  * free again when the call has run.  Rows of Q that no sequence holds get unspecified results.  bf16 OUT is rounded from sums
- * that differ in their last bits with and without LSE. */
+ * whose last bits differ with and without LSE. */
 int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE, int type, const int32_t* TABLES,
                    const int32_t* LENGTHS, const int32_t* STARTS, const int32_t* PREFIX, const float* SLOPES, int64_t T,
                    int64_t batch, int64_t heads, int64_t q_stride_t, int64_t q_stride_h, int64_t out_stride_t,
