@@ -23,9 +23,11 @@ hipError_t launch_attend_mode(const AttendArgs& a, const AttendPlan& plan, int b
   if (plan.many) {
     const dim3 heads_first(grid.y, grid.z, grid.x);
     if constexpr (MODE == KV_BF16) {
-      if (a.lse == nullptr) return launch_attend_many<NB, KF, VF, MODE, true>(a, heads_first, stream);
+      if (a.lse == nullptr) return launch_attend_many<NB, KF, VF, MODE, KV_ALL_SCALED>(a, heads_first, stream);
+      return launch_attend_many<NB, KF, VF, MODE, KV_VALUES_SCALED>(a, heads_first, stream);
+    } else {
+      return launch_attend_many<NB, KF, VF, MODE, KV_EXACT>(a, heads_first, stream);
     }
-    return launch_attend_many<NB, KF, VF, MODE, false>(a, heads_first, stream);
   }
   return run(kv_attend_few_kernel<NB, KF, VF, MODE>, kAttendWaves * 64);
 }

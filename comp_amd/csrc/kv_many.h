@@ -7,15 +7,15 @@
 // after that in flight.
 //
 // f16 and f32 queries: the operands hold the codes, exact; the scales lie beside them and are used as in Columns::step.
-// bf16 queries (SCALED): the operands hold d * code, rounded to f16 after a power of two that brings the tile's largest scale
-// to [1, 2) and that the scores' factor or the probabilities' exponent takes back.  2^-12 of a key or value is an eighth of
-// what bf16 keeps of the result, and saves the f32 products of the partial dots and of the probabilities, half of a
-// column's instructions.  (Where the logarithms of the sums are asked for, in f32, the operands stay exact.)  A value block
+// bf16 queries: the operands hold d * code, rounded to f16 after a power of two that brings the tile's largest scale to [1, 2)
+// and that the scores' factor or the probabilities' exponent takes back.  2^-12 of a key or value is an eighth of what bf16
+// keeps of the result, and saves the f32 products of the partial dots and of the probabilities, half of a column's
+// instructions.  (Where the logarithms of the sums are asked for, in f32, keys stay exact: KV_VALUES_SCALED.)  A value block
 // whose scale is no number is held as zeros then, and makes NaN of its channels in the columns that see it.  f16 holds a scale
 // times that power whole down to 2^-14 of the largest (or at all, where the largest is below 2); where a tile has a smaller one,
 // of keys that some column sees or not, the workgroup begins again with exact operands.
 // Measured, 32 query heads over 8 of 128 channels, 4-bit: a prompt of 4096 tokens 268 us in bf16 (with the sums' logarithms
-// 356, f16 354, f32 516), 600 TFLOP/s where every key is seen (f16 450, f32 283, twice the products), where a large library
+// 309, f16 354, f32 515), 600 TFLOP/s where every key is seen (f16 450, f32 283, twice the products), where a large library
 // product reaches 1160: the vector unit is busy 43% of the time, the matrix unit 20%.
 #pragma once
 
@@ -23,10 +23,21 @@
 
 namespace komp {
 
-template <int NB, int KF, int VF, int MODE, bool SCALED>
+// what of the operands is multiplied by its scales: nothing, values, values and keys
+enum { KV_EXACT = 0, KV_VALUES_SCALED = 1, KV_ALL_SCALED = 2 };
+
+template <int NB, int KF, int VF, int MODE, int SCALED>
 struct Many {
-  static constexpr bool IN_OPERANDS = SCALED;
+  static constexpr bool V_SCALED = SCALED != KV_EXACT, K_SCALED = SCALED == KV_ALL_SCALED;
   static constexpr int BLOCKS = NB;
+  // Exact keys, and values multiplied by their scales on their way, of 128 channels: more than 256 registers, and a kernel may not
+  // spill.  Partial dots are held two blocks at a time then, and a lane's addresses are formed where they are used (which costs
+  // the kernels that have the room some 5%).
+  static constexpr bool TIGHT = SCALED == KV_VALUES_SCALED && NB == 4;
+  static __device__ __forceinline__ int here(int lane) {
+    if constexpr (TIGHT) asm volatile("" : "+v"(lane));
+    return lane;
+  }
   // two column tiles a wave halve the operand reads and the unpacking a column, where the registers (of two waves a SIMD)
   // hold their queries and sums: not f32 queries, in two parts, nor 256 channels
   static constexpr bool PAIR = NB <= 4 && MODE != KV_F32;
@@ -39,17 +50,17 @@ struct Many {
   static constexpr int KCHUNKS = KEYS / 16 * KG, VCHUNKS = HALVES * VG, CHUNKS = KCHUNKS + VCHUNKS;
   static constexpr int TURNS = (CHUNKS + WAVES - 1) / WAVES;  // chunks of one wave
   static constexpr int SW = (16 * NB + 63) / 64;              // dwords a lane of a half's scales, in a wave
-  // the largest exponent fields of a tile: of the values' and the keys' scales (SCALED), or of each half's values' scales
-  static constexpr int MOST = SCALED ? 2 : HALVES;
+  // the largest exponent fields of a tile: of the values' and the keys' scales, or of each half's values' scales (KV_EXACT)
+  static constexpr int MOST = V_SCALED ? 2 : HALVES;
   using Cols = Columns<NB, KF, VF, MODE, CT, true>;
 
   struct Shared {
     f16x8 k[2][HALVES * 2 * NB][64];  // [16 tokens][block]
     f16x8 v[2][HALVES * NB * 2][64];  // [32 tokens][block][channels 0..15, 16..31]
-    unsigned ks[2][SCALED ? 1 : HALVES][SCALED ? 1 : 16 * NB];
-    unsigned vs[2][SCALED ? 1 : HALVES][SCALED ? 1 : 16 * NB];
+    unsigned ks[2][K_SCALED ? 1 : HALVES][K_SCALED ? 1 : 16 * NB];
+    unsigned vs[2][V_SCALED ? 1 : HALVES][V_SCALED ? 1 : 16 * NB];
     unsigned most[4][MOST];
-    unsigned bad[4][SCALED ? 1 + HALVES * NB : 1];  // a tile's flags; which tokens of a half and block have a value scale
+    unsigned bad[4][V_SCALED ? 1 + HALVES * NB : 1];  // a tile's flags; which tokens of a half and block have a value scale
                                                     // that is no number
   };
   // flags: there are value scales that are no numbers; scales too far below the largest
@@ -57,11 +68,11 @@ struct Many {
   // a wave's chunks on their way from the cache to shared memory, and for the first waves the scales of a half
   struct Chunk {
     unsigned code[MD];
-    unsigned scale[SCALED ? 4 * VB : 1];
+    unsigned scale[V_SCALED ? 4 * VB : 1];
   };
   Chunk chunk[TURNS];
   bool there[TURNS];
-  unsigned ks[SCALED ? 1 : SW], vs[SCALED ? 1 : SW];
+  unsigned ks[K_SCALED ? 1 : SW], vs[V_SCALED ? 1 : SW];
 
   static __device__ __forceinline__ int half_of(int c) { return c < KCHUNKS ? c / KG >> 1 : (c - KCHUNKS) / VG; }
 
@@ -82,7 +93,7 @@ struct Many {
         const int t16 = c / KG & 1, g = c % KG;
         load_words<KD, KD>(cache.kq + u * (NB * 32 * kv_code_bytes(KF)) + t16 * (NB * 16 * kv_code_bytes(KF)) + (g * 64 + lane) * (KD * 4),
                            chunk[i].code);
-        if constexpr (SCALED) {
+        if constexpr (K_SCALED) {
           const uint16_t* sp = cache.ks + u * (32 * NB) + (t16 * 16 + (lane & 15)) * NB + g * KB;
           if constexpr (KB % 2 == 0) {
             load_words<KB / 2, KB / 2>(reinterpret_cast<const uint8_t*>(sp), chunk[i].scale);
@@ -94,19 +105,19 @@ struct Many {
       } else {
         const int g = (c - KCHUNKS) % VG;
         load_words<VD, VD>(cache.vq + u * (NB * 32 * kv_code_bytes(VF)) + (g * 64 + lane) * (VD * 4), chunk[i].code);
-        if constexpr (SCALED) {
+        if constexpr (V_SCALED) {
           const uint16_t* sp = cache.vs + u * (32 * NB) + ((lane >> 4) * NB + g * VB) * 8;
           load_words<4 * VB, 4>(reinterpret_cast<const uint8_t*>(sp), chunk[i].scale);
         }
       }
     }
-    if constexpr (!SCALED) if (wave < HALVES) {
+    if constexpr (!K_SCALED) if (wave < HALVES) {
       const int64_t u = unit(wave);
 #pragma unroll
       for (int i = 0; i < SW; ++i) {
         const int at = min(i * 64 + lane, 16 * NB - 1);
         ks[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.ks)[u * (16 * NB) + at];
-        vs[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.vs)[u * (16 * NB) + at];
+        if constexpr (!V_SCALED) vs[i] = u < 0 ? 0u : reinterpret_cast<const unsigned*>(cache.vs)[u * (16 * NB) + at];
       }
     }
   }
@@ -122,18 +133,20 @@ struct Many {
   // bad[slot]; the largest exponents go to most[slot].  (Scales beside the operands: the masks keep the products numbers.)
   __device__ __forceinline__ void look(Shared& sh, int slot, int first, int length, int wave, int lane) {
     unsigned e = 0, ek = 0;
-    if constexpr (SCALED) {
+    if constexpr (V_SCALED) {
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int c = i * WAVES + wave;
         if (!there[i]) continue;
         if (c < KCHUNKS) {
-          const bool in = (c / KG & 1) * 16 + (lane & 15) < length - first - half_of(c) * 32;
+          if constexpr (K_SCALED) {
+            const bool in = (c / KG & 1) * 16 + (lane & 15) < length - first - half_of(c) * 32;
 #pragma unroll
-          for (int b = 0; b < (KB % 2 == 0 ? KB / 2 : KB); ++b) {
-            chunk[i].scale[b] = in ? chunk[i].scale[b] : 0u;
-            const unsigned lo = chunk[i].scale[b] & 0x7C00u, hi = chunk[i].scale[b] >> 16 & 0x7C00u;
-            ek = max(ek, max(lo == 0x7C00u ? 0u : lo, hi == 0x7C00u ? 0u : hi));
+            for (int b = 0; b < (KB % 2 == 0 ? KB / 2 : KB); ++b) {
+              chunk[i].scale[b] = in ? chunk[i].scale[b] : 0u;
+              const unsigned lo = chunk[i].scale[b] & 0x7C00u, hi = chunk[i].scale[b] >> 16 & 0x7C00u;
+              ek = max(ek, max(lo == 0x7C00u ? 0u : lo, hi == 0x7C00u ? 0u : hi));
+            }
           }
           continue;
         }
@@ -173,14 +186,16 @@ struct Many {
       }
     }
     int top = static_cast<int>(e);
-    if constexpr (!SCALED) top = row16_max_i(top);  // (value operands: a row's lanes have the same scales)
+    if constexpr (!V_SCALED) top = row16_max_i(top);  // (value operands: a row's lanes have the same scales)
     top = static_cast<int>(quarters_max(static_cast<float>(top)));
-    if constexpr (!SCALED) {
+    if constexpr (!V_SCALED) {
       if (wave < HALVES && lane == 0) sh.most[slot][wave] = static_cast<unsigned>(top);
     } else {
       if (top && lane == 0) atomicMax(&sh.most[slot][0], static_cast<unsigned>(top));
-      const int k = row16_max_i(static_cast<int>(ek >> 10));  // (the quarters have the same keys)
-      if (k && lane == 0) atomicMax(&sh.most[slot][1], static_cast<unsigned>(k));
+      if constexpr (K_SCALED) {
+        const int k = row16_max_i(static_cast<int>(ek >> 10));  // (the quarters have the same keys)
+        if (k && lane == 0) atomicMax(&sh.most[slot][1], static_cast<unsigned>(k));
+      }
     }
   }
 
@@ -191,7 +206,7 @@ struct Many {
       const _Float16 f = static_cast<_Float16>(__builtin_ldexpf(1.f, 15 - static_cast<int>(max(sh.most[slot][which], 1u))));
       return f16x2{f, f};
     };
-    if constexpr (SCALED) {
+    if constexpr (V_SCALED) {
       fv = power(0), fk = power(1);
       // f16 scales (but 0) of exponent fields below this, 2 at least, lose bits to the power
       auto least = [&](int which) { return __builtin_amdgcn_readfirstlane(static_cast<int>(sh.most[slot][which])) - 14; };
@@ -199,7 +214,7 @@ struct Many {
         const unsigned lo = pair & 0x7FFFu, hi = pair >> 16 & 0x7FFFu, to = static_cast<unsigned>(field) << 10;
         return (lo != 0 && lo < to) || (hi != 0 && hi < to);
       };
-      const int kl = least(1), vl = least(0);
+      const int kl = K_SCALED ? least(1) : 0, vl = least(0);
       if (kl > 1 || vl > 1) {
         bool scattered = false;
 #pragma unroll
@@ -207,7 +222,7 @@ struct Many {
           if (!there[i]) continue;
           if (i * WAVES + wave < KCHUNKS) {
 #pragma unroll
-            for (int b = 0; b < (KB % 2 == 0 ? KB / 2 : KB); ++b) scattered |= kl > 1 && below(chunk[i].scale[b], kl);
+            for (int b = 0; K_SCALED && b < (KB % 2 == 0 ? KB / 2 : KB); ++b) scattered |= kl > 1 && below(chunk[i].scale[b], kl);
           } else {
 #pragma unroll
             for (int j = 0; j < 4 * VB; ++j) scattered |= vl > 1 && below(chunk[i].scale[j], vl);
@@ -227,7 +242,7 @@ struct Many {
           f16x8 x;
           if constexpr (KF == KV_Q4_0) x = key_codes<true, KF>(chunk[i].code[b], 0u);
           else x = key_codes<true, KF>(chunk[i].code[2 * b], chunk[i].code[2 * b + 1]);
-          if constexpr (SCALED) {
+          if constexpr (K_SCALED) {
             const _Float16 d = KB % 2 == 0 ? as_f16x2(chunk[i].scale[b >> 1])[b & 1] : as_f16x2(chunk[i].scale[b])[0];
             const f16x2 dd = f16x2{d, d} * fk;
             x *= f16x8{dd[0], dd[0], dd[0], dd[0], dd[0], dd[0], dd[0], dd[0]};
@@ -239,7 +254,7 @@ struct Many {
 #pragma unroll
         for (int b = 0; b < VB; ++b) {
           u32x4 d;
-          if constexpr (SCALED) {
+          if constexpr (V_SCALED) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) d[j] = __builtin_bit_cast(unsigned, as_f16x2(chunk[i].scale[4 * b + j]) * fv);
           }
@@ -248,18 +263,18 @@ struct Many {
             f16x8 x;
             if constexpr (VF == KV_Q4_0) x = value_codes<VF>(chunk[i].code[2 * b], chunk[i].code[2 * b + 1], hh);
             else x = value_codes<VF>(chunk[i].code[4 * b + 2 * hh], chunk[i].code[4 * b + 2 * hh + 1], 0);
-            if constexpr (SCALED) x *= __builtin_bit_cast(f16x8, d);
+            if constexpr (V_SCALED) x *= __builtin_bit_cast(f16x8, d);
             to[(b * 2 + hh) * 64] = x;
           }
         }
       }
     }
-    if constexpr (!SCALED) if (wave < HALVES) {
+    if constexpr (!K_SCALED) if (wave < HALVES) {
 #pragma unroll
       for (int i = 0; i < SW; ++i) {
         const int at = min(i * 64 + lane, 16 * NB - 1);
         sh.ks[buf][wave][at] = ks[i];
-        sh.vs[buf][wave][at] = vs[i];
+        if constexpr (!V_SCALED) sh.vs[buf][wave][at] = vs[i];
       }
     }
   }
@@ -269,48 +284,58 @@ struct Many {
                                               int half, int first, int lane) {
     constexpr int ROWS = (4 * NB + 15) / 16;  // a quarter's scales: dwords a lane of its 16
     const int quarter = lane >> 4, key0 = first + quarter * 4;
-    const int e = __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][SCALED ? 0 : half], 1u)));
+    const int e = __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][V_SCALED ? 0 : half], 1u)));
     unsigned ks[ROWS] = {};
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const int at = min(i * 16 + (lane & 15), 4 * NB - 1), t = at / (2 * NB);
-      if constexpr (!SCALED) ks[i] = sh.ks[buf][half][t * 8 * NB + quarter * 2 * NB + at - t * 2 * NB];
+      if constexpr (!K_SCALED) ks[i] = sh.ks[buf][half][t * 8 * NB + quarter * 2 * NB + at - t * 2 * NB];
     }
     float y[CT][2][4];
     each<2>([&](auto tc) {
       constexpr int t = tc.value;
-      f32x4 c[CT][NB];
+      // blocks at a time, whose partial dots are held until their scales come
+      constexpr int AT = TIGHT ? 2 : NB;
+      each<NB / AT>([&](auto gc) {
+        constexpr int b0 = gc.value * AT;
+        f32x4 c[CT][AT];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const f16x8 k = sh.k[buf][(half * 2 + t) * NB + b][lane];
+        for (int b = 0; b < AT; ++b) {
+          const f16x8 k = sh.k[buf][(half * 2 + t) * NB + b0 + b][lane];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          f32x4& x = c[ct][SCALED ? 0 : b];
-          if (!SCALED || b == 0) x = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int ct = 0; ct < CT; ++ct) {
+            f32x4& x = c[ct][K_SCALED ? 0 : b];
+            if (!K_SCALED || b == 0) x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int p = 0; p < Cols::PARTS; ++p) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, cols.qf[ct][b][p], x, 0, 0, 0);
+            for (int p = 0; p < Cols::PARTS; ++p) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, cols.qf[ct][b0 + b][p], x, 0, 0, 0);
+          }
         }
-      }
-      if constexpr (SCALED) {
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) y[ct][t][r] = c[ct][0][r];
-      } else each<2 * NB>([&](auto jc) {
-        constexpr int j = jc.value, at = t * 2 * NB + j;
-        const f16x2 d = as_f16x2(row_lane<at % 16>(ks[at / 16]));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = (2 * j + h) / NB, b = (2 * j + h) % NB;
+        if constexpr (K_SCALED) {
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct)
-            y[ct][t][r] = b == 0 ? static_cast<float>(d[h]) * c[ct][b][r] : fmaf(static_cast<float>(d[h]), c[ct][b][r], y[ct][t][r]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[ct][t][r] = c[ct][0][r];
+        } else {
+          // dword j has the scales of places 2 j and 2 j + 1 of [4 keys][NB]
+          each<2 * AT>([&](auto ic) {
+            constexpr int i = ic.value, j = AT == NB ? i : i * (NB / 2) + b0 / 2, at = t * 2 * NB + j;
+            const f16x2 d = as_f16x2(row_lane<at % 16>(ks[at / 16]));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = (2 * j + h) / NB, b = (2 * j + h) % NB - b0;
+#pragma unroll
+              for (int ct = 0; ct < CT; ++ct)
+                y[ct][t][r] = b0 + b == 0 ? static_cast<float>(d[h]) * c[ct][b][r] : fmaf(static_cast<float>(d[h]), c[ct][b][r], y[ct][t][r]);
+            }
+          });
         }
       });
     });
     const int left = min(Cols::ROOM, 21 - e);
-    if constexpr (SCALED) {
-      const float unit = __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][1], 1u))) - 15);
+    if constexpr (V_SCALED) {
+      float unit = 1.f;
+      if constexpr (K_SCALED)
+        unit = __builtin_ldexpf(1.f, __builtin_amdgcn_readfirstlane(static_cast<int>(max(sh.most[slot][1], 1u))) - 15);
       // (the power of two is the whole tile's, and so is what P may reach)
       cols.soften(a, masked, key0, left, unit, e - 15, y, nullptr);
     } else {
@@ -321,7 +346,7 @@ struct Many {
         return own;
       });
     }
-    if constexpr (SCALED) {
+    if constexpr (V_SCALED) {
       unsigned w[CT][4];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) Cols::pack(y[ct], w[ct]);
@@ -378,7 +403,7 @@ struct Many {
       const unsigned seen = lo >= hi ? 0u : (hi == 32 ? ~0u : (1u << hi) - 1) & ~((1u << lo) - 1);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const bool to = (sh.bad[slot][SCALED ? 1 + half * NB + b : 0] & seen) != 0;
+        const bool to = (sh.bad[slot][V_SCALED ? 1 + half * NB + b : 0] & seen) != 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           cols.acc[ct][2 * b][r] = to ? __builtin_nanf("") : cols.acc[ct][2 * b][r];
@@ -392,11 +417,11 @@ struct Many {
 // A workgroup's columns over its keys; false where a tile's scales are scattered, for all of its waves at the same point, and
 // nothing is stored then.
 template <typename M>
-__device__ __forceinline__ bool attend_many(const AttendArgs& a, typename M::Shared& sh) {
+__device__ __forceinline__ bool attend_many(const AttendArgs& a, typename M::Shared& sh, int thread, int h, int seq) {
   constexpr int NB = M::BLOCKS;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
   __builtin_assume(wave >= 0 && wave < M::WAVES);
-  const int h = blockIdx.x, seq = blockIdx.y, split = blockIdx.z / a.groups;
+  const int split = blockIdx.z / a.groups;
   // the groups of the latest positions, which see the most keys, begin first, those of all heads and sequences together
   const int group0 = (a.groups - 1 - (static_cast<int>(blockIdx.z) - split * a.groups)) * (M::WAVES * M::COLS);
   const Sequence s(a, seq);
@@ -433,9 +458,9 @@ __device__ __forceinline__ bool attend_many(const AttendArgs& a, typename M::Sha
   cols.begin(a, s, h, col0, lane, query);
   if (tile0 < tile1) {
     M m;
-    if (M::IN_OPERANDS && threadIdx.x < 4 * M::MOST) (&sh.most[0][0])[threadIdx.x] = 0;
-    constexpr int BAD = M::IN_OPERANDS ? 1 + M::HALVES * NB : 0;
-    if (threadIdx.x < 4 * BAD) (&sh.bad[0][0])[threadIdx.x] = 0;
+    if (M::V_SCALED && thread < 4 * M::MOST) (&sh.most[0][0])[thread] = 0;
+    constexpr int BAD = M::V_SCALED ? 1 + M::HALVES * NB : 0;
+    if (thread < 4 * BAD) (&sh.bad[0][0])[thread] = 0;
     unsigned now = halves(tile0);
     m.load(a.c, [&](int half) { return unit(tile0, half); }, wave, lane);
     __syncthreads();
@@ -450,25 +475,26 @@ __device__ __forceinline__ bool attend_many(const AttendArgs& a, typename M::Sha
       // most[] and bad[]: this tile's are in slot i, the next one's in i + 1, the one after's are filled in i + 2, and i + 3,
       // last read a turn ago, is cleared for the turn to come
       const int i = tile - tile0, buf = i & 1;
-      if (M::IN_OPERANDS && threadIdx.x < M::MOST) sh.most[(i + 3) & 3][threadIdx.x] = 0;
-      if (threadIdx.x < BAD) sh.bad[(i + 3) & 3][threadIdx.x] = 0;
-      m.unpack(sh, buf ^ 1, (i + 1) & 3, wave, lane);
+      if (M::V_SCALED && thread < M::MOST) sh.most[(i + 3) & 3][thread] = 0;
+      if (thread < BAD) sh.bad[(i + 3) & 3][thread] = 0;
+      const int at = M::here(lane);
+      m.unpack(sh, buf ^ 1, (i + 1) & 3, wave, at);
       const unsigned after = halves(tile + 2);
-      m.load(a.c, [&](int half) { return unit(tile + 2, half); }, wave, lane);
-      const unsigned flags = M::IN_OPERANDS ? __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) : 0u;
+      m.load(a.c, [&](int half) { return unit(tile + 2, half); }, wave, at);
+      const unsigned flags = M::V_SCALED ? __builtin_amdgcn_readfirstlane(sh.bad[i & 3][0]) : 0u;
       if (flags & M::SCATTERED) return false;  // (set before the last barrier: every wave sees it here)
 #pragma unroll 1
       for (int half = 0; half < M::HALVES; ++half) {
         const int first = tile * M::KEYS + half * 32;
         if (!any || first >= w1.hi || first + 32 <= w0.lo || !(now >> half & 1)) continue;
-        M::step(cols, a, sh, first < w1.lo || first + 32 > w0.hi, buf, i & 3, half, first, lane);
+        M::step(cols, a, sh, first < w1.lo || first + 32 > w0.hi, buf, i & 3, half, first, M::here(lane));
       }
       if (flags & M::SPOILT) {
 #pragma unroll 1
         for (int half = 0; half < M::HALVES; ++half)
           if (any && (now >> half & 1)) M::spoil(cols, sh, i & 3, half, tile * M::KEYS + half * 32);
       }
-      m.look(sh, (i + 2) & 3, (tile + 2) * M::KEYS, s.length, wave, lane);
+      m.look(sh, (i + 2) & 3, (tile + 2) * M::KEYS, s.length, wave, at);
       now = next;
       next = after;
       __syncthreads();
@@ -481,29 +507,34 @@ __device__ __forceinline__ bool attend_many(const AttendArgs& a, typename M::Sha
   return true;
 }
 
-template <int NB, int KF, int VF, int MODE, bool SCALED>
+template <int NB, int KF, int VF, int MODE, int SCALED>
 struct ManyKernel {
   using First = Many<NB, KF, VF, MODE, SCALED>;
-  using Exact = Many<NB, KF, VF, MODE, false>;
+  using Exact = Many<NB, KF, VF, MODE, KV_EXACT>;
   static constexpr int THREADS = 64 * First::WAVES;
   static constexpr size_t SHARED = sizeof(typename First::Shared) > sizeof(typename Exact::Shared) ? sizeof(typename First::Shared)
                                                                                                    : sizeof(typename Exact::Shared);
   static_assert(First::WAVES == Exact::WAVES && First::COLS == Exact::COLS, "one launch serves both");
 };
-template <int NB, int KF, int VF, int MODE, bool SCALED>
+template <int NB, int KF, int VF, int MODE, int SCALED>
 __global__ void __launch_bounds__((ManyKernel<NB, KF, VF, MODE, SCALED>::THREADS), (ManyKernel<NB, KF, VF, MODE, SCALED>::THREADS / 256))
 kv_attend_many_kernel(const AttendArgs a) {
   using K = ManyKernel<NB, KF, VF, MODE, SCALED>;
   extern __shared__ __attribute__((aligned(16))) unsigned char shared_bytes[];
-  const bool done = attend_many<typename K::First>(a, *reinterpret_cast<typename K::First::Shared*>(shared_bytes));
-  if constexpr (SCALED) {
+  int thread = threadIdx.x, h = blockIdx.x, seq = blockIdx.y;
+  const bool done = attend_many<typename K::First>(a, *reinterpret_cast<typename K::First::Shared*>(shared_bytes), thread, h, seq);
+  if constexpr (SCALED != KV_EXACT) {
     if (done) return;
     __syncthreads();
-    attend_many<typename K::Exact>(a, *reinterpret_cast<typename K::Exact::Shared*>(shared_bytes));
+    // (nothing of the first pass is held for this one: it loads the arguments again)
+    auto args = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+v"(thread), "+s"(h), "+s"(seq), "+s"(args));
+    const AttendArgs again = *(const AttendArgs*)(const void*)args;
+    attend_many<typename K::Exact>(again, *reinterpret_cast<typename K::Exact::Shared*>(shared_bytes), thread, h, seq);
   }
 }
 
-template <int NB, int KF, int VF, int MODE, bool SCALED>
+template <int NB, int KF, int VF, int MODE, int SCALED>
 hipError_t launch_attend_many(const AttendArgs& a, const dim3& grid, hipStream_t stream) {
   using K = ManyKernel<NB, KF, VF, MODE, SCALED>;
   static std::atomic<unsigned> limit[kMaxDevices];
