@@ -291,8 +291,8 @@ def attend(cache, q, tables, lengths, starts=None, *, max_queries=None, max_leng
     tables' width by default); any value gives the right result.
 
     Scores, sums and accumulators are f32.  f32 queries keep 22 bits of queries and probabilities; f16 and bf16 queries hold the
-    probabilities in f16 (2^-12), bf16 ones of many rows also keys and values times their scales (where the logarithms are not
-    asked for: with return_lse their last bits differ)."""
+    probabilities in f16 (2^-12), bf16 ones of many rows also values times their scales, and keys too where the logarithms are
+    not asked for (the results' last bits differ with return_lse)."""
     if not _attend_fits(cache, q, tables, lengths, starts, max_queries, prefix, slopes):
         _check_attend(cache, q, None, tables, lengths, starts, max_queries, prefix, slopes, None)
     out = cache.kq.new_empty(q.shape, dtype=q.dtype)
