@@ -75,6 +75,12 @@ SIGNATURES = {
     "komp_kv_attend": (_INT, [_P, _P, _P, _P, _INT, _P, _P, _P, _P, _P, *[_I64] * 11, ctypes.c_float, ctypes.c_float, _I64,
                               _P, _I64, _P]),
     "komp_kv_attend_workspace": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _I64, _P]),
+    "komp_mx_quantize": (_INT, [_P, _P, _INT, _I64, _INT, _P]),
+    "komp_mx_lookup": (_INT, [_P, _P, _I64, _P, _INT, _I64, ctypes.c_float, _P]),
+    "komp_mx_pack": (_INT, [_P, _P, _P, _P]),
+    "komp_mx_unpack": (_INT, [_P, _P, _P, _P]),
+    "komp_mx_gemm": (_INT, [_P, _P, _P, _INT, _I64, _P]),
+    "komp_mx_linear": (_INT, [_P, _INT, _I64, _I64, _INT, _P, _P, _INT, _I64, _P]),
     "komp_timing_begin": (_INT, [_I64]),
     "komp_timing_end": (_INT, [_P, _P]),
     "komp_stamps_begin": (_INT, [_P, _I64]),
@@ -89,6 +95,12 @@ class KvCacheStruct(ctypes.Structure):
 
     _fields_ = [("KQ", _P), ("KS", _P), ("VQ", _P), ("VS", _P), ("pages", _I64), ("heads", _INT), ("head_dim", _INT),
                 ("page", _INT), ("k_fmt", _INT), ("v_fmt", _INT)]  # fmt: skip
+
+
+class MxRowsStruct(ctypes.Structure):
+    """komp_mx_rows of include/komp_abi.h."""
+
+    _fields_ = [("CODES", _P), ("SCALES", _P), ("rows", _I64), ("k", _I64), ("fmt", _INT)]
 
 
 _lib = None

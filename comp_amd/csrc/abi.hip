@@ -12,6 +12,7 @@
 #include "../../include/komp_abi.h"
 #include "komp_internal.h"
 #include "kv_layout.h"
+#include "mx_layout.h"
 
 namespace komp {
 namespace {
@@ -1354,6 +1355,161 @@ int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE,
   c.work = WORK;
   c.work_bytes = work_bytes;
   return hip_status(launch_kv_attend(c, static_cast<hipStream_t>(stream)), name);
+}
+
+}  // extern "C"
+
+namespace komp {
+namespace {
+
+int mx_rows_of(const char* name, const char* what, const komp_mx_rows* R, MxRows& r) {
+  if (R == nullptr) return fail(KOMP_EINVAL, "%s: %s is NULL", name, what);
+  if (R->fmt != MX_E2M1 && R->fmt != MX_E4M3) return fail(KOMP_EINVAL, "%s: %s: fmt=%d (0 e2m1, 1 e4m3)", name, what, R->fmt);
+  if (R->k < 32 || R->k % 32 != 0 || R->k > (INT64_C(1) << 26))
+    return fail(KOMP_EINVAL, "%s: %s: k=%lld must be a multiple of 32, from 32 to 2^26", name, what, static_cast<long long>(R->k));
+  if (R->rows < 0 || R->rows > INT64_C(0x7FFFFFFF) || mx_tiles(R->rows) * mx_supers(R->k) > INT64_C(0x7FFFFFFF))
+    return fail(KOMP_EINVAL, "%s: %s: %lld rows of %lld", name, what, static_cast<long long>(R->rows), static_cast<long long>(R->k));
+  if (R->rows > 0 && (R->CODES == nullptr || R->SCALES == nullptr)) return fail(KOMP_EINVAL, "%s: %s: a plane is NULL", name, what);
+  if (!aligned(R->CODES, 16) || !aligned(R->SCALES, 16))
+    return fail(KOMP_EINVAL, "%s: %s: the planes must be 16-byte aligned", name, what);
+  r = MxRows{R->CODES, R->SCALES, R->rows, R->k, R->fmt};
+  return KOMP_OK;
+}
+
+int mx_type_of(const char* name, int type, const void* p, int64_t stride) {
+  if (type < MX_F32 || type > MX_BF16) return fail(KOMP_EINVAL, "%s: type=%d (0 f32, 1 f16, 2 bf16)", name, type);
+  if (p == nullptr) return fail(KOMP_EINVAL, "%s: an array is NULL", name);
+  if (!aligned(p, type == MX_F32 ? 4 : 2)) return fail(KOMP_EINVAL, "%s: an array is not aligned to its elements", name);
+  const int64_t most = INT64_C(1) << 40;
+  if (stride > most || stride < -most) return fail(KOMP_EINVAL, "%s: row stride %lld", name, static_cast<long long>(stride));
+  return KOMP_OK;
+}
+
+// Y [t][w.rows]: the shapes that the kernels' grids and 32-bit sizes hold
+int mx_product(const char* name, int64_t t, const MxRows& w) {
+  if (w.fmt != MX_E2M1) return fail(KOMP_EINVAL, "%s: W must be e2m1 rows", name);
+  if (mx_tiles(t) > 65535 || mx_tiles(w.rows) > (INT64_C(1) << 22))
+    return fail(KOMP_EINVAL, "%s: %lld x %lld results (2^20 - 16 rows of X and 2^26 of W at most)", name, static_cast<long long>(t),
+                static_cast<long long>(w.rows));
+  return KOMP_OK;
+}
+
+}  // namespace
+}  // namespace komp
+
+extern "C" {
+
+int komp_mx_quantize(const komp_mx_rows* R, const void* X, int type, int64_t x_stride, int act, void* stream) {
+  const char* name = "komp_mx_quantize";
+  MxQuantCall c;
+  int st = mx_rows_of(name, "R", R, c.r);
+  if (st != KOMP_OK) return st;
+  if (act < MX_PLAIN || act > MX_RELU2) return fail(KOMP_EINVAL, "%s: act=%d (0 none, 1 silu, 2 relu2)", name, act);
+  if (c.r.rows == 0) return KOMP_OK;
+  st = mx_type_of(name, type, X, x_stride);
+  if (st != KOMP_OK) return st;
+  c.x = X;
+  c.type = type;
+  c.stride = x_stride;
+  c.act = act;
+  return hip_status(launch_mx_quantize(c, static_cast<hipStream_t>(stream)), name);
+}
+
+int komp_mx_lookup(const komp_mx_rows* R, const int64_t* IDS, int64_t count, void* OUT, int type, int64_t out_stride,
+                   float factor, void* stream) {
+  const char* name = "komp_mx_lookup";
+  MxLookupCall c;
+  int st = mx_rows_of(name, "R", R, c.r);
+  if (st != KOMP_OK) return st;
+  if (count < 0 || count > INT64_C(0x7FFFFFFF) || mx_tiles(count) * mx_supers(c.r.k) > INT64_C(0x7FFFFFFF))
+    return fail(KOMP_EINVAL, "%s: count=%lld rows of %lld", name, static_cast<long long>(count), static_cast<long long>(c.r.k));
+  if (count == 0) return KOMP_OK;  // (an empty array of ids may be NULL)
+  if (IDS == nullptr && count != c.r.rows)
+    return fail(KOMP_EINVAL, "%s: count=%lld without IDS (all of the %lld rows)", name, static_cast<long long>(count),
+                static_cast<long long>(c.r.rows));
+  if (!aligned(IDS, 8)) return fail(KOMP_EINVAL, "%s: IDS must be 8-byte aligned", name);
+  st = mx_type_of(name, type, OUT, out_stride);
+  if (st != KOMP_OK) return st;
+  c.ids = IDS;
+  c.count = count;
+  c.out = OUT;
+  c.type = type;
+  c.stride = out_stride;
+  c.factor = factor;
+  return hip_status(launch_mx_lookup(c, static_cast<hipStream_t>(stream)), name);
+}
+
+int komp_mx_pack(const komp_mx_rows* R, const uint8_t* CODES, const uint8_t* SCALES, void* stream) {
+  const char* name = "komp_mx_pack";
+  MxPackCall c;
+  const int st = mx_rows_of(name, "R", R, c.r);
+  if (st != KOMP_OK) return st;
+  c.ggml = SCALES == nullptr;
+  if (c.ggml && c.r.fmt != MX_E2M1) return fail(KOMP_EINVAL, "%s: SCALES is NULL (block_mxfp4 blocks are e2m1)", name);
+  if (c.r.rows == 0) return KOMP_OK;
+  if (CODES == nullptr) return fail(KOMP_EINVAL, "%s: CODES is NULL", name);
+  c.codes = const_cast<uint8_t*>(CODES);
+  c.scales = const_cast<uint8_t*>(SCALES);
+  c.unpack = false;
+  return hip_status(launch_mx_pack(c, static_cast<hipStream_t>(stream)), name);
+}
+
+int komp_mx_unpack(const komp_mx_rows* R, uint8_t* CODES, uint8_t* SCALES, void* stream) {
+  const char* name = "komp_mx_unpack";
+  MxPackCall c;
+  const int st = mx_rows_of(name, "R", R, c.r);
+  if (st != KOMP_OK) return st;
+  if (c.r.rows == 0) return KOMP_OK;
+  if (CODES == nullptr || SCALES == nullptr) return fail(KOMP_EINVAL, "%s: CODES or SCALES is NULL", name);
+  c.codes = CODES;
+  c.scales = SCALES;
+  c.ggml = false;
+  c.unpack = true;
+  return hip_status(launch_mx_pack(c, static_cast<hipStream_t>(stream)), name);
+}
+
+int komp_mx_gemm(const komp_mx_rows* X, const komp_mx_rows* W, void* Y, int type, int64_t y_stride, void* stream) {
+  const char* name = "komp_mx_gemm";
+  MxGemmCall c;
+  int st = mx_rows_of(name, "X", X, c.x);
+  if (st == KOMP_OK) st = mx_rows_of(name, "W", W, c.w);
+  if (st == KOMP_OK) st = mx_product(name, c.x.rows, c.w);
+  if (st != KOMP_OK) return st;
+  if (c.x.k != c.w.k)
+    return fail(KOMP_EINVAL, "%s: X has rows of %lld, W of %lld", name, static_cast<long long>(c.x.k), static_cast<long long>(c.w.k));
+  if (c.x.rows == 0 || c.w.rows == 0) return KOMP_OK;
+  st = mx_type_of(name, type, Y, y_stride);
+  if (st != KOMP_OK) return st;
+  c.src = nullptr;
+  c.src_type = 0;
+  c.src_stride = 0;
+  c.y = Y;
+  c.type = type;
+  c.stride = y_stride;
+  return hip_status(launch_mx_gemm(c, static_cast<hipStream_t>(stream)), name);
+}
+
+int komp_mx_linear(const void* X, int x_type, int64_t x_stride, int64_t T, int fmt, const komp_mx_rows* W, void* Y, int type,
+                   int64_t y_stride, void* stream) {
+  const char* name = "komp_mx_linear";
+  MxGemmCall c;
+  int st = mx_rows_of(name, "W", W, c.w);
+  if (st == KOMP_OK) st = mx_product(name, T, c.w);
+  if (st != KOMP_OK) return st;
+  if (fmt != MX_E2M1 && fmt != MX_E4M3) return fail(KOMP_EINVAL, "%s: fmt=%d (0 e2m1, 1 e4m3)", name, fmt);
+  if (T < 0 || T > kMxLinearRows) return fail(KOMP_EINVAL, "%s: T=%lld rows (0 to %d)", name, static_cast<long long>(T), kMxLinearRows);
+  if (T == 0 || c.w.rows == 0) return KOMP_OK;
+  st = mx_type_of(name, x_type, X, x_stride);
+  if (st == KOMP_OK) st = mx_type_of(name, type, Y, y_stride);
+  if (st != KOMP_OK) return st;
+  c.x = MxRows{nullptr, nullptr, T, c.w.k, fmt};
+  c.src = X;
+  c.src_type = x_type;
+  c.src_stride = x_stride;
+  c.y = Y;
+  c.type = type;
+  c.stride = y_stride;
+  return hip_status(launch_mx_gemm(c, static_cast<hipStream_t>(stream)), name);
 }
 
 }  // extern "C"

@@ -294,12 +294,51 @@ int komp_kv_attend(const komp_kv_cache* C, const void* Q, void* OUT, float* LSE,
 int komp_kv_attend_workspace(const komp_kv_cache* C, int type, int64_t T, int64_t batch, int64_t heads,
                              int64_t max_queries, int64_t max_length, int64_t* bytes);
 
+/* Microscaled rows: blocks of 32 floating point elements, e2m1 (4 bits) or e4m3 (8 bits), with one scale byte s that stands for
+ * 2^(s - 127) (255: every value of the block is NaN), the OCP microscaling formats MXFP4 and MXFP8.  No reference counterpart.
+ *   k a multiple of 32; with S = ceil(k / 128), CODES u8 [ceil(rows / 16)][S * 1024 (e2m1) or S * 2048 (e4m3)] and SCALES u8
+ *   [ceil(rows / 16)][ceil(k / 512) * 256], each 16-byte aligned.  The order of the bytes is the library's own (tiles of 16 rows
+ *   in the matrix instruction's order): rows are written and read through these entries, which keep the places behind the
+ *   last row and the last block zero.
+ * type: 0 f32, 1 f16, 2 bf16 (X, Y, OUT); fmt: 0 e2m1, 1 e4m3.  Strides count elements between rows; a row is contiguous. */
+typedef struct komp_mx_rows {
+  uint8_t* CODES;
+  uint8_t* SCALES;
+  int64_t rows;
+  int64_t k;
+  int fmt;
+} komp_mx_rows;
+
+/* R = the rows of X [rows][k] (act 0), of silu(g) * u (act 1) or of max(g, 0)^2 * u (act 2) with g and u the halves of X's rows
+ * [rows][2 k]: computed in 64 bits and rounded to f32 once, silu(g) = g / (1 + e^-g).  A block's scale is 2^(floor(log2 of its
+ * largest magnitude) - 2 (e2m1) or 8 (e4m3)), 2^-127 at least; elements are rounded to the nearest, ties to even, and saturate (at 6
+ * and 448).  A block that holds an infinity or a NaN gets the scale byte 255 and zero codes. */
+int komp_mx_quantize(const komp_mx_rows* R, const void* X, int type, int64_t x_stride, int act, void* stream);
+
+/* OUT [count][k]: the values of the rows IDS[0 .. count - 1], each times `factor` in f32, rounded to `type`; IDS NULL: all rows
+ * (count = R->rows).  An id below 0 or past the rows gives zeros. */
+int komp_mx_lookup(const komp_mx_rows* R, const int64_t* IDS, int64_t count, void* OUT, int type, int64_t out_stride,
+                   float factor, void* stream);
+
+/* Rows from and to plain planes: CODES u8 [rows][k / 2] (e2m1, the low nibble first) or [rows][k] (e4m3), SCALES u8 [rows]
+ * [k / 32].  komp_mx_pack with SCALES NULL: CODES are ggml block_mxfp4 blocks [rows][k / 32][17]. */
+int komp_mx_pack(const komp_mx_rows* R, const uint8_t* CODES, const uint8_t* SCALES, void* stream);
+int komp_mx_unpack(const komp_mx_rows* R, uint8_t* CODES, uint8_t* SCALES, void* stream);
+
+/* Y [X->rows][W->rows] = X W^T of what the rows stand for, W e2m1, sums in f32, rounded once to `type`. */
+int komp_mx_gemm(const komp_mx_rows* X, const komp_mx_rows* W, void* Y, int type, int64_t y_stride, void* stream);
+
+/* The same for T rows X [T][W->k] of floats (T at most 16), quantized to `fmt` inside the launch: equal to komp_mx_quantize and
+ * komp_mx_gemm bit for bit. */
+int komp_mx_linear(const void* X, int x_type, int64_t x_stride, int64_t T, int fmt, const komp_mx_rows* W, void* Y, int type,
+                   int64_t y_stride, void* stream);
+
 /* Dispatch timing for the tuning harness (no reference counterpart; the reference was never timed).
  * Between komp_timing_begin() and komp_timing_end(), every launch made by this library on the calling process is
  * issued with hipExtLaunchKernel start/stop events, which the runtime stamps with the dispatch's own begin and end.
  * komp_timing_end() waits for those events and returns, per kernel kind, the summed dispatch time in milliseconds and
  * the dispatch count.  Kinds: 0 quant_q8_0, 1 quant_q8_K, 2 q4_0 GEMV / GEMM, 3 tq2_0 GEMV / GEMM, 4 probes,
- * weight splits and the key/value cache's operators, 5 q8_0 GEMV / GEMM, 6 iq4_nl GEMV / GEMM, 7 q4_k GEMV (arrays of length 8).
+ * weight splits, the key/value cache's and the microscaled rows' operators, 5 q8_0 GEMV / GEMM, 6 iq4_nl GEMV / GEMM, 7 q4_k GEMV (arrays of length 8).
  * max_dispatches bounds the events created. */
 #define KOMP_TIMING_KINDS 8
 int komp_timing_begin(int64_t max_dispatches);
