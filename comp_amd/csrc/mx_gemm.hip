@@ -26,6 +26,8 @@ struct GemmArgs {
   int k;
   void* y;
   int64_t y_stride;
+  int type;                // of y
+  int x_type;              // of x, quantized on the way
 };
 
 // One step's operand of one row tile: codes, and the dword of its four steps' scales.
@@ -92,8 +94,7 @@ __device__ __forceinline__ void mma_step(f32x4 (&acc)[RT][CT], const Operand<MX_
 
 // Four outputs n .. n + 3 of row t.
 template <int TYPE>
-__device__ __forceinline__ void store4(const GemmArgs& a, int64_t t, int64_t n, f32x4 v) {
-  if (t >= a.t || n >= a.n) return;
+__device__ __forceinline__ void store4_as(const GemmArgs& a, int64_t t, int64_t n, f32x4 v) {
   const int64_t at = t * a.y_stride + n;
   if (n + 4 <= a.n) {
     const float f[4] = {v[0], v[1], v[2], v[3]};
@@ -106,16 +107,221 @@ __device__ __forceinline__ void store4(const GemmArgs& a, int64_t t, int64_t n, 
     }
   }
 }
+__device__ __forceinline__ void store4(const GemmArgs& a, int64_t t, int64_t n, f32x4 v) {
+  if (t >= a.t || n >= a.n) return;
+  if (a.type == MX_F32) store4_as<MX_F32>(a, t, n, v);
+  else if (a.type == MX_F16) store4_as<MX_F16>(a, t, n, v);
+  else store4_as<MX_BF16>(a, t, n, v);
+}
+
+// Eight elements each of the first `count` of N rows that are quantized on the way, zeros of the others.
+template <int TYPE, int N>
+__device__ __forceinline__ void load_rows_as(const GemmArgs& a, int count, int64_t at, float (&v)[N][8]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    if (i < count) mx_load<TYPE>(a.x, at + i * a.x_stride, v[i]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_rows(const GemmArgs& a, int count, int64_t at, float (&v)[N][8]) {
+  if (a.x_type == MX_F32) load_rows_as<MX_F32>(a, count, at, v);
+  else if (a.x_type == MX_F16) load_rows_as<MX_F16>(a, count, at, v);
+  else load_rows_as<MX_BF16>(a, count, at, v);
+}
+
+// ---- one column tile of X --------------------------------------------------------------------------------------------
+
+// X's operands of a four-step piece, ready for mma_piece: as they are (e2m1; e4m3 in eight registers a step), or in bf16.
+template <int FMT, bool WIDE>
+struct PieceX {
+  Operand<FMT> x[4];
+  unsigned scales;
+};
+template <>
+struct PieceX<MX_E4M3, true> {
+  bf16x8 b[4][4];
+};
+
+struct PieceW {
+  Operand<MX_E2M1> w[4];
+  unsigned scales;
+};
+
+// acc += a piece's products.  A step behind K's end has zero codes in X (the codes of W are the last step's again).
+template <int FMT, bool WIDE>
+__device__ __forceinline__ void mma_piece(f32x4& acc, const PieceW& w, const PieceX<FMT, WIDE>& x) {
+  f32x4 out[1][1] = {{acc}};
+  if constexpr (FMT == MX_E4M3 && WIDE) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const float scale = scale_of(w.scales, s);
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        out[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_part(w.w[s], p, scale), x.b[s][p], out[0][0], 0, 0, 0);
+    }
+  } else {
+    auto step = [&](auto at) {
+      constexpr int S = decltype(at)::value;
+      const Operand<MX_E2M1> ws[1] = {w.w[S]};
+      const Operand<FMT> xs[1] = {x.x[S]};
+      const unsigned w_scales[1] = {w.scales}, x_scales[1] = {x.scales};
+      mma_step<FMT, S>(out, ws, w_scales, xs, x_scales);
+    };
+    step(std::integral_constant<int, 0>());
+    step(std::integral_constant<int, 1>());
+    step(std::integral_constant<int, 2>());
+    step(std::integral_constant<int, 3>());
+  }
+  acc = out[0][0];
+}
+
+// Up to 16 rows of X.  A workgroup keeps X in registers, each wave P pieces of K, and walks over row tiles of W, whose codes
+// it loads D pieces ahead; its waves join in shared memory, in their order.  FLOATS: the rows are quantized on the way, by each
+// wave its own pieces, eight elements a lane, through shared memory into the operands' order.
+template <int FMT, bool FLOATS, int P, int D>
+__global__ __launch_bounds__(P == 1 ? 1024 : 512) void mx_step_kernel(const GemmArgs a) {
+  constexpr bool kWide = P == 1;
+  constexpr int kTiles = D > P ? D / P : 1;                   // row tiles a turn of the loop
+  constexpr int kColumn = (FMT == MX_E2M1 ? 256 : 512) + 16;  // bytes of a column's piece, apart in the banks
+  extern __shared__ f32x4 shared[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int steps = static_cast<int>(mx_steps(a.k)), supers = static_cast<int>(mx_supers(a.k));
+  const int tiles = static_cast<int>(mx_tiles(a.n)), pace = gridDim.x;
+  const int64_t w_bytes = mx_code_bytes(a.k, MX_E2M1), s_bytes = mx_scale_bytes(a.k);
+  const int column = lane & 15, group = lane >> 4;
+  PieceW w[D];
+  auto fetch = [&](PieceW& into, int tile, int p) {
+    const int sp = wave + waves * p;
+    if (tile >= tiles || sp >= supers) return;
+    into.scales = reinterpret_cast<const unsigned*>(a.ws + tile * s_bytes)[sp * 64 + lane];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int step = sp * 4 + s < steps ? sp * 4 + s : steps - 1;
+      into.w[s].q[0] = reinterpret_cast<const u32x4*>(a.w + tile * w_bytes)[step * 64 + lane];
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) fetch(w[d], blockIdx.x + d / P * pace, d % P);
+  PieceX<FMT, kWide> x[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int sp = wave + waves * p;
+    Operand<FMT> q[4];
+    unsigned scales = 0;
+    if (sp < supers) {
+      if constexpr (FLOATS) {
+        uint8_t* const mine = reinterpret_cast<uint8_t*>(shared) + wave * (static_cast<int>(a.t) * kColumn + 256);
+        uint8_t* const mine_scales = mine + a.t * kColumn;
+        constexpr int kAtOnce = P == 1 ? 4 : 2;  // rows whose loads are on their way together
+        const int count = static_cast<int>(a.t);
+        const bool in = (sp * 16 + (lane >> 2)) * 32 < a.k;
+        for (int t0 = 0; t0 < count; t0 += kAtOnce) {
+          float v[kAtOnce][8];
+          load_rows<kAtOnce>(a, in ? count - t0 : 0, t0 * a.x_stride + sp * 512 + lane * 8, v);
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) {
+            const int t = t0 + i;
+            if (t >= count) break;
+            unsigned most = mx_most(v[i]);
+            most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR1>(static_cast<int>(most))));
+            most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR2>(static_cast<int>(most))));
+            const unsigned scale = mx_scale<FMT>(most);
+            unsigned c[FMT == MX_E2M1 ? 1 : 2];
+            mx_codes8<FMT>(v[i], scale, c);
+            if constexpr (FMT == MX_E2M1) *reinterpret_cast<unsigned*>(mine + t * kColumn + lane * 4) = c[0];
+            else *reinterpret_cast<u32x2*>(mine + t * kColumn + lane * 8) = u32x2{c[0], c[1]};
+            // block 4 s + g of the piece: byte s of group g's dword
+            if ((lane & 3) == 0) mine_scales[(((lane >> 2) & 3) * 16 + t) * 4 + (lane >> 4)] = static_cast<uint8_t>(scale);
+          }
+        }
+        // lanes read what others of their wave wrote
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (column < a.t) {
+          scales = reinterpret_cast<const unsigned*>(mine_scales)[lane];
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const u32x4* const from = reinterpret_cast<const u32x4*>(mine + column * kColumn) + (s * 4 + group) * (FMT == MX_E2M1 ? 1 : 2);
+            q[s].q[0] = from[0];
+            if constexpr (FMT == MX_E4M3) q[s].q[1] = from[1];
+          }
+        }
+      } else {
+        scales = reinterpret_cast<const unsigned*>(a.xs)[sp * 64 + lane];
+        constexpr int parts = FMT == MX_E2M1 ? 1 : 2;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int h = 0; h < parts; ++h) {
+            const int step = sp * 4 + s < steps ? sp * 4 + s : steps - 1;
+            q[s].q[h] = reinterpret_cast<const u32x4*>(a.x)[(step * parts + h) * 64 + lane];
+          }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const bool in = column < a.t && sp * 4 + s < steps;
+#pragma unroll
+      for (int h = 0; h < (FMT == MX_E2M1 ? 1 : 2); ++h) q[s].q[h] = in ? q[s].q[h] : u32x4{0, 0, 0, 0};
+      if (!in) scales &= ~(255u << (8 * s));
+    }
+    if constexpr (FMT == MX_E4M3 && kWide) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[p].b[s][j] = bf16_part(q[s], j, scale_of(scales, s));
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) x[p].x[s] = q[s];
+      x[p].scales = scales;
+    }
+  }
+  if constexpr (FLOATS) __syncthreads();  // the waves' places are the join's from here on
+  int turn = 0;
+  for (int base = blockIdx.x; base < tiles; base += kTiles * pace) {
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u) {
+      const int tile = base + u * pace;
+      if (tile >= tiles) break;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        // (opaque scales: nothing made from x is kept over the tiles, which would not fit)
+        if constexpr (!(FMT == MX_E4M3 && kWide)) asm volatile("" : "+v"(x[p].scales));
+        const int item = u * P + p;  // of this turn; D items on, its place is free again
+        if (wave + waves * p < supers) mma_piece<FMT, kWide>(acc, w[item % D], x[p]);
+        fetch(w[item % D], base + (item + D) / P * pace, (item + D) % P);
+      }
+      const int64_t n = static_cast<int64_t>(tile) * 16 + group * 4;
+      if (waves == 1) {
+        store4(a, column, n, acc);
+        continue;
+      }
+      f32x4* const join = shared + (turn & 1) * waves * 64 + lane;
+      if (column < a.t) join[wave * 64] = acc;
+      __syncthreads();
+      if (wave == turn % waves && column < a.t) {
+        f32x4 sum = join[0];
+        for (int v = 1; v < waves; ++v) sum += join[v * 64];
+        store4(a, column, n, sum);
+      }
+      ++turn;
+    }
+  }
+}
 
 // ---- few rows of X ---------------------------------------------------------------------------------------------------
 
 // Operands come straight from memory: a workgroup has RT row tiles of W and CT tiles of X, its waves take four-step pieces of
 // K in turn and join in shared memory, in the waves' order.  SRC: the type of the rows that are quantized on the way (each wave
 // its own pieces), -1: X is quantized already.
-template <int FMT, int SRC, int TYPE, int RT, int CT>
-__global__ __launch_bounds__(512) void mx_stream_kernel(const GemmArgs a) {
+template <int FMT, int SRC, int RT, int CT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const GemmArgs a) {
+  constexpr int kParts = FMT == MX_E2M1 ? 1 : 2;
   extern __shared__ f32x4 join[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int steps = static_cast<int>(mx_steps(a.k)), supers = static_cast<int>(mx_supers(a.k));
   const int64_t w_tiles = mx_tiles(a.n), x_tiles = mx_tiles(a.t);
   const int64_t w0 = static_cast<int64_t>(blockIdx.x) * RT, x0 = static_cast<int64_t>(blockIdx.y) * CT;
@@ -127,35 +333,43 @@ __global__ __launch_bounds__(512) void mx_stream_kernel(const GemmArgs a) {
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int j = 0; j < CT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int sp = wave; sp < supers; sp += waves) {
-    Operand<MX_E2M1> w[4][RT];
-    unsigned ws[RT], xs[CT];
-    Operand<FMT> x[4][CT];
-    const int here = steps - sp * 4;  // steps of this piece
+  Operand<MX_E2M1> w[4][RT];
+  Operand<FMT> x[4][CT];
+  unsigned ws[RT], xs[CT], ws_next[RT], xs_next[CT];
+  // step `s` of piece `sp`; a step past the last one is the last one again, and not used
+  auto fetch = [&](int sp, int s) {
+    const int step = sp * 4 + s < steps ? sp * 4 + s : steps - 1;
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int64_t tile = tile_of(w0 + i, w_tiles);
-      ws[i] = reinterpret_cast<const unsigned*>(a.ws + tile * s_bytes)[sp * 64 + lane];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int step = sp * 4 + (s < here ? s : here - 1);
-        w[s][i].q[0] = reinterpret_cast<const u32x4*>(a.w + tile * w_bytes)[step * 64 + lane];
-      }
-    }
+    for (int i = 0; i < RT; ++i)
+      w[s][i].q[0] = reinterpret_cast<const u32x4*>(a.w + tile_of(w0 + i, w_tiles) * w_bytes)[step * 64 + lane];
     if constexpr (SRC < 0) {
 #pragma unroll
-      for (int j = 0; j < CT; ++j) {
-        const int64_t tile = tile_of(x0 + j, x_tiles);
-        xs[j] = reinterpret_cast<const unsigned*>(a.xs + tile * s_bytes)[sp * 64 + lane];
+      for (int j = 0; j < CT; ++j)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const int step = sp * 4 + (s < here ? s : here - 1);
-          constexpr int parts = FMT == MX_E2M1 ? 1 : 2;
+        for (int h = 0; h < kParts; ++h)
+          x[s][j].q[h] = reinterpret_cast<const u32x4*>(a.x + tile_of(x0 + j, x_tiles) * x_bytes)[(step * kParts + h) * 64 + lane];
+    }
+  };
+  auto fetch_scales = [&](int sp) {
 #pragma unroll
-          for (int h = 0; h < parts; ++h)
-            x[s][j].q[h] = reinterpret_cast<const u32x4*>(a.x + tile * x_bytes)[(step * parts + h) * 64 + lane];
-        }
-      }
+    for (int i = 0; i < RT; ++i) ws_next[i] = reinterpret_cast<const unsigned*>(a.ws + tile_of(w0 + i, w_tiles) * s_bytes)[sp * 64 + lane];
+    if constexpr (SRC < 0) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+        xs_next[j] = reinterpret_cast<const unsigned*>(a.xs + tile_of(x0 + j, x_tiles) * s_bytes)[sp * 64 + lane];
+    }
+  };
+  if (wave < supers) {
+    fetch_scales(wave);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) fetch(wave, s);
+  }
+  for (int sp = wave; sp < supers; sp += waves) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) ws[i] = ws_next[i];
+    if constexpr (SRC < 0) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j) xs[j] = xs_next[j];
     } else {
       static_assert(SRC < 0 || CT == 1, "one column tile");
       xs[0] = 0;
@@ -186,13 +400,22 @@ __global__ __launch_bounds__(512) void mx_stream_kernel(const GemmArgs a) {
         }
       }
     }
-    mma_step<FMT, 0>(acc, w[0], ws, x[0], xs);
-    if (here > 1) mma_step<FMT, 1>(acc, w[1], ws, x[1], xs);
-    if (here > 2) mma_step<FMT, 2>(acc, w[2], ws, x[2], xs);
-    if (here > 3) mma_step<FMT, 3>(acc, w[3], ws, x[3], xs);
+    // a step's registers take the wave's next piece as soon as they are used
+    const int next = sp + waves;
+    const bool more = next < supers;
+    if (more) fetch_scales(next);
+    auto one = [&](auto at) {
+      constexpr int STEP = decltype(at)::value;
+      if (sp * 4 + STEP < steps) mma_step<FMT, STEP>(acc, w[STEP], ws, x[STEP], xs);
+      if (more) fetch(next, STEP);
+    };
+    one(std::integral_constant<int, 0>());
+    one(std::integral_constant<int, 1>());
+    one(std::integral_constant<int, 2>());
+    one(std::integral_constant<int, 3>());
   }
   auto put = [&](int i, int j, int l, f32x4 v) {
-    store4<TYPE>(a, (x0 + j) * 16 + (l & 15), (w0 + i) * 16 + (l >> 4) * 4, v);
+    store4(a, (x0 + j) * 16 + (l & 15), (w0 + i) * 16 + (l >> 4) * 4, v);
   };
   if (waves == 1) {
 #pragma unroll
@@ -215,81 +438,118 @@ __global__ __launch_bounds__(512) void mx_stream_kernel(const GemmArgs a) {
 
 // ---- many rows of X --------------------------------------------------------------------------------------------------
 
-// A workgroup of GN x GT waves has GN * WN row tiles of W and GT * WT of X: a step's codes go through shared memory, two
-// buffers, the next step's loads in flight during one step's products; scales come straight from memory, four steps at once.
-template <int FMT, int TYPE, int WN, int WT, int GN, int GT>
+// 1 KB (16 bytes a lane) or 256 bytes (4 a lane) from memory straight into shared memory at `place`, lane after lane.  The
+// compiler does not see these loads: dma_wait waits for them, and the barrier behind it for the other waves'.
+__device__ __forceinline__ void dma16(unsigned place, const uint8_t* base, unsigned offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(place), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void dma4(unsigned place, const uint8_t* base, unsigned offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(place), "v"(offset), "s"(base) : "memory");
+}
+// until at most N of this wave's loads are on their way, and its reads of shared memory are done
+template <int N>
+__device__ __forceinline__ void dma_wait() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+// Row tiles of W in a workgroup, column tiles of X, and the loads of a wave a step.
+template <int FMT, int WN, int WT, int GN, int GT>
+struct TileShape {
+  static constexpr int kParts = FMT == MX_E2M1 ? 1 : 2, kWaves = GN * GT;
+  static constexpr int kW = GN * WN, kX = GT * WT, kPieces = kW + kX * kParts;  // 1 KB each
+  static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves;
+  static constexpr int kScaleLoads = (kW + kX + 4 * kWaves - 1) / (4 * kWaves);  // of 256 bytes
+  static constexpr int kStage = kLoads * kWaves * 1024, kScales = kScaleLoads * 4 * kWaves * 256;
+};
+
+// A workgroup of GN x GT waves has GN * WN row tiles of W and GT * WT of X.  A step's codes lie in one of NS places in shared memory,
+// loaded NS - 1 steps ahead; the scales of the next four steps are loaded beside them, a quarter a step, into one of two places.
+template <int FMT, int WN, int WT, int GN, int GT, int NS>
 __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) {
-  constexpr int kParts = FMT == MX_E2M1 ? 1 : 2, kWaves = GN * GT;
-  constexpr int kW = GN * WN, kX = GT * WT * kParts, kPieces = kW + kX, kLoads = (kPieces + kWaves - 1) / kWaves;  // 1 KB each
-  __shared__ u32x4 buffer[2][kPieces * 64];
+  using S = TileShape<FMT, WN, WT, GN, GT>;
+  static_assert(NS >= 2 && NS <= 4, "scales are read before the next but one's loads");
+  extern __shared__ f32x4 shared[];
+  uint8_t* const lds = reinterpret_cast<uint8_t*>(shared);
+  uint8_t* const lds_scales = lds + NS * S::kStage;
+  const unsigned place0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave % GN, wt = wave / GN;
-  const int steps = static_cast<int>(mx_steps(a.k)), supers = static_cast<int>(mx_supers(a.k));
+  const int supers = static_cast<int>(mx_supers(a.k));
+  const int last = static_cast<int>(mx_steps(a.k)) - 1;
   const int64_t w_tiles = mx_tiles(a.n), x_tiles = mx_tiles(a.t);
-  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * kW, x0 = static_cast<int64_t>(blockIdx.y) * (GT * WT);
+  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * S::kW, x0 = static_cast<int64_t>(blockIdx.y) * S::kX;
   const int64_t w_bytes = mx_code_bytes(a.k, MX_E2M1), x_bytes = mx_code_bytes(a.k, FMT), s_bytes = mx_scale_bytes(a.k);
+  // a tile past the last one is read again as the last one, and not stored
   auto tile_of = [](int64_t tile, int64_t tiles) { return tile < tiles ? tile : tiles - 1; };
-  // this wave's pieces of a step: where they come from
-  const u32x4* from[kLoads];
-  int pace[kLoads];
+  const uint8_t *from[S::kLoads], *from_scales[4][S::kScaleLoads];
+  unsigned pace[S::kLoads];
 #pragma unroll
-  for (int l = 0; l < kLoads; ++l) {
-    const int p = wave + l * kWaves;
-    if (p < kW) {
-      from[l] = reinterpret_cast<const u32x4*>(a.w + tile_of(w0 + p, w_tiles) * w_bytes) + lane;
-      pace[l] = 64;
-    } else {
-      const int c = p < kPieces ? p - kW : 0;
-      from[l] = reinterpret_cast<const u32x4*>(a.x + tile_of(x0 + c / kParts, x_tiles) * x_bytes) + (c % kParts) * 64 + lane;
-      pace[l] = 64 * kParts;
+  for (int l = 0; l < S::kLoads; ++l) {
+    const int p = wave + l * S::kWaves;
+    if (p < S::kW) {
+      from[l] = a.w + tile_of(w0 + p, w_tiles) * w_bytes;
+      pace[l] = 1024;
+    } else {  // (past the last piece: the last one again)
+      const int c = p < S::kPieces ? p - S::kW : S::kX * S::kParts - 1;
+      from[l] = a.x + tile_of(x0 + c / S::kParts, x_tiles) * x_bytes + c % S::kParts * 1024;
+      pace[l] = 1024 * S::kParts;
     }
   }
-  const unsigned *ws_at[WN], *xs_at[WT];
 #pragma unroll
-  for (int i = 0; i < WN; ++i)
-    ws_at[i] = reinterpret_cast<const unsigned*>(a.ws + tile_of(w0 + wn * WN + i, w_tiles) * s_bytes) + lane;
+  for (int q = 0; q < 4; ++q)
 #pragma unroll
-  for (int j = 0; j < WT; ++j)
-    xs_at[j] = reinterpret_cast<const unsigned*>(a.xs + tile_of(x0 + wt * WT + j, x_tiles) * s_bytes) + lane;
+    for (int l = 0; l < S::kScaleLoads; ++l) {
+      const int p = (q * S::kScaleLoads + l) * S::kWaves + wave;
+      const int c = p < S::kW + S::kX ? p : S::kW + S::kX - 1;
+      from_scales[q][l] = c < S::kW ? a.ws + tile_of(w0 + c, w_tiles) * s_bytes : a.xs + tile_of(x0 + c - S::kW, x_tiles) * s_bytes;
+    }
+  // the loads of a step, and a quarter of the next piece's scales; steps and pieces past the end are the last one again
+  auto fetch_scales = [&](int q, int sp) {
+    const unsigned at = place0 + NS * S::kStage + (sp & 1) * S::kScales;
+    const int64_t offset = static_cast<int64_t>(sp < supers ? sp : supers - 1) * 256;
+#pragma unroll
+    for (int l = 0; l < S::kScaleLoads; ++l)
+      dma4(at + ((q * S::kScaleLoads + l) * S::kWaves + wave) * 256, from_scales[q][l] + offset, lane * 4);
+  };
+  auto fetch = [&](int step, int slot) {
+    const int64_t at = step < last ? step : last;
+#pragma unroll
+    for (int l = 0; l < S::kLoads; ++l)
+      dma16(place0 + slot * S::kStage + (wave + l * S::kWaves) * 1024, from[l] + at * pace[l], lane * 16);
+  };
   f32x4 acc[WN][WT];
 #pragma unroll
   for (int i = 0; i < WN; ++i)
 #pragma unroll
     for (int j = 0; j < WT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  u32x4 next[kLoads];
-  unsigned ws[WN], xs[WT], ws_next[WN], xs_next[WT];
-  auto fetch = [&](int step) {
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l)
-      if (kPieces % kWaves == 0 || wave + l * kWaves < kPieces) next[l] = from[l][static_cast<int64_t>(step) * pace[l]];
-  };
-  auto place = [&](int b) {
+  for (int q = 0; q < 4; ++q) fetch_scales(q, 0);
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l)
-      if (kPieces % kWaves == 0 || wave + l * kWaves < kPieces) buffer[b][(wave + l * kWaves) * 64 + lane] = next[l];
-  };
-  auto fetch_scales = [&](int sp) {
-#pragma unroll
-    for (int i = 0; i < WN; ++i) ws_next[i] = ws_at[i][sp * 64];
-#pragma unroll
-    for (int j = 0; j < WT; ++j) xs_next[j] = xs_at[j][sp * 64];
-  };
-  fetch(0);
-  fetch_scales(0);
-  place(0);
-  __syncthreads();
-  auto one = [&](auto step_in, int step) {
+  for (int s = 0; s < NS - 1; ++s) {
+    fetch(s, s);
+    fetch_scales(s, 1);
+  }
+  unsigned ws[WN], xs[WT];
+  int slot = 0;
+  auto one = [&](auto step_in, int sp) {
     constexpr int STEP = decltype(step_in)::value;
-    if (step >= steps) return;
-    if (step + 1 < steps) fetch(step + 1);
+    const int step = sp * 4 + STEP;
+    if (step > last) return;
+    dma_wait<(NS - 2) * (S::kLoads + S::kScaleLoads)>();
+    __builtin_amdgcn_s_barrier();
+    // every wave is done with the place of the step before
+    const int free_slot = slot == 0 ? NS - 1 : slot - 1;
+    constexpr int AHEAD = STEP + NS - 1;
+    fetch(step + NS - 1, free_slot);
+    fetch_scales(AHEAD & 3, sp + AHEAD / 4 + 1);
     if constexpr (STEP == 0) {
+      const unsigned* const held = reinterpret_cast<const unsigned*>(lds_scales + (sp & 1) * S::kScales) + lane;
 #pragma unroll
-      for (int i = 0; i < WN; ++i) ws[i] = ws_next[i];
+      for (int i = 0; i < WN; ++i) ws[i] = held[(wn * WN + i) * 64];
 #pragma unroll
-      for (int j = 0; j < WT; ++j) xs[j] = xs_next[j];
-      if (step + 4 < steps) fetch_scales(step / 4 + 1);
+      for (int j = 0; j < WT; ++j) xs[j] = held[(S::kW + wt * WT + j) * 64];
     }
-    const u32x4* const held = buffer[STEP & 1] + lane;
+    const u32x4* const held = reinterpret_cast<const u32x4*>(lds + slot * S::kStage) + lane;
     Operand<MX_E2M1> w[WN];
     Operand<FMT> x[WT];
 #pragma unroll
@@ -297,22 +557,22 @@ __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) 
 #pragma unroll
     for (int j = 0; j < WT; ++j)
 #pragma unroll
-      for (int h = 0; h < kParts; ++h) x[j].q[h] = held[(kW + (wt * WT + j) * kParts + h) * 64];
+      for (int h = 0; h < S::kParts; ++h) x[j].q[h] = held[(S::kW + (wt * WT + j) * S::kParts + h) * 64];
     mma_step<FMT, STEP>(acc, w, ws, x, xs);
-    if (step + 1 < steps) place((STEP + 1) & 1);
-    __syncthreads();
+    slot = slot == NS - 1 ? 0 : slot + 1;
   };
   for (int sp = 0; sp < supers; ++sp) {
-    one(std::integral_constant<int, 0>(), sp * 4);
-    one(std::integral_constant<int, 1>(), sp * 4 + 1);
-    one(std::integral_constant<int, 2>(), sp * 4 + 2);
-    one(std::integral_constant<int, 3>(), sp * 4 + 3);
+    one(std::integral_constant<int, 0>(), sp);
+    one(std::integral_constant<int, 1>(), sp);
+    one(std::integral_constant<int, 2>(), sp);
+    one(std::integral_constant<int, 3>(), sp);
   }
+  dma_wait<0>();  // no load is on its way into this workgroup's shared memory when it ends
 #pragma unroll
   for (int i = 0; i < WN; ++i)
 #pragma unroll
     for (int j = 0; j < WT; ++j)
-      store4<TYPE>(a, (x0 + wt * WT + j) * 16 + (lane & 15), (w0 + wn * WN + i) * 16 + (lane >> 4) * 4, acc[i][j]);
+      store4(a, (x0 + wt * WT + j) * 16 + (lane & 15), (w0 + wn * WN + i) * 16 + (lane >> 4) * 4, acc[i][j]);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------
@@ -327,44 +587,60 @@ hipError_t run(void (*kern)(GemmArgs), dim3 grid, int threads, size_t lds, hipSt
   return hipGetLastError();
 }
 
-template <int FMT, int SRC, int TYPE, int RT, int CT>
-hipError_t launch_stream(const GemmArgs& a, int waves, hipStream_t stream) {
+template <int FMT, int SRC, int RT, int CT, int WAVES>
+hipError_t launch_stream(const GemmArgs& a, hipStream_t stream) {
+  static std::atomic<unsigned> limit[kMaxDevices];
+  const int waves = static_cast<int>(mx_supers(a.k) < WAVES ? mx_supers(a.k) : WAVES);
   const dim3 grid(static_cast<unsigned>((mx_tiles(a.n) + RT - 1) / RT), static_cast<unsigned>((mx_tiles(a.t) + CT - 1) / CT));
-  return run(mx_stream_kernel<FMT, SRC, TYPE, RT, CT>, grid, waves * 64, waves > 1 ? waves * RT * CT * 1024 : 0, stream, a);
+  const size_t lds = waves > 1 ? waves * RT * CT * 1024 : 0;
+  const auto kern = mx_stream_kernel<FMT, SRC, RT, CT, WAVES>;
+  const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds, limit);
+  return e != hipSuccess ? e : run(kern, grid, waves * 64, lds, stream, a);
 }
 
-template <int FMT, int TYPE, int WN, int WT, int GN, int GT>
+template <int FMT, int WN, int WT, int GN, int GT, int NS>
 hipError_t launch_tile(const GemmArgs& a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((mx_tiles(a.n) + GN * WN - 1) / (GN * WN)),
-                  static_cast<unsigned>((mx_tiles(a.t) + GT * WT - 1) / (GT * WT)));
-  return run(mx_tile_kernel<FMT, TYPE, WN, WT, GN, GT>, grid, GN * GT * 64, 0, stream, a);
+  using S = TileShape<FMT, WN, WT, GN, GT>;
+  static std::atomic<unsigned> limit[kMaxDevices];
+  const dim3 grid(static_cast<unsigned>((mx_tiles(a.n) + S::kW - 1) / S::kW), static_cast<unsigned>((mx_tiles(a.t) + S::kX - 1) / S::kX));
+  const size_t lds = NS * S::kStage + 2 * S::kScales;
+  const auto kern = mx_tile_kernel<FMT, WN, WT, GN, GT, NS>;
+  const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds, limit);
+  return e != hipSuccess ? e : run(kern, grid, GN * GT * 64, lds, stream, a);
 }
 
-int stream_waves(int64_t k) {
-  const int64_t supers = mx_supers(k);
-  return static_cast<int>(supers < 8 ? supers : 8);
-}
-
-template <int FMT, int TYPE>
-hipError_t launch_rows(const MxGemmCall& c, const GemmArgs& a, hipStream_t stream) {
-  if (c.src != nullptr) {
-    const int waves = stream_waves(c.w.k);
-    if (c.src_type == MX_F32) return launch_stream<FMT, MX_F32, TYPE, 1, 1>(a, waves, stream);
-    if (c.src_type == MX_F16) return launch_stream<FMT, MX_F16, TYPE, 1, 1>(a, waves, stream);
-    return launch_stream<FMT, MX_BF16, TYPE, 1, 1>(a, waves, stream);
-  }
-  const int waves = stream_waves(c.w.k);
-  if (a.t <= 16) return launch_stream<FMT, -1, TYPE, 1, 1>(a, waves, stream);
-  if (a.t <= 32) return launch_stream<FMT, -1, TYPE, 1, 2>(a, waves, stream);
-  if (a.t <= 64) return launch_stream<FMT, -1, TYPE, 1, 4>(a, waves, stream);
-  return launch_tile<FMT, TYPE, 4, 4, 2, 2>(a, stream);
+template <int FMT, bool FLOATS, int P, int D>
+hipError_t launch_step(const GemmArgs& a, hipStream_t stream) {
+  static std::atomic<unsigned> limit[kMaxDevices];
+  const int waves = static_cast<int>((mx_supers(a.k) + P - 1) / P);
+  const int column = (FMT == MX_E2M1 ? 256 : 512) + 16;
+  const size_t place = FLOATS ? waves * (a.t * column + 256) : 0, join = waves > 1 ? 2 * waves * 1024 : 0;
+  const size_t lds = place > join ? place : join;
+  const int64_t tiles = mx_tiles(a.n), most = static_cast<int64_t>(device_cu_count()) * (waves <= 16 ? 16 / waves : 1);
+  const auto kern = mx_step_kernel<FMT, FLOATS, P, D>;
+  const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds, limit);
+  if (e != hipSuccess) return e;
+  return run(kern, dim3(static_cast<unsigned>(tiles < most ? tiles : most)), waves * 64, lds, stream, a);
 }
 
 template <int FMT>
 hipError_t launch_format(const MxGemmCall& c, const GemmArgs& a, hipStream_t stream) {
-  if (c.type == MX_F32) return launch_rows<FMT, MX_F32>(c, a, stream);
-  if (c.type == MX_F16) return launch_rows<FMT, MX_F16>(c, a, stream);
-  return launch_rows<FMT, MX_BF16>(c, a, stream);
+  const bool floats = c.src != nullptr;
+  if (a.t <= 16) {
+    if (mx_supers(a.k) <= 16) return floats ? launch_step<FMT, true, 1, 2>(a, stream) : launch_step<FMT, false, 1, 2>(a, stream);
+    if (mx_supers(a.k) <= 32) return floats ? launch_step<FMT, true, 4, 2>(a, stream) : launch_step<FMT, false, 4, 2>(a, stream);
+    if (!floats) return launch_stream<FMT, -1, 1, 1, 8>(a, stream);
+    if (c.src_type == MX_F32) return launch_stream<FMT, MX_F32, 1, 1, 8>(a, stream);
+    if (c.src_type == MX_F16) return launch_stream<FMT, MX_F16, 1, 1, 8>(a, stream);
+    return launch_stream<FMT, MX_BF16, 1, 1, 8>(a, stream);
+  }
+  const int64_t cus = device_cu_count(), n16 = mx_tiles(a.n), t16 = mx_tiles(a.t);
+  auto groups = [&](int64_t rows, int64_t cols) { return ((n16 + rows - 1) / rows) * ((t16 + cols - 1) / cols); };
+  if (groups(16, 16) >= 2 * cus) return launch_tile<FMT, 8, 4, 2, 4, 3>(a, stream);
+  if (8 * groups(8, 8) >= 5 * cus) return launch_tile<FMT, 4, 4, 2, 2, 3>(a, stream);
+  if (groups(4, 2) >= cus) return launch_stream<FMT, -1, 4, 2, 8>(a, stream);
+  if (groups(2, 2) >= cus) return launch_stream<FMT, -1, 2, 2, 8>(a, stream);
+  return launch_stream<FMT, -1, 1, 2, 8>(a, stream);
 }
 
 }  // namespace
@@ -381,6 +657,8 @@ hipError_t launch_mx_gemm(const MxGemmCall& c, hipStream_t stream) {
   a.k = static_cast<int>(c.w.k);
   a.y = c.y;
   a.y_stride = c.stride;
+  a.type = c.type;
+  a.x_type = c.src_type;
   return c.x.fmt == MX_E2M1 ? launch_format<MX_E2M1>(c, a, stream) : launch_format<MX_E4M3>(c, a, stream);
 }
 

@@ -271,12 +271,16 @@ def _need_weights(w, k, device):
         raise _BAD(f"w must be e2m1 rows of {k} elements on cuda:{device}, got {w.fmt} rows of {w.k} on {w.device}")
 
 
+def _gemm(x, w, y, stride):
+    _launch("komp_mx_gemm", w._device, x._ref, w._ref, y.data_ptr(), TYPES[y.dtype], stride)
+
+
 def gemm_into(x, w, y):
     """gemm() into y [T][N] (f32, f16 or bf16; rows contiguous, any stride between them that keeps them apart)."""
     _need_rows(x, "x")
     _need_weights(w, x.k, x._device)
     _need_matrix(y, "y", w.rows, x._device, x.rows, output=True)
-    _launch("komp_mx_gemm", x._device, x._ref, w._ref, y.data_ptr(), TYPES[y.dtype], y.stride(0))
+    _gemm(x, w, y, y.stride(0))
 
 
 def gemm(x, w, dtype=torch.float32):
@@ -284,9 +288,9 @@ def gemm(x, w, dtype=torch.float32):
     elements stand for, in f32, rounded once."""
     _need_rows(x, "x")
     _need_weights(w, x.k, x._device)
-    number = _type(dtype)
+    _type(dtype)
     y = w.codes.new_empty((x.rows, w.rows), dtype=dtype)
-    _launch("komp_mx_gemm", x._device, x._ref, w._ref, y.data_ptr(), number, w.rows)
+    _gemm(x, w, y, w.rows)
     return y
 
 
@@ -295,7 +299,7 @@ def _linear(x, w, y, fmt):
     if t > LINEAR_ROWS:
         rows = _empty(w.codes, t, w.k, fmt)  # kept until the calls are on the stream; torch hands it to later work of this stream
         _quantize(x, rows, 0)
-        _launch("komp_mx_gemm", w._device, rows._ref, w._ref, y.data_ptr(), TYPES[y.dtype], y.stride(0))
+        _gemm(rows, w, y, y.stride(0))
     else:
         _launch("komp_mx_linear", w._device, x.data_ptr(), TYPES[x.dtype], x.stride(0), t, FORMATS[fmt], w._ref, y.data_ptr(),
                 TYPES[y.dtype], y.stride(0))  # fmt: skip

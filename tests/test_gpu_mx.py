@@ -194,7 +194,8 @@ def test_lookup(fmt, dtype):
 # ---- products --------------------------------------------------------------------------------------------------------
 
 PRODUCTS = [(1, 1, 32), (1, 16, 128), (2, 17, 96), (3, 100, 160), (16, 33, 512), (17, 48, 544), (31, 5, 1056), (33, 64, 2560),
-            (64, 200, 640), (65, 130, 1024), (100, 257, 96), (130, 300, 1312), (257, 129, 4096), (5, 700, 14336)]  # fmt: skip
+            (64, 200, 640), (65, 130, 1024), (100, 257, 96), (130, 300, 1312), (257, 129, 4096), (5, 700, 14336), (3, 40, 20000), (40, 33, 20000), (300, 1100, 1024),
+            (1100, 300, 320)]  # fmt: skip
 
 
 def check_product(y, x, w, fmt, dtype):
@@ -283,7 +284,7 @@ def test_gemm_far_scales(fmt, t):
     check_product(mx.gemm(x, w), xv, wv, fmt, "f32")
 
 
-@pytest.mark.parametrize("shape", [(1, 1, 32), (1, 700, 2560), (2, 33, 544), (7, 64, 4096), (16, 50, 96), (5, 17, 14336), (17, 40, 160),
+@pytest.mark.parametrize("shape", [(1, 1, 32), (1, 700, 2560), (2, 33, 544), (7, 64, 4096), (16, 50, 96), (5, 17, 14336), (17, 40, 160), (3, 40, 20000), (16, 300, 8192),
                                    (70, 300, 1024)], ids=str)  # fmt: skip
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fmt", mx.FORMATS)
