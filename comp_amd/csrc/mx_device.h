@@ -96,24 +96,30 @@ __device__ __forceinline__ void mx_codes8(const float* v, unsigned s, unsigned (
   }
 }
 
-// What eight elements stand for, in f32 (exact).
-template <int FMT>
-__device__ __forceinline__ void mx_values8(const unsigned (&q)[FMT == MX_E2M1 ? 1 : 2], unsigned s, float (&v)[8]) {
-  const float scale = __uint_as_float(s << 23);
-  f32x2 p[4];
+// What four or eight elements in shared memory stand for, in f32 (exact).
+template <int FMT, int N>
+__device__ __forceinline__ void mx_values(const uint8_t* from, float scale, float (&v)[N]) {
+  f32x2 p[N / 2];
   if constexpr (FMT == MX_E2M1) {
-    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[0], scale, 0);
-    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[0], scale, 1);
-    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[0], scale, 2);
-    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[0], scale, 3);
+    const unsigned q = N == 8 ? *reinterpret_cast<const unsigned*>(from) : *reinterpret_cast<const uint16_t*>(from);
+    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 0);
+    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 1);
+    if constexpr (N == 8) {
+      p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 2);
+      p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 3);
+    }
   } else {
-    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[0], scale, false);
-    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[0], scale, true);
-    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[1], scale, false);
-    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[1], scale, true);
+    const unsigned q = reinterpret_cast<const unsigned*>(from)[0];
+    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q, scale, false);
+    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q, scale, true);
+    if constexpr (N == 8) {
+      const unsigned r = reinterpret_cast<const unsigned*>(from)[1];
+      p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(r, scale, false);
+      p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(r, scale, true);
+    }
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = p[e / 2][e % 2];
+  for (int e = 0; e < N; ++e) v[e] = p[e / 2][e % 2];
 }
 
 }  // namespace komp

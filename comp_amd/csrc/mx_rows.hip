@@ -17,14 +17,66 @@ constexpr int kThreads = 256;
 // workgroups of a launch at most (a grid holds 2^32 threads); they walk over more tiles than that
 constexpr unsigned kGrid = 1u << 22;
 
-// The product whose rounding to f32 is quantized, from 64 bits: an f32 exp would be off by enough to move values over an
-// element's border.
+// The product whose rounding to f32 is quantized, from 64 bits.
 template <int ACT>
 __device__ __forceinline__ float mx_act(float g, float u) {
   const double a = g, b = u;
   if constexpr (ACT == MX_SILU) return static_cast<float>(a / (1.0 + exp(-a)) * b);
   const double p = a > 0.0 ? a : a != a ? a : 0.0;
   return static_cast<float>(p * p * b);
+}
+
+// The same in f32, within 2^-20 of it for products from 2^-126 on: e^-g is 2^t with t = -g log2(e) in two parts, so that t's
+// rounding (up to 2^-18) does not count; the exponential and the reciprocal are off by one step each.  `far`: gates for which a
+// step in between leaves f32's range.
+template <int ACT>
+__device__ __forceinline__ float mx_act_near(float g, float u, bool& far) {
+  if constexpr (ACT == MX_SILU) {
+    far |= !(g >= -80.f) || (__builtin_fabsf(g) < 0x1p-100f && g != 0.f);
+    const float t = g * -1.44269502f, rest = __builtin_fmaf(g, -1.44269502f, -t) + g * -1.92596303e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return g * __builtin_amdgcn_rcpf(1.f + __builtin_fmaf(e, rest * 0.693147182f, e)) * u;
+  } else {
+    far |= g != g || (g > 0.f && g < 0x1p-50f);
+    const float p = g > 0.f ? g : 0.f;
+    return p * p * u;
+  }
+}
+
+// the largest of a quad of lanes
+__device__ __forceinline__ unsigned most4(unsigned most) {
+  most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR1>(static_cast<int>(most))));
+  return umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR2>(static_cast<int>(most))));
+}
+
+// A quad of lanes' block of gated products: scale and codes.  They come from f32 products where all that these may stand for, 2^-19 to
+// either side, give the same ones (scale and rounding are monotonous), and from 64 bits otherwise: with e4m3 one block in a thousand
+// (2^-15 an element).  Blocks of tiny products, and gates out of f32's range, take 64 bits too.
+template <int FMT, int ACT>
+__device__ __forceinline__ void gate8(const float (&g)[8], const float (&u)[8], unsigned& s, unsigned (&c)[FMT == MX_E2M1 ? 1 : 2]) {
+  float low[8], high[8];
+  bool far = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = mx_act_near<ACT>(g[e], u[e], far);
+    low[e] = v - v * 0x1p-19f;
+    high[e] = v + v * 0x1p-19f;
+  }
+  const unsigned most = most4(mx_most(high));
+  s = mx_scale<FMT>(most4(mx_most(low)));
+  far |= s != mx_scale<FMT>(most) || most < (27u << 23) || most >= (255u << 23);  // 2^-100
+  unsigned d[FMT == MX_E2M1 ? 1 : 2];
+  mx_codes8<FMT>(low, s, c);
+  mx_codes8<FMT>(high, s, d);
+#pragma unroll
+  for (int h = 0; h < (FMT == MX_E2M1 ? 1 : 2); ++h) far |= c[h] != d[h];
+  if (most4(far) != 0) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = mx_act<ACT>(g[e], u[e]);
+    s = mx_scale<FMT>(most4(mx_most(v)));
+    mx_codes8<FMT>(v, s, c);
+  }
 }
 
 struct QuantArgs {
@@ -43,38 +95,36 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const QuantArgs a
   for (unsigned tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const int64_t rt = tile / supers, piece = tile % supers;
     const int64_t step = piece * 4 + wave, r = rt * 16 + row;
-    float v[4][8];
+    float v[4][8], u[ACT == MX_PLAIN ? 1 : 4][8];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int64_t b = step * 4 + g;
       if (b < blocks && r < a.r.rows) {
         mx_load<TYPE>(a.x, r * a.stride + b * 32 + q * 8, v[g]);
-        if constexpr (ACT != MX_PLAIN) {
-          float u[8];
-          mx_load<TYPE>(a.x, r * a.stride + a.r.k + b * 32 + q * 8, u);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[g][e] = mx_act<ACT>(v[g][e], u[e]);
-        }
+        if constexpr (ACT != MX_PLAIN) mx_load<TYPE>(a.x, r * a.stride + a.r.k + b * 32 + q * 8, u[g]);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[g][e] = 0.f;
+        if constexpr (ACT != MX_PLAIN) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[g][e] = 0.f;
+        }
       }
     }
     uint8_t* const codes = a.r.codes + rt * mx_code_bytes(a.r.k, FMT);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      unsigned most = mx_most(v[g]);
-      most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR1>(static_cast<int>(most))));
-      most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR2>(static_cast<int>(most))));
-      const unsigned s = mx_scale<FMT>(most);
+      unsigned s, c[FMT == MX_E2M1 ? 1 : 2];
+      if constexpr (ACT == MX_PLAIN) {
+        s = mx_scale<FMT>(most4(mx_most(v[g])));
+        mx_codes8<FMT>(v[g], s, c);
+      } else {
+        gate8<FMT, ACT>(v[g], u[g], s, c);
+      }
       if (step < steps) {
         if constexpr (FMT == MX_E2M1) {
-          unsigned c[1];
-          mx_codes8<FMT>(v[g], s, c);
           *reinterpret_cast<unsigned*>(codes + step * 1024 + (g * 16 + row) * 16 + q * 4) = c[0];
         } else {
-          unsigned c[2];
-          mx_codes8<FMT>(v[g], s, c);
           *reinterpret_cast<u32x2*>(codes + step * 2048 + (q >> 1) * 1024 + (g * 16 + row) * 16 + (q & 1) * 8) = u32x2{c[0], c[1]};
         }
       }
@@ -97,52 +147,63 @@ struct LookupArgs {
   unsigned tiles;
 };
 
+// A workgroup has 16 of the rows asked for and 512 elements of each, a wave four rows: a lane loads one block, 16 or 32 bytes
+// from anywhere, and through shared memory the wave turns them into whole rows, 1 KB a store.
 template <int FMT, int TYPE>
 __global__ __launch_bounds__(kThreads) void mx_lookup_kernel(const LookupArgs a) {
-  const int wave = threadIdx.x >> 6, row = (threadIdx.x & 63) >> 2, q = threadIdx.x & 3;
+  constexpr int kParts = FMT == MX_E2M1 ? 1 : 2;
+  constexpr int kE = TYPE == MX_F32 ? 4 : 8;  // elements a store
+  constexpr unsigned kMissing = 1u << 31;     // in a scale's place: no such row
+  __shared__ u32x4 codes_of[kThreads / 64][64 * kParts];
+  __shared__ unsigned scales_of[kThreads / 64][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, block = lane & 15;
   const int64_t blocks = a.r.k >> 5;
   const unsigned supers = static_cast<unsigned>(mx_supers(a.r.k));
   for (unsigned tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const int64_t t16 = tile / supers, piece = tile % supers;
-    const int64_t step = piece * 4 + wave, t = t16 * 16 + row;
-    if (t >= a.count) continue;
-    const int64_t id = a.ids == nullptr ? t : a.ids[t];
-    const bool in = id >= 0 && id < a.r.rows;
-    const int64_t rt = in ? id >> 4 : 0;
-    const int lane = in ? static_cast<int>(id & 15) : 0;
-    const uint8_t* const codes = a.r.codes + rt * mx_code_bytes(a.r.k, FMT);
-    const uint8_t* const scales = a.r.scales + rt * mx_scale_bytes(a.r.k) + piece * 256;
-    unsigned c[4][FMT == MX_E2M1 ? 1 : 2], s[4];
+    const int64_t t0 = static_cast<int64_t>(tile / supers) * 16 + wave * 4, piece = tile % supers;
+    const int64_t t = t0 + (lane >> 4);
+    int64_t id = -1;
+    if (t < a.count) id = a.ids == nullptr ? t : a.ids[t];
+    const bool there = id >= 0 && id < a.r.rows;
+    u32x4 c[kParts];
+    unsigned s = 0;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      c[g][0] = 0;
-      if constexpr (FMT == MX_E4M3) c[g][1] = 0;
-      s[g] = 0;
-      if (in && step * 4 + g < blocks) {
-        s[g] = scales[(g * 16 + lane) * 4 + wave];
-        if constexpr (FMT == MX_E2M1) {
-          c[g][0] = *reinterpret_cast<const unsigned*>(codes + step * 1024 + (g * 16 + lane) * 16 + q * 4);
-        } else {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(codes + step * 2048 + (q >> 1) * 1024 + (g * 16 + lane) * 16 + (q & 1) * 8);
-          c[g][0] = w[0];
-          c[g][1] = w[1];
+    for (int h = 0; h < kParts; ++h) c[h] = u32x4{0, 0, 0, 0};
+    if (there && piece * 16 + block < blocks) {
+      const int at = (block & 3) * 16 + static_cast<int>(id & 15);
+      const u32x4* const from =
+          reinterpret_cast<const u32x4*>(a.r.codes + (id >> 4) * mx_code_bytes(a.r.k, FMT)) + (piece * 4 + (block >> 2)) * 64 * kParts + at;
+#pragma unroll
+      for (int h = 0; h < kParts; ++h) c[h] = from[h * 64];
+      s = (a.r.scales + (id >> 4) * mx_scale_bytes(a.r.k) + piece * 256)[at * 4 + (block >> 2)];
+    }
+    // (a wave's own places: its reads of the turn before are done, in order)
+#pragma unroll
+    for (int h = 0; h < kParts; ++h) codes_of[wave][lane * kParts + h] = c[h];
+    scales_of[wave][lane] = there ? s << 23 : kMissing;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int p = 0; p < 8 / kE; ++p) {
+        const int e = p * 256 + lane * kE;  // of the piece's 512 elements
+        if (t0 + r >= a.count || (piece * 16 + (e >> 5)) >= blocks) continue;
+        const unsigned scale = scales_of[wave][r * 16 + (e >> 5)];
+        const uint8_t* const from = reinterpret_cast<const uint8_t*>(&codes_of[wave][r * 16 * kParts]) + (FMT == MX_E2M1 ? e / 2 : e);
+        float v[kE];
+        mx_values<FMT, kE>(from, __uint_as_float(scale), v);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          v[i] = scale == kMissing ? 0.f : v[i] * a.factor;
+          // the compiler makes v_fma_mixlo_f16 with an addend of +0 of a product and its rounding to f16, which loses -0
+          if constexpr (TYPE == MX_F16) asm("" : "+v"(v[i]));
         }
+        mx_store<TYPE>(a.out, (t0 + r) * a.stride + piece * 512 + e, v);
       }
     }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int64_t b = step * 4 + g;
-      if (b >= blocks) continue;
-      float v[8];
-      mx_values8<FMT>(c[g], s[g], v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = in ? v[e] * a.factor : 0.f;
-        // the compiler makes v_fma_mixlo_f16 with an addend of +0 of a product and its rounding to f16, which loses -0
-        if constexpr (TYPE == MX_F16) asm("" : "+v"(v[e]));
-      }
-      mx_store<TYPE>(a.out, t * a.stride + b * 32 + q * 8, v);
-    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 

@@ -21,6 +21,7 @@ No reference counterpart.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -34,6 +35,7 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTS = {"silu": 1, "relu2": 2}
 LINEAR_ROWS = 16  # rows that linear() quantizes and multiplies in one launch
 _BAD = _abi.KompArgumentError
+_new = object.__new__
 
 
 class Rows:
@@ -45,22 +47,32 @@ class Rows:
     def __init__(self, rows, k, fmt="e2m1", device="cuda"):
         if torch.device(device).type != "cuda":
             raise _BAD(f"Rows: {device}: the rows live on a HIP device")
-        codes, scales = _plane_sizes(rows, k, fmt)
-        self._hold(rows, k, fmt, torch.zeros(codes, dtype=_U8, device=device), torch.zeros(scales, dtype=_U8, device=device))
+        sizes = _plane_sizes(rows, k, fmt)
+        self._hold(rows, k, fmt, sizes, torch.zeros(sizes[2], dtype=_U8, device=device))
 
-    def _hold(self, rows, k, fmt, codes, scales):
-        self.rows, self.k, self.fmt, self.codes, self.scales = rows, k, fmt, codes, scales
-        self._struct = _abi.MxRowsStruct(codes.data_ptr(), scales.data_ptr(), rows, k, FORMATS[fmt])
+    def _hold(self, rows, k, fmt, sizes, planes):
+        # (one allocation for both planes: an eager call is mostly host time)
+        self.rows, self.k, self.fmt = rows, k, fmt
+        self._planes, self._sizes, self._device = planes, sizes, planes.get_device()
+        at = planes.data_ptr()
+        self._struct = _abi.MxRowsStruct(at, at + sizes[0], rows, k, FORMATS[fmt])
         self._ref = ctypes.addressof(self._struct)
-        self._device = codes.get_device()
+
+    @property
+    def codes(self):
+        return self._planes[: self._sizes[0]].view(-(-self.rows // 16), -1) if self.rows else self._planes.view(0, 0)
+
+    @property
+    def scales(self):
+        return self._planes[self._sizes[0] :].view(-(-self.rows // 16), -1) if self.rows else self._planes.view(0, 0)
 
     @property
     def device(self):
-        return self.codes.device
+        return self._planes.device
 
     def nbytes(self):
         """Bytes of the two planes."""
-        return self.codes.numel() + self.scales.numel()
+        return self._sizes[2]
 
 
 def _need_format(fmt):
@@ -68,21 +80,24 @@ def _need_format(fmt):
         raise _BAD(f"fmt={fmt!r}: one of {tuple(FORMATS)}")
 
 
+@functools.lru_cache(maxsize=4096)
 def _plane_sizes(rows, k, fmt):
+    """(bytes of the codes, of the scales, of both)."""
     _need_format(fmt)
     if k < 32 or k % 32 or k > 1 << 26:
         raise _BAD(f"k={k} must be a multiple of 32, from 32 to 2^26")
     tiles, pieces = -(-rows // 16), -(-k // 512)
     if rows < 0 or rows > 0x7FFFFFFF or tiles * pieces > 0x7FFFFFFF:
         raise _BAD(f"{rows} rows of {k} elements")
-    return (tiles, -(-k // 128) * (1024 << FORMATS[fmt])), (tiles, pieces * 256)
+    codes, scales = tiles * -(-k // 128) * (1024 << FORMATS[fmt]), tiles * pieces * 256
+    return codes, scales, codes + scales
 
 
 def _empty(like, rows, k, fmt):
     """Rows that the next launch writes, places behind the last row and block too."""
-    codes, scales = _plane_sizes(rows, k, fmt)
-    r = Rows.__new__(Rows)
-    r._hold(rows, k, fmt, like.new_empty(codes, dtype=_U8), like.new_empty(scales, dtype=_U8))
+    sizes = _plane_sizes(rows, k, fmt)
+    r = _new(Rows)
+    r._hold(rows, k, fmt, sizes, like.new_empty(sizes[2], dtype=_U8))
     return r
 
 
@@ -214,7 +229,7 @@ def lookup(rows, ids, dtype=torch.float32, scale=1.0):
     _need_rows(rows, "rows")
     _need_ids(ids, rows)
     number = _type(dtype)
-    out = rows.codes.new_empty((ids.shape[0], rows.k), dtype=dtype)
+    out = rows._planes.new_empty((ids.shape[0], rows.k), dtype=dtype)
     _launch("komp_mx_lookup", rows._device, rows._ref, ids.data_ptr(), ids.shape[0], out.data_ptr(), number, rows.k, scale)
     return out
 
@@ -223,7 +238,7 @@ def values(rows, dtype=torch.float32):
     """All rows as values [rows][K] of dtype (bf16 holds every value of magnitude 2^-126 and more exactly, f32 all)."""
     _need_rows(rows, "rows")
     number = _type(dtype)
-    out = rows.codes.new_empty((rows.rows, rows.k), dtype=dtype)
+    out = rows._planes.new_empty((rows.rows, rows.k), dtype=dtype)
     _launch("komp_mx_lookup", rows._device, rows._ref, None, rows.rows, out.data_ptr(), number, rows.k, 1.0)
     return out
 
@@ -244,8 +259,8 @@ def pack(codes, scales, fmt="e2m1"):
 def unpack(rows):
     """Rows -> (codes, scales), the plain planes that pack() takes."""
     _need_rows(rows, "rows")
-    codes = rows.codes.new_empty((rows.rows, rows.k // 2 if rows.fmt == "e2m1" else rows.k))
-    scales = rows.codes.new_empty((rows.rows, rows.k // 32))
+    codes = rows._planes.new_empty((rows.rows, rows.k // 2 if rows.fmt == "e2m1" else rows.k))
+    scales = rows._planes.new_empty((rows.rows, rows.k // 32))
     _launch("komp_mx_unpack", rows._device, rows._ref, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
@@ -289,7 +304,7 @@ def gemm(x, w, dtype=torch.float32):
     _need_rows(x, "x")
     _need_weights(w, x.k, x._device)
     _type(dtype)
-    y = w.codes.new_empty((x.rows, w.rows), dtype=dtype)
+    y = w._planes.new_empty((x.rows, w.rows), dtype=dtype)
     _gemm(x, w, y, w.rows)
     return y
 
@@ -297,7 +312,7 @@ def gemm(x, w, dtype=torch.float32):
 def _linear(x, w, y, fmt):
     t = x.shape[0]
     if t > LINEAR_ROWS:
-        rows = _empty(w.codes, t, w.k, fmt)  # kept until the calls are on the stream; torch hands it to later work of this stream
+        rows = _empty(w._planes, t, w.k, fmt)  # kept until the calls are on the stream; torch hands it to later work of this stream
         _quantize(x, rows, 0)
         _gemm(rows, w, y, y.stride(0))
     else:
@@ -326,6 +341,6 @@ def linear(x, w, fmt="e4m3", dtype=None):
     _need_matrix(x, "x", w.k, w._device)
     dtype = x.dtype if dtype is None else dtype
     _type(dtype)
-    y = w.codes.new_empty((x.shape[0], w.rows), dtype=dtype)
+    y = w._planes.new_empty((x.shape[0], w.rows), dtype=dtype)
     _linear(x, w, y, fmt)
     return y

@@ -189,6 +189,16 @@ def test_lookup(fmt, dtype):
             same(f64(guard[:, 3 : 3 + k]), v)
             assert bool((guard[:, :3] == 7).all()) and bool((guard[:, 3 + k :] == 7).all())
     assert mx.lookup(rows, torch.empty(0, dtype=torch.int64, device="cuda")).shape == (0, k)
+    assert mx.lookup(rows, torch.tensor([-1], device="cuda"), DTYPES[dtype], scale=float("inf")).abs().max() == 0
+
+
+@pytest.mark.parametrize("act", mx.ACTS)
+@pytest.mark.parametrize("fmt", mx.FORMATS)
+def test_gate_many(fmt, act):
+    """A million products of one block's magnitudes: the blocks whose elements lie next to a border take the 64-bit path."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((512, 2 * 2048), generator=g, device="cuda") * torch.exp2(torch.randint(-8, 9, (512, 1), generator=g, device="cuda"))
+    same(f64(mx.values(mx.gate(x, fmt, act))), R.kept(R.gate(f64(x), act), fmt))
 
 
 # ---- products --------------------------------------------------------------------------------------------------------
