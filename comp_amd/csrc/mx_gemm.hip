@@ -114,23 +114,6 @@ __device__ __forceinline__ void store4(const GemmArgs& a, int64_t t, int64_t n, 
   else store4_as<MX_BF16>(a, t, n, v);
 }
 
-// Eight elements each of the first `count` of N rows that are quantized on the way, zeros of the others.
-template <int TYPE, int N>
-__device__ __forceinline__ void load_rows_as(const GemmArgs& a, int count, int64_t at, float (&v)[N][8]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-    if (i < count) mx_load<TYPE>(a.x, at + i * a.x_stride, v[i]);
-  }
-}
-template <int N>
-__device__ __forceinline__ void load_rows(const GemmArgs& a, int count, int64_t at, float (&v)[N][8]) {
-  if (a.x_type == MX_F32) load_rows_as<MX_F32>(a, count, at, v);
-  else if (a.x_type == MX_F16) load_rows_as<MX_F16>(a, count, at, v);
-  else load_rows_as<MX_BF16>(a, count, at, v);
-}
-
 // ---- one column tile of X --------------------------------------------------------------------------------------------
 
 // X's operands of a four-step piece, ready for mma_piece: as they are (e2m1; e4m3 in eight registers a step), or in bf16.
@@ -177,11 +160,49 @@ __device__ __forceinline__ void mma_piece(f32x4& acc, const PieceW& w, const Pie
   acc = out[0][0];
 }
 
+// A wave's piece of the rows of X into shared memory: codes by rows, scales as the operands' dwords.  As many rows' loads are on their
+// way together as the registers beside W's hold.
+template <int FMT, int TYPE, int P>
+__device__ __forceinline__ void quantize_rows(const GemmArgs& a, int sp, bool in, int lane, uint8_t* codes, uint8_t* scales, int column) {
+  constexpr int kAtOnce = P > 1 ? 2 : TYPE == MX_F32 || FMT == MX_E4M3 ? 4 : 8;
+  typedef typename MxElement<TYPE>::type T;
+  typedef T vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  const int count = static_cast<int>(a.t);
+  const T* const from = reinterpret_cast<const T*>(a.x) + sp * 512 + lane * 8;
+  for (int t0 = 0; t0 < count; t0 += kAtOnce) {
+    vec raw[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) raw[i][e] = static_cast<T>(0.f);
+      if (in && t0 + i < count) raw[i] = *reinterpret_cast<const vec*>(from + (t0 + i) * a.x_stride);
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int t = t0 + i;
+      if (t >= count) break;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(raw[i][e]);
+      unsigned most = mx_most(v);
+      most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR1>(static_cast<int>(most))));
+      most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR2>(static_cast<int>(most))));
+      const unsigned scale = mx_scale<FMT>(most);
+      unsigned c[FMT == MX_E2M1 ? 1 : 2];
+      mx_codes8<FMT>(v, scale, c);
+      if constexpr (FMT == MX_E2M1) *reinterpret_cast<unsigned*>(codes + t * column + lane * 4) = c[0];
+      else *reinterpret_cast<u32x2*>(codes + t * column + lane * 8) = u32x2{c[0], c[1]};
+      // block 4 s + g of the piece: byte s of group g's dword
+      if ((lane & 3) == 0) scales[(((lane >> 2) & 3) * 16 + t) * 4 + (lane >> 4)] = static_cast<uint8_t>(scale);
+    }
+  }
+}
+
 // Up to 16 rows of X.  A workgroup keeps X in registers, each wave P pieces of K, and walks over row tiles of W, whose codes
 // it loads D pieces ahead; its waves join in shared memory, in their order.  FLOATS: the rows are quantized on the way, by each
 // wave its own pieces, eight elements a lane, through shared memory into the operands' order.
 template <int FMT, bool FLOATS, int P, int D>
-__global__ __launch_bounds__(P == 1 ? 1024 : 512) void mx_step_kernel(const GemmArgs a) {
+__global__ __launch_bounds__(P <= 2 ? 1024 : 512) void mx_step_kernel(const GemmArgs a) {
   constexpr bool kWide = P == 1;
   constexpr int kTiles = D > P ? D / P : 1;                   // row tiles a turn of the loop
   constexpr int kColumn = (FMT == MX_E2M1 ? 256 : 512) + 16;  // bytes of a column's piece, apart in the banks
@@ -214,28 +235,10 @@ __global__ __launch_bounds__(P == 1 ? 1024 : 512) void mx_step_kernel(const Gemm
       if constexpr (FLOATS) {
         uint8_t* const mine = reinterpret_cast<uint8_t*>(shared) + wave * (static_cast<int>(a.t) * kColumn + 256);
         uint8_t* const mine_scales = mine + a.t * kColumn;
-        constexpr int kAtOnce = P == 1 ? 4 : 2;  // rows whose loads are on their way together
-        const int count = static_cast<int>(a.t);
         const bool in = (sp * 16 + (lane >> 2)) * 32 < a.k;
-        for (int t0 = 0; t0 < count; t0 += kAtOnce) {
-          float v[kAtOnce][8];
-          load_rows<kAtOnce>(a, in ? count - t0 : 0, t0 * a.x_stride + sp * 512 + lane * 8, v);
-#pragma unroll
-          for (int i = 0; i < kAtOnce; ++i) {
-            const int t = t0 + i;
-            if (t >= count) break;
-            unsigned most = mx_most(v[i]);
-            most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR1>(static_cast<int>(most))));
-            most = umax(most, static_cast<unsigned>(dpp_i<KOMP_DPP_XOR2>(static_cast<int>(most))));
-            const unsigned scale = mx_scale<FMT>(most);
-            unsigned c[FMT == MX_E2M1 ? 1 : 2];
-            mx_codes8<FMT>(v[i], scale, c);
-            if constexpr (FMT == MX_E2M1) *reinterpret_cast<unsigned*>(mine + t * kColumn + lane * 4) = c[0];
-            else *reinterpret_cast<u32x2*>(mine + t * kColumn + lane * 8) = u32x2{c[0], c[1]};
-            // block 4 s + g of the piece: byte s of group g's dword
-            if ((lane & 3) == 0) mine_scales[(((lane >> 2) & 3) * 16 + t) * 4 + (lane >> 4)] = static_cast<uint8_t>(scale);
-          }
-        }
+        if (a.x_type == MX_F32) quantize_rows<FMT, MX_F32, P>(a, sp, in, lane, mine, mine_scales, kColumn);
+        else if (a.x_type == MX_F16) quantize_rows<FMT, MX_F16, P>(a, sp, in, lane, mine, mine_scales, kColumn);
+        else quantize_rows<FMT, MX_BF16, P>(a, sp, in, lane, mine, mine_scales, kColumn);
         // lanes read what others of their wave wrote
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -616,7 +619,7 @@ hipError_t launch_step(const GemmArgs& a, hipStream_t stream) {
   const int column = (FMT == MX_E2M1 ? 256 : 512) + 16;
   const size_t place = FLOATS ? waves * (a.t * column + 256) : 0, join = waves > 1 ? 2 * waves * 1024 : 0;
   const size_t lds = place > join ? place : join;
-  const int64_t tiles = mx_tiles(a.n), most = static_cast<int64_t>(device_cu_count()) * (waves <= 16 ? 16 / waves : 1);
+  const int64_t tiles = mx_tiles(a.n), most = static_cast<int64_t>(device_cu_count()) * (FLOATS && a.t > 8 ? 1 : 16 / waves);
   const auto kern = mx_step_kernel<FMT, FLOATS, P, D>;
   const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds, limit);
   if (e != hipSuccess) return e;
