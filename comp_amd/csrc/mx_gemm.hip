@@ -220,7 +220,7 @@ __global__ __launch_bounds__(P <= 2 ? 1024 : 512) void mx_step_kernel(const Gemm
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int step = sp * 4 + s < steps ? sp * 4 + s : steps - 1;
-      into.w[s].q[0] = reinterpret_cast<const u32x4*>(a.w + tile * w_bytes)[step * 64 + lane];
+      into.w[s].q[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.w + tile * w_bytes) + step * 64 + lane);
     }
   };
 #pragma unroll

@@ -26,20 +26,18 @@ __device__ __forceinline__ float mx_act(float g, float u) {
   return static_cast<float>(p * p * b);
 }
 
-// The same in f32, within 2^-20 of it for products from 2^-126 on: e^-g is 2^t with t = -g log2(e) in two parts, so that t's
-// rounding (up to 2^-18) does not count; the exponential and the reciprocal are off by one step each.  `far`: gates for which a
-// step in between leaves f32's range.
+// The same in f32, within 2^-20 of it for products from 2^-126 on and gates from -80 on.  e^-g is 2^t with t = -g log2(e) in two
+// parts, so that t's rounding (up to 2^-18) does not count; the exponential and the reciprocal are off by one step each.  The
+// gate meets the other factor first: a step that leaves f32's range on the way to a product inside it is infinite, never a zero.
 template <int ACT>
-__device__ __forceinline__ float mx_act_near(float g, float u, bool& far) {
+__device__ __forceinline__ float mx_act_near(float g, float u) {
   if constexpr (ACT == MX_SILU) {
-    far |= !(g >= -80.f) || (__builtin_fabsf(g) < 0x1p-100f && g != 0.f);
-    const float t = g * -1.44269502f, rest = __builtin_fmaf(g, -1.44269502f, -t) + g * -1.92596303e-8f;
+    const float t = g * -1.44269502f, rest = __builtin_fmaf(g, -1.92596303e-8f, __builtin_fmaf(g, -1.44269502f, -t));
     const float e = __builtin_amdgcn_exp2f(t);
-    return g * __builtin_amdgcn_rcpf(1.f + __builtin_fmaf(e, rest * 0.693147182f, e)) * u;
+    return g * u * __builtin_amdgcn_rcpf(1.f + __builtin_fmaf(e, rest * 0.693147182f, e));
   } else {
-    far |= g != g || (g > 0.f && g < 0x1p-50f);
-    const float p = g > 0.f ? g : 0.f;
-    return p * p * u;
+    const float p = __builtin_fmaxf(g, 0.f);
+    return p * u * p;
   }
 }
 
@@ -51,20 +49,24 @@ __device__ __forceinline__ unsigned most4(unsigned most) {
 
 // A quad of lanes' block of gated products: scale and codes.  They come from f32 products where all that these may stand for, 2^-19 to
 // either side, give the same ones (scale and rounding are monotonous), and from 64 bits otherwise: with e4m3 one block in a thousand
-// (2^-15 an element).  Blocks of tiny products, and gates out of f32's range, take 64 bits too.
+// (2^-15 an element).  Blocks of products below 2^-60, with values that are no numbers, or with gates below -80 take 64 bits too.
 template <int FMT, int ACT>
 __device__ __forceinline__ void gate8(const float (&g)[8], const float (&u)[8], unsigned& s, unsigned (&c)[FMT == MX_E2M1 ? 1 : 2]) {
-  float low[8], high[8];
-  bool far = false;
+  float low[8], high[8], largest = 0.f, least = 0.f, zero = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float v = mx_act_near<ACT>(g[e], u[e], far);
+    const float v = mx_act_near<ACT>(g[e], u[e]);
+    largest = __builtin_fmaxf(largest, __builtin_fabsf(v));
+    zero = __builtin_fmaf(v, 0.f, zero);  // NaN from an infinity or a NaN on
+    if constexpr (ACT == MX_SILU) least = __builtin_fminf(least, g[e]);
+    else zero = __builtin_fmaf(g[e], 0.f, zero);
     low[e] = v - v * 0x1p-19f;
     high[e] = v + v * 0x1p-19f;
   }
-  const unsigned most = most4(mx_most(high));
-  s = mx_scale<FMT>(most4(mx_most(low)));
-  far |= s != mx_scale<FMT>(most) || most < (27u << 23) || most >= (255u << 23);  // 2^-100
+  const unsigned most = most4(__float_as_uint(largest));
+  s = mx_scale<FMT>(most);
+  // (2^-19 are up to 32 steps of an f32)
+  bool far = !(zero == 0.f) || least < -80.f || most < (67u << 23) || mx_scale<FMT>(most - 32) != s || mx_scale<FMT>(most + 32) != s;
   unsigned d[FMT == MX_E2M1 ? 1 : 2];
   mx_codes8<FMT>(low, s, c);
   mx_codes8<FMT>(high, s, d);
