@@ -540,11 +540,7 @@ __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) 
     if (step > last) return;
     dma_wait<(NS - 2) * (S::kLoads + S::kScaleLoads)>();
     __builtin_amdgcn_s_barrier();
-    // every wave is done with the place of the step before
-    const int free_slot = slot == 0 ? NS - 1 : slot - 1;
-    constexpr int AHEAD = STEP + NS - 1;
-    fetch(step + NS - 1, free_slot);
-    fetch_scales(AHEAD & 3, sp + AHEAD / 4 + 1);
+    asm volatile("" ::: "memory");  // (no read of shared memory moves up)
     if constexpr (STEP == 0) {
       const unsigned* const held = reinterpret_cast<const unsigned*>(lds_scales + (sp & 1) * S::kScales) + lane;
 #pragma unroll
@@ -561,6 +557,11 @@ __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) 
     for (int j = 0; j < WT; ++j)
 #pragma unroll
       for (int h = 0; h < S::kParts; ++h) x[j].q[h] = held[(S::kW + (wt * WT + j) * S::kParts + h) * 64];
+    // the next loads, while the reads are on their way: every wave is done with the place of the step before
+    const int free_slot = slot == 0 ? NS - 1 : slot - 1;
+    constexpr int AHEAD = STEP + NS - 1;
+    fetch(step + NS - 1, free_slot);
+    fetch_scales(AHEAD & 3, sp + AHEAD / 4 + 1);
     mma_step<FMT, STEP>(acc, w, ws, x, xs);
     slot = slot == NS - 1 ? 0 : slot + 1;
   };
