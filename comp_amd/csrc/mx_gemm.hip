@@ -5,7 +5,12 @@
 // memory; a product of two e2m1 elements has at most four bits, and its sums are f32's.  X in e4m3: that instruction adds a
 // block's products of e2m1 and e4m3 with some 15 bits below the largest one (measured: 2688 - 2688 + 1/16 gives 0), which
 // is not a 32-bit sum.  So both operands become bf16, scale included, which is exact (four bits at most, and bf16's exponents
-// are f32's; only activations below 2^-126 may lose bits), and v_mfma_f32_16x16x32_bf16 adds them in f32.
+// are f32's; only activations below 2^-126 may lose bits), and v_mfma_f32_16x16x32_bf16 adds them in f32.  (The scaled instruction
+// would save the conversions and half the matrix cores' time; on random codes its results were off by 2.7 times what f32 sums and
+// the rounding to bf16 allow.)
+//
+// Three kernels: one column tile of X (decode steps), tiles straight from memory (batches), tiles through shared memory (prompts).
+// Figures: one MI355X, 6.9 TB/s read, 1.22 PFLOP/s in an 8192^3 bf16 library product.
 #include <hip/hip_ext.h>
 
 #include <type_traits>
@@ -201,6 +206,12 @@ __device__ __forceinline__ void quantize_rows(const GemmArgs& a, int sp, bool in
 // Up to 16 rows of X.  A workgroup keeps X in registers, each wave P pieces of K, and walks over row tiles of W, whose codes
 // it loads D pieces ahead; its waves join in shared memory, in their order.  FLOATS: the rows are quantized on the way, by each
 // wave its own pieces, eight elements a lane, through shared memory into the operands' order.
+//
+// Bound by W's bytes where there are many: 128256 x 4096, one bf16 row to e4m3, in 44.7 us (6.3 TB/s; with W's loads through the
+// caches 48.9, quantizing X again for every row tile 182), 28672 x 4096, five rows to e2m1, in 12.0 us.  Small products are a chain of
+// latencies: 6912 x 2560 and one f32 row in 6.0 us in a graph, of which reading 9.4 MB is 1.4.  X as bf16 operands in registers costs
+// e4m3 64 conversions a piece of W and none of X; from 16 pieces on (K above 8192) a wave holds four pieces, as codes.  D = 2: one
+// piece on its way beside the one in use; with three the registers of P = 1 (128 for 16 waves) spill.
 template <int FMT, bool FLOATS, int P, int D>
 __global__ __launch_bounds__(P <= 2 ? 1024 : 512) void mx_step_kernel(const GemmArgs a) {
   constexpr bool kWide = P == 1;
@@ -319,7 +330,12 @@ __global__ __launch_bounds__(P <= 2 ? 1024 : 512) void mx_step_kernel(const Gemm
 
 // Operands come straight from memory: a workgroup has RT row tiles of W and CT tiles of X, its waves take four-step pieces of
 // K in turn and join in shared memory, in the waves' order.  SRC: the type of the rows that are quantized on the way (each wave
-// its own pieces), -1: X is quantized already.
+// its own pieces; rows of more than 16384 elements, which mx_step_kernel cannot hold), -1: X is quantized already.
+//
+// For batches, whose tiles are too few for the device unless a tile is small and K is shared out inside the workgroup.  Bound by the
+// caches (each operand is read by N / (16 RT) or T / (16 CT) workgroups) and, in e4m3, by conversions: 64 x 4096 x 14336 in 15.7 us
+// with cold weights, in e2m1 11.8; 100 x 4096 x 4096 in 8.4 us.  (K shared out over workgroups, tiles of 128 x 64 through shared
+// memory and the sums joined by a second launch: 19.0 and 14.4 us.)
 template <int FMT, int SRC, int RT, int CT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const GemmArgs a) {
   constexpr int kParts = FMT == MX_E2M1 ? 1 : 2;
@@ -467,6 +483,11 @@ struct TileShape {
 
 // A workgroup of GN x GT waves has GN * WN row tiles of W and GT * WT of X.  A step's codes lie in one of NS places in shared memory,
 // loaded NS - 1 steps ahead; the scales of the next four steps are loaded beside them, a quarter a step, into one of two places.
+//
+// Bound by the matrix cores, at the clock that their power leaves: 8192 x 14336 x 4096 in 632 us in e4m3 (1.52 PFLOP/s; the matrix cores
+// busy 66% of the time, conversions 46% of the issue slots) and 267 us in e2m1 (3.6 PFLOP/s, of which storing Y is some 55 us).  256 x
+// 256 tiles of eight waves, 128 x 64 each (a step reads 12 operands for 32 products); two or three places measured the same, loads by way
+// of registers and one step ahead 758 us.
 template <int FMT, int WN, int WT, int GN, int GT, int NS>
 __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) {
   using S = TileShape<FMT, WN, WT, GN, GT>;
@@ -620,6 +641,8 @@ hipError_t launch_step(const GemmArgs& a, hipStream_t stream) {
   const int column = (FMT == MX_E2M1 ? 256 : 512) + 16;
   const size_t place = FLOATS ? waves * (a.t * column + 256) : 0, join = waves > 1 ? 2 * waves * 1024 : 0;
   const size_t lds = place > join ? place : join;
+  // as many workgroups as the CUs hold waves for, each with several row tiles; one a CU where each quantizes many rows (16 rows of
+  // 4096, 14336 of W: 15.8 us against 18.9; one row: the same)
   const int64_t tiles = mx_tiles(a.n), most = static_cast<int64_t>(device_cu_count()) * (FLOATS && a.t > 8 ? 1 : 16 / waves);
   const auto kern = mx_step_kernel<FMT, FLOATS, P, D>;
   const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds, limit);
@@ -638,6 +661,12 @@ hipError_t launch_format(const MxGemmCall& c, const GemmArgs& a, hipStream_t str
     if (c.src_type == MX_F16) return launch_stream<FMT, MX_F16, 1, 1, 8>(a, stream);
     return launch_stream<FMT, MX_BF16, 1, 1, 8>(a, stream);
   }
+  // The largest tiles that are enough for the device.  Both sides, us (T x N x K):
+  //   256 x 256 tiles against 128 x 128: 8192 x 14336 x 4096 (1792 of 256 x 256) 647 and 698 in e4m3, 282 and 309 in e2m1; 2048 x 4096 x
+  //     4096 (128) 87 and 55
+  //   128 x 128 against 64 x 32: 256 x 14336 x 4096 (224 of 128 x 128) 17.5 and 31.5 in e2m1; 256 x 4096 x 14336 (64) 99 and 38 in e4m3
+  //   64 x 32 against 32 x 32: 100 x 4096 x 4096 (256 of 64 x 32) 9.0 and 10.0; 64 x 4096 x 14336 (128) 21.0 and 16.1
+  //   32 x 32 against 16 x 32: 64 x 4096 x 14336 (256 of 32 x 32) 16.1 and 20.8; 32 x 4096 x 14336 (128) 16.7 and 14.2
   const int64_t cus = device_cu_count(), n16 = mx_tiles(a.n), t16 = mx_tiles(a.t);
   auto groups = [&](int64_t rows, int64_t cols) { return ((n16 + rows - 1) / rows) * ((t16 + cols - 1) / cols); };
   if (groups(16, 16) >= 2 * cus) return launch_tile<FMT, 8, 4, 2, 4, 3>(a, stream);

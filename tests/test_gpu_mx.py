@@ -10,7 +10,7 @@ from tests import mx_ref as R
 pytestmark = pytest.mark.gpu
 
 DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
-SHAPES = [(1, 32), (2, 96), (15, 128), (16, 160), (17, 512), (33, 544), (5, 2560), (64, 1056)]
+SHAPES = [(1, 32), (2, 96), (15, 128), (16, 160), (17, 512), (33, 544), (5, 2560), (64, 1056), (300, 32), (131, 64), (70, 256), (33, 288)]
 
 
 def f64(t):
@@ -172,7 +172,7 @@ def test_gate_far_values(act):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fmt", mx.FORMATS)
 def test_lookup(fmt, dtype):
-    for n, k, count in [(1, 32, 1), (37, 96, 50), (100, 544, 17), (16, 2560, 3)]:
+    for n, k, count in [(1, 32, 1), (9, 32, 700), (20, 64, 129), (37, 96, 50), (50, 256, 77), (30, 288, 33), (100, 544, 17), (16, 2560, 3)]:
         rows, want = random_rows(n, k, fmt, n, 100, 140)
         ids = np.random.default_rng(count).integers(0, n, count)
         if count > 2:
