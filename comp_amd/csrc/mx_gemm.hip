@@ -335,7 +335,7 @@ __global__ __launch_bounds__(P <= 2 ? 1024 : 512) void mx_step_kernel(const Gemm
 // For batches, whose tiles are too few for the device unless a tile is small and K is shared out inside the workgroup.  Bound by the
 // caches (each operand is read by N / (16 RT) or T / (16 CT) workgroups) and, in e4m3, by conversions: 64 x 4096 x 14336 in 15.7 us
 // with cold weights, in e2m1 11.8; 100 x 4096 x 4096 in 8.4 us.  (K shared out over workgroups, tiles of 128 x 64 through shared
-// memory and the sums joined by a second launch: 19.0 and 14.4 us.)
+// memory and the sums joined by a second launch: 19.0 and 14.4 us; two pieces of a wave's on their way: 18.4 and 12.6 us.)
 template <int FMT, int SRC, int RT, int CT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const GemmArgs a) {
   constexpr int kParts = FMT == MX_E2M1 ? 1 : 2;
@@ -641,9 +641,9 @@ hipError_t launch_step(const GemmArgs& a, hipStream_t stream) {
   const int column = (FMT == MX_E2M1 ? 256 : 512) + 16;
   const size_t place = FLOATS ? waves * (a.t * column + 256) : 0, join = waves > 1 ? 2 * waves * 1024 : 0;
   const size_t lds = place > join ? place : join;
-  // as many workgroups as the CUs hold waves for, each with several row tiles; one a CU where each quantizes many rows (16 rows of
+  // as many workgroups as make 16 waves a CU, each with several row tiles; 8 waves where each workgroup quantizes many rows (16 rows of
   // 4096, 14336 of W: 15.8 us against 18.9; one row: the same)
-  const int64_t tiles = mx_tiles(a.n), most = static_cast<int64_t>(device_cu_count()) * (FLOATS && a.t > 8 ? 1 : 16 / waves);
+  const int64_t tiles = mx_tiles(a.n), most = static_cast<int64_t>(device_cu_count()) * (FLOATS && a.t > 8 ? (waves < 8 ? 8 / waves : 1) : 16 / waves);
   const auto kern = mx_step_kernel<FMT, FLOATS, P, D>;
   const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds, limit);
   if (e != hipSuccess) return e;

@@ -33,7 +33,8 @@ _Tensor, _I64, _U8 = torch.Tensor, torch.int64, torch.uint8
 FORMATS = {"e2m1": 0, "e4m3": 1}
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTS = {"silu": 1, "relu2": 2}
-LINEAR_ROWS = 16  # rows that linear() quantizes and multiplies in one launch
+LINEAR_ROWS = 16  # rows that linear() quantizes and multiplies in one launch,
+LINEAR_VALUES = 98304  # of fewer values than these in all
 _BAD = _abi.KompArgumentError
 _new = object.__new__
 
@@ -311,7 +312,10 @@ def gemm(x, w, dtype=torch.float32):
 
 def _linear(x, w, y, fmt):
     t = x.shape[0]
-    if t > LINEAR_ROWS:
+    # Each workgroup of the one launch quantizes all rows; two launches cost an eager call 15 us of host time in all.  One launch and two,
+    # in a graph, to e4m3 (us): 16 rows through 4096 x 14336 27.5 and 14.7, 8 rows 19.1 and 14.8, 5 rows 16.3 and 14.7, 2 rows 12.7 and
+    # 14.7; 16 rows through 4096 x 8192 15.0 and 10.8, through 14336 x 4096 14.3 and 13.3.
+    if t > LINEAR_ROWS or t * w.k >= LINEAR_VALUES:
         rows = _empty(w._planes, t, w.k, fmt)  # kept until the calls are on the stream; torch hands it to later work of this stream
         _quantize(x, rows, 0)
         _gemm(rows, w, y, y.stride(0))
@@ -321,8 +325,8 @@ def _linear(x, w, y, fmt):
 
 
 def linear_into(x, w, y, fmt="e4m3"):
-    """linear() into y [T][N] (f32, f16 or bf16; rows contiguous, any stride between them that keeps them apart).  (More than
-    LINEAR_ROWS rows still take a workspace for their quantized form from torch.)"""
+    """linear() into y [T][N] (f32, f16 or bf16; rows contiguous, any stride between them that keeps them apart).  (Rows that
+    take two launches still take a workspace for their quantized form from torch.)"""
     _need_format(fmt)
     _need_rows(w, "w")
     _need_weights(w, w.k, w._device)
@@ -333,8 +337,8 @@ def linear_into(x, w, y, fmt="e4m3"):
 
 def linear(x, w, fmt="e4m3", dtype=None):
     """x [T][K] (f32, f16 or bf16; rows contiguous, any stride between them), quantized to fmt, times w Rows [N][K] (e2m1) -> Y
-    [T][N] of dtype (x's by default).  Equal to gemm(quantize(x, fmt), w, dtype) bit for bit; up to LINEAR_ROWS rows take one
-    launch."""
+    [T][N] of dtype (x's by default).  Equal to gemm(quantize(x, fmt), w, dtype) bit for bit; up to LINEAR_ROWS rows of fewer
+    than LINEAR_VALUES values in all take one launch."""
     _need_format(fmt)
     _need_rows(w, "w")
     _need_weights(w, w.k, w._device)

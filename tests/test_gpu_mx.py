@@ -314,6 +314,17 @@ def test_linear(fmt, dtype, shape):
     assert mx.linear(x.cuda(), w, fmt).dtype is DTYPES[dtype]
 
 
+@pytest.mark.parametrize("t,k", [(5, 9216), (16, 4096), (16, 14336), (16, 20000)])
+@pytest.mark.parametrize("fmt", mx.FORMATS)
+def test_linear_one_launch(fmt, t, k):
+    """The C entry on rows that linear() gives two launches."""
+    x = inputs(t, k, "bf16", 2, special=False).cuda()
+    w, _ = random_rows(50, k, "e2m1", 3)
+    y = torch.zeros(t, 50, device="cuda")
+    _abi.call("komp_mx_linear", x.data_ptr(), 2, k, t, mx.FORMATS[fmt], w._ref, y.data_ptr(), 0, 50, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(y, mx.linear(x, w, fmt, torch.float32))
+
+
 def test_linear_special():
     x = inputs(9, 1056, "f32", 3).cuda()
     w, _ = random_rows(65, 1056, "e2m1", 12)
