@@ -301,7 +301,7 @@ def gemm_into(x, w, y):
 
 def gemm(x, w, dtype=torch.float32):
     """x Rows [T][K] (e2m1 or e4m3) times w Rows [N][K] (e2m1) -> Y [T][N] of dtype: the sums over K of the products of what the
-    elements stand for, in f32, rounded once."""
+    elements stand for, in f32, rounded once.  T up to 2^20 - 16, N up to 2^26; the order of the sums depends on the sizes alone."""
     _need_rows(x, "x")
     _need_weights(w, x.k, x._device)
     _type(dtype)
