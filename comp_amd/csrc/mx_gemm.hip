@@ -460,10 +460,10 @@ __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const GemmArgs a)
 // 1 KB (16 bytes a lane) or 256 bytes (4 a lane) from memory straight into shared memory at `place`, lane after lane.  The
 // compiler does not see these loads: dma_wait waits for them, and the barrier behind it for the other waves'.
 __device__ __forceinline__ void dma16(unsigned place, const uint8_t* base, unsigned offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(place), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(place), "v"(offset), "s"(base) : "m0", "memory");
 }
 __device__ __forceinline__ void dma4(unsigned place, const uint8_t* base, unsigned offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(place), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(place), "v"(offset), "s"(base) : "m0", "memory");
 }
 // until at most N of this wave's loads are on their way, and its reads of shared memory are done
 template <int N>
