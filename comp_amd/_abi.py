@@ -80,6 +80,7 @@ SIGNATURES = {
     "komp_mx_pack": (_INT, [_P, _P, _P, _P]),
     "komp_mx_unpack": (_INT, [_P, _P, _P, _P]),
     "komp_mx_gemm": (_INT, [_P, _P, _P, _INT, _I64, _P]),
+    "komp_mx_gemm_launch": (_INT, [_I64, _I64, _I64, _P, _P, _P]),
     "komp_mx_linear": (_INT, [_P, _INT, _I64, _I64, _INT, _P, _P, _INT, _I64, _P]),
     "komp_timing_begin": (_INT, [_I64]),
     "komp_timing_end": (_INT, [_P, _P]),
@@ -170,6 +171,16 @@ def gemm_launch(fmt_id, m, n, k, sw, store_s=False):
     v = [ctypes.c_int(0) for _ in range(6)]
     st = lib().komp_gemm_launch(fmt_id, int(store_s), m, n, k, sw, *(ctypes.byref(x) for x in v))
     return (bool(v[0].value), *(x.value for x in v[1:])) if st == 0 else None
+
+
+MX_KERNELS = ("step", "stream", "tile")
+
+
+def mx_gemm_launch(t, n, k):
+    """(kernel: one of MX_KERNELS, tiles of 16 weight rows, tiles of 16 rows of X) of a workgroup of the microscaled product."""
+    v = [ctypes.c_int(0) for _ in range(3)]
+    call("komp_mx_gemm_launch", t, n, k, *(ctypes.byref(x) for x in v))
+    return (MX_KERNELS[v[0].value], *(x.value for x in v[1:]))
 
 
 def gemv_mfma_plan(fmt_id, fused, mode, m, n, k, sw):

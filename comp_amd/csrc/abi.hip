@@ -1489,6 +1489,23 @@ int komp_mx_gemm(const komp_mx_rows* X, const komp_mx_rows* W, void* Y, int type
   return hip_status(launch_mx_gemm(c, static_cast<hipStream_t>(stream)), name);
 }
 
+int komp_mx_gemm_launch(int64_t T, int64_t N, int64_t K, int* kernel, int* row_tiles, int* col_tiles) {
+  const char* name = "komp_mx_gemm_launch";
+  if (T < 1 || N < 1) return fail(KOMP_EINVAL, "%s: T=%lld N=%lld", name, static_cast<long long>(T), static_cast<long long>(N));
+  alignas(16) uint8_t plane[16];  // (descriptors as the product would get them)
+  const komp_mx_rows xs = {plane, plane, T, K, MX_E2M1}, ws = {plane, plane, N, K, MX_E2M1};
+  MxRows x, w;
+  int st = mx_rows_of(name, "X", &xs, x);
+  if (st == KOMP_OK) st = mx_rows_of(name, "W", &ws, w);
+  if (st == KOMP_OK) st = mx_product(name, T, w);
+  if (st != KOMP_OK) return st;
+  const MxGemmPlan p = mx_gemm_plan(T, N, K);
+  if (kernel != nullptr) *kernel = p.kernel;
+  if (row_tiles != nullptr) *row_tiles = p.row_tiles;
+  if (col_tiles != nullptr) *col_tiles = p.col_tiles;
+  return KOMP_OK;
+}
+
 int komp_mx_linear(const void* X, int x_type, int64_t x_stride, int64_t T, int fmt, const komp_mx_rows* W, void* Y, int type,
                    int64_t y_stride, void* stream) {
   const char* name = "komp_mx_linear";

@@ -653,30 +653,45 @@ hipError_t launch_step(const GemmArgs& a, hipStream_t stream) {
 template <int FMT>
 hipError_t launch_format(const MxGemmCall& c, const GemmArgs& a, hipStream_t stream) {
   const bool floats = c.src != nullptr;
-  if (a.t <= 16) {
+  const MxGemmPlan p = mx_gemm_plan(a.t, a.n, a.k);
+  if (p.kernel == MX_STEP) {
     if (mx_supers(a.k) <= 16) return floats ? launch_step<FMT, true, 1, 2>(a, stream) : launch_step<FMT, false, 1, 2>(a, stream);
-    if (mx_supers(a.k) <= 32) return floats ? launch_step<FMT, true, 4, 2>(a, stream) : launch_step<FMT, false, 4, 2>(a, stream);
-    if (!floats) return launch_stream<FMT, -1, 1, 1, 8>(a, stream);
-    if (c.src_type == MX_F32) return launch_stream<FMT, MX_F32, 1, 1, 8>(a, stream);
-    if (c.src_type == MX_F16) return launch_stream<FMT, MX_F16, 1, 1, 8>(a, stream);
-    return launch_stream<FMT, MX_BF16, 1, 1, 8>(a, stream);
+    return floats ? launch_step<FMT, true, 4, 2>(a, stream) : launch_step<FMT, false, 4, 2>(a, stream);
   }
+  if (p.kernel == MX_TILE) {
+    if (p.row_tiles == 16) return launch_tile<FMT, 8, 4, 2, 4, 3>(a, stream);
+    return launch_tile<FMT, 4, 4, 2, 2, 3>(a, stream);
+  }
+  if (p.col_tiles == 2) {
+    if (p.row_tiles == 4) return launch_stream<FMT, -1, 4, 2, 8>(a, stream);
+    if (p.row_tiles == 2) return launch_stream<FMT, -1, 2, 2, 8>(a, stream);
+    return launch_stream<FMT, -1, 1, 2, 8>(a, stream);
+  }
+  if (!floats) return launch_stream<FMT, -1, 1, 1, 8>(a, stream);
+  if (c.src_type == MX_F32) return launch_stream<FMT, MX_F32, 1, 1, 8>(a, stream);
+  if (c.src_type == MX_F16) return launch_stream<FMT, MX_F16, 1, 1, 8>(a, stream);
+  return launch_stream<FMT, MX_BF16, 1, 1, 8>(a, stream);
+}
+
+}  // namespace
+
+MxGemmPlan mx_gemm_plan(int64_t t, int64_t n, int64_t k) {
+  // (mx_step_kernel holds rows of up to 16384 elements)
+  if (t <= 16) return mx_supers(k) <= 32 ? MxGemmPlan{MX_STEP, 1, 1} : MxGemmPlan{MX_STREAM, 1, 1};
   // The largest tiles that are enough for the device.  Both sides, us (T x N x K):
   //   256 x 256 tiles against 128 x 128: 8192 x 14336 x 4096 (1792 of 256 x 256) 647 and 698 in e4m3, 282 and 309 in e2m1; 2048 x 4096 x
   //     4096 (128) 87 and 55
   //   128 x 128 against 64 x 32: 256 x 14336 x 4096 (224 of 128 x 128) 17.5 and 31.5 in e2m1; 256 x 4096 x 14336 (64) 99 and 38 in e4m3
   //   64 x 32 against 32 x 32: 100 x 4096 x 4096 (256 of 64 x 32) 9.0 and 10.0; 64 x 4096 x 14336 (128) 21.0 and 16.1
   //   32 x 32 against 16 x 32: 64 x 4096 x 14336 (256 of 32 x 32) 16.1 and 20.8; 32 x 4096 x 14336 (128) 16.7 and 14.2
-  const int64_t cus = device_cu_count(), n16 = mx_tiles(a.n), t16 = mx_tiles(a.t);
+  const int64_t cus = device_cu_count(), n16 = mx_tiles(n), t16 = mx_tiles(t);
   auto groups = [&](int64_t rows, int64_t cols) { return ((n16 + rows - 1) / rows) * ((t16 + cols - 1) / cols); };
-  if (groups(16, 16) >= 2 * cus) return launch_tile<FMT, 8, 4, 2, 4, 3>(a, stream);
-  if (8 * groups(8, 8) >= 5 * cus) return launch_tile<FMT, 4, 4, 2, 2, 3>(a, stream);
-  if (groups(4, 2) >= cus) return launch_stream<FMT, -1, 4, 2, 8>(a, stream);
-  if (groups(2, 2) >= cus) return launch_stream<FMT, -1, 2, 2, 8>(a, stream);
-  return launch_stream<FMT, -1, 1, 2, 8>(a, stream);
+  if (groups(16, 16) >= 2 * cus) return {MX_TILE, 16, 16};
+  if (8 * groups(8, 8) >= 5 * cus) return {MX_TILE, 8, 8};
+  if (groups(4, 2) >= cus) return {MX_STREAM, 4, 2};
+  if (groups(2, 2) >= cus) return {MX_STREAM, 2, 2};
+  return {MX_STREAM, 1, 2};
 }
-
-}  // namespace
 
 hipError_t launch_mx_gemm(const MxGemmCall& c, hipStream_t stream) {
   GemmArgs a;

@@ -76,6 +76,15 @@ struct MxGemmCall {
   int64_t stride;
 };
 
+// The kernel that a product runs on, and the tiles of 16 rows of W and of X that a workgroup has at once.
+enum MxKernel { MX_STEP = 0, MX_STREAM = 1, MX_TILE = 2 };
+struct MxGemmPlan {
+  MxKernel kernel;
+  int row_tiles;
+  int col_tiles;
+};
+MxGemmPlan mx_gemm_plan(int64_t t, int64_t n, int64_t k);
+
 constexpr int kMxLinearRows = 16;  // rows that one launch quantizes on the way: one column tile
 
 hipError_t launch_mx_quantize(const MxQuantCall& c, hipStream_t stream);

@@ -334,6 +334,11 @@ int komp_mx_gemm(const komp_mx_rows* X, const komp_mx_rows* W, void* Y, int type
 int komp_mx_linear(const void* X, int x_type, int64_t x_stride, int64_t T, int fmt, const komp_mx_rows* W, void* Y, int type,
                    int64_t y_stride, void* stream);
 
+/* The kernel that the product of T rows and N weight rows of K elements runs on, on the current device: 0 one tile of 16 rows of X, kept
+ * in registers, 1 tiles straight from memory, 2 tiles through shared memory, and the tiles of 16 rows of W and of X that a
+ * workgroup has at once.  NULL outputs are skipped.  Returns KOMP_EINVAL for sizes that komp_mx_gemm refuses, or without rows. */
+int komp_mx_gemm_launch(int64_t T, int64_t N, int64_t K, int* kernel, int* row_tiles, int* col_tiles);
+
 /* Dispatch timing for the tuning harness (no reference counterpart; the reference was never timed).
  * Between komp_timing_begin() and komp_timing_end(), every launch made by this library on the calling process is
  * issued with hipExtLaunchKernel start/stop events, which the runtime stamps with the dispatch's own begin and end.
