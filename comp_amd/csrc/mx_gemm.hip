@@ -684,12 +684,21 @@ MxGemmPlan mx_gemm_plan(int64_t t, int64_t n, int64_t k) {
   //   128 x 128 against 64 x 32: 256 x 14336 x 4096 (224 of 128 x 128) 17.5 and 31.5 in e2m1; 256 x 4096 x 14336 (64) 99 and 38 in e4m3
   //   64 x 32 against 32 x 32: 100 x 4096 x 4096 (256 of 64 x 32) 9.0 and 10.0; 64 x 4096 x 14336 (128) 21.0 and 16.1
   //   32 x 32 against 16 x 32: 64 x 4096 x 14336 (256 of 32 x 32) 16.1 and 20.8; 32 x 4096 x 14336 (128) 16.7 and 14.2
+  //
+  // A group that ends past T or N takes its full time for what it throws away, so a tile must also be mostly filled.  Both sides, us:
+  //   256 x 256 covers at most 5/4 of what 128 x 128 tiles cover: with 131072 of W and K = 4096, 17 rows of X (twice as much) 177 and 108 in
+  //     e4m3, 85 and 58 in e2m1; 300 rows (4/3) 376 and 318, 178 and 179; 640 rows (6/5) 577 and 547, 281 and 304; 144 rows (as much) 187 and 211
+  //   128 x 128 against 64 x 32 where one of these holds all rows of X or of W: 32 x 28672 x 4096 30.7 and 19.7 in e4m3, 17.6 and 16.2 in
+  //     e2m1, 32 x 128256 x 4096 106 and 71, 57 and 58; 262144 x 64 x 1024 69 and 63, 40 and 29; past that, 33 x 131072 x 4096 110 and 127, 59 and
+  //     105; 262144 x 80 x 1024 69 and 101, 41 and 53
+  //   64 x 32 against 32 x 32 for W of 32 rows: 262144 x 32 x 1024 52 and 42 in e4m3, 24 and 23 in e2m1; 32 x 32 against 16 x 32 for 16
+  //     rows: 8192 x 16 x 4096 5.4 and 4.8, 3.9 and 3.7
   const int64_t cus = device_cu_count(), n16 = mx_tiles(n), t16 = mx_tiles(t);
   auto groups = [&](int64_t rows, int64_t cols) { return ((n16 + rows - 1) / rows) * ((t16 + cols - 1) / cols); };
-  if (groups(16, 16) >= 2 * cus) return {MX_TILE, 16, 16};
-  if (8 * groups(8, 8) >= 5 * cus) return {MX_TILE, 8, 8};
-  if (groups(4, 2) >= cus) return {MX_STREAM, 4, 2};
-  if (groups(2, 2) >= cus) return {MX_STREAM, 2, 2};
+  if (groups(16, 16) >= 2 * cus && 16 * groups(16, 16) <= 5 * groups(8, 8)) return {MX_TILE, 16, 16};
+  if (8 * groups(8, 8) >= 5 * cus && n16 > 4 && t16 > 2) return {MX_TILE, 8, 8};
+  if (groups(4, 2) >= cus && n16 > 2) return {MX_STREAM, 4, 2};
+  if (groups(2, 2) >= cus && n16 > 1) return {MX_STREAM, 2, 2};
   return {MX_STREAM, 1, 2};
 }
 
