@@ -35,6 +35,7 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTS = {"silu": 1, "relu2": 2}
 LINEAR_ROWS = 16  # rows that linear() quantizes and multiplies in one launch,
 LINEAR_VALUES = 98304  # of fewer values than these in all
+MAX_ROWS, MAX_WEIGHTS = (1 << 20) - 16, 1 << 26  # of one product
 _BAD = _abi.KompArgumentError
 _new = object.__new__
 
@@ -281,10 +282,12 @@ def from_ggml(W, n, k):
 # ---- products --------------------------------------------------------------------------------------------------------
 
 
-def _need_weights(w, k, device):
+def _need_weights(w, k, device, t):
     _need_rows(w, "w")
     if w.fmt != "e2m1" or w.k != k or w._device != device:
         raise _BAD(f"w must be e2m1 rows of {k} elements on cuda:{device}, got {w.fmt} rows of {w.k} on {w.device}")
+    if t > MAX_ROWS or w.rows > MAX_WEIGHTS:
+        raise _BAD(f"{t} x {w.rows} results (2^20 - 16 rows of x and 2^26 of w at most)")
 
 
 def _gemm(x, w, y, stride):
@@ -294,7 +297,7 @@ def _gemm(x, w, y, stride):
 def gemm_into(x, w, y):
     """gemm() into y [T][N] (f32, f16 or bf16; rows contiguous, any stride between them that keeps them apart)."""
     _need_rows(x, "x")
-    _need_weights(w, x.k, x._device)
+    _need_weights(w, x.k, x._device, x.rows)
     _need_matrix(y, "y", w.rows, x._device, x.rows, output=True)
     _gemm(x, w, y, y.stride(0))
 
@@ -303,7 +306,7 @@ def gemm(x, w, dtype=torch.float32):
     """x Rows [T][K] (e2m1 or e4m3) times w Rows [N][K] (e2m1) -> Y [T][N] of dtype: the sums over K of the products of what the
     elements stand for, in f32, rounded once.  T up to 2^20 - 16, N up to 2^26; the order of the sums depends on the sizes alone."""
     _need_rows(x, "x")
-    _need_weights(w, x.k, x._device)
+    _need_weights(w, x.k, x._device, x.rows)
     _type(dtype)
     y = w._planes.new_empty((x.rows, w.rows), dtype=dtype)
     _gemm(x, w, y, w.rows)
@@ -329,8 +332,8 @@ def linear_into(x, w, y, fmt="e4m3"):
     take two launches still take a workspace for their quantized form from torch.)"""
     _need_format(fmt)
     _need_rows(w, "w")
-    _need_weights(w, w.k, w._device)
     _need_matrix(x, "x", w.k, w._device)
+    _need_weights(w, w.k, w._device, x.shape[0])
     _need_matrix(y, "y", w.rows, w._device, x.shape[0], output=True)
     _linear(x, w, y, fmt)
 
@@ -338,11 +341,11 @@ def linear_into(x, w, y, fmt="e4m3"):
 def linear(x, w, fmt="e4m3", dtype=None):
     """x [T][K] (f32, f16 or bf16; rows contiguous, any stride between them), quantized to fmt, times w Rows [N][K] (e2m1) -> Y
     [T][N] of dtype (x's by default).  Equal to gemm(quantize(x, fmt), w, dtype) bit for bit; up to LINEAR_ROWS rows of fewer
-    than LINEAR_VALUES values in all take one launch."""
+    than LINEAR_VALUES values in all take one launch.  T and N as gemm()'s."""
     _need_format(fmt)
     _need_rows(w, "w")
-    _need_weights(w, w.k, w._device)
     _need_matrix(x, "x", w.k, w._device)
+    _need_weights(w, w.k, w._device, x.shape[0])
     dtype = x.dtype if dtype is None else dtype
     _type(dtype)
     y = w._planes.new_empty((x.shape[0], w.rows), dtype=dtype)
