@@ -1385,6 +1385,14 @@ int mx_type_of(const char* name, int type, const void* p, int64_t stride) {
   return KOMP_OK;
 }
 
+// an array that is written, rows of `width` elements
+int mx_out_of(const char* name, int type, const void* p, int64_t stride, int64_t rows, int64_t width) {
+  const int st = mx_type_of(name, type, p, stride);
+  if (st == KOMP_OK && rows > 1 && stride < width && stride > -width)
+    return fail(KOMP_EINVAL, "%s: rows of %lld overlap (row stride %lld)", name, static_cast<long long>(width), static_cast<long long>(stride));
+  return st;
+}
+
 // Y [t][w.rows]: the shapes that the kernels' grids and 32-bit sizes hold
 int mx_product(const char* name, int64_t t, const MxRows& w) {
   if (w.fmt != MX_E2M1) return fail(KOMP_EINVAL, "%s: W must be e2m1 rows", name);
@@ -1428,7 +1436,7 @@ int komp_mx_lookup(const komp_mx_rows* R, const int64_t* IDS, int64_t count, voi
     return fail(KOMP_EINVAL, "%s: count=%lld without IDS (all of the %lld rows)", name, static_cast<long long>(count),
                 static_cast<long long>(c.r.rows));
   if (!aligned(IDS, 8)) return fail(KOMP_EINVAL, "%s: IDS must be 8-byte aligned", name);
-  st = mx_type_of(name, type, OUT, out_stride);
+  st = mx_out_of(name, type, OUT, out_stride, count, c.r.k);
   if (st != KOMP_OK) return st;
   c.ids = IDS;
   c.count = count;
@@ -1478,7 +1486,7 @@ int komp_mx_gemm(const komp_mx_rows* X, const komp_mx_rows* W, void* Y, int type
   if (c.x.k != c.w.k)
     return fail(KOMP_EINVAL, "%s: X has rows of %lld, W of %lld", name, static_cast<long long>(c.x.k), static_cast<long long>(c.w.k));
   if (c.x.rows == 0 || c.w.rows == 0) return KOMP_OK;
-  st = mx_type_of(name, type, Y, y_stride);
+  st = mx_out_of(name, type, Y, y_stride, c.x.rows, c.w.rows);
   if (st != KOMP_OK) return st;
   c.src = nullptr;
   c.src_type = 0;
@@ -1517,7 +1525,7 @@ int komp_mx_linear(const void* X, int x_type, int64_t x_stride, int64_t T, int f
   if (T < 0 || T > kMxLinearRows) return fail(KOMP_EINVAL, "%s: T=%lld rows (0 to %d)", name, static_cast<long long>(T), kMxLinearRows);
   if (T == 0 || c.w.rows == 0) return KOMP_OK;
   st = mx_type_of(name, x_type, X, x_stride);
-  if (st == KOMP_OK) st = mx_type_of(name, type, Y, y_stride);
+  if (st == KOMP_OK) st = mx_out_of(name, type, Y, y_stride, T, c.w.rows);
   if (st != KOMP_OK) return st;
   c.x = MxRows{nullptr, nullptr, T, c.w.k, fmt};
   c.src = X;

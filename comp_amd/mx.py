@@ -14,7 +14,8 @@ scale is 2^(floor(log2(largest magnitude)) - 2) for e2m1 and - 8 for e4m3 (2^-12
 ties to even, and saturate.  A block that holds an infinity or a NaN is NaN throughout.
 
 As in comp_amd.host, tensors live on a HIP device, calls run on the current torch stream without synchronising, wrong
-arguments raise KompArgumentError before anything is launched, and the *_into forms allocate no result.  There are no gradients.
+arguments raise KompArgumentError before anything is launched, and the *_into forms allocate no result.  What is written must not
+overlap what the same call reads: no call works in place.  There are no gradients.
 No reference counterpart.
 """
 

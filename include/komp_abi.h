@@ -300,7 +300,8 @@ int komp_kv_attend_workspace(const komp_kv_cache* C, int type, int64_t T, int64_
  *   [ceil(rows / 16)][ceil(k / 512) * 256], each 16-byte aligned.  The order of the bytes is the library's own (tiles of 16 rows
  *   in the matrix instruction's order): rows are written and read through these entries, which keep the places behind the
  *   last row and the last block zero.
- * type: 0 f32, 1 f16, 2 bf16 (X, Y, OUT); fmt: 0 e2m1, 1 e4m3.  Strides count elements between rows; a row is contiguous. */
+ * type: 0 f32, 1 f16, 2 bf16 (X, Y, OUT); fmt: 0 e2m1, 1 e4m3.  Strides count elements between rows; a row is contiguous.  X's rows may
+ * overlap, those of Y and OUT must not, nor what is written with what the same call reads. */
 typedef struct komp_mx_rows {
   uint8_t* CODES;
   uint8_t* SCALES;
