@@ -5,7 +5,8 @@
 // memory; a product of two e2m1 elements has at most four bits, and its sums are f32's.  X in e4m3: that instruction adds a
 // block's products of e2m1 and e4m3 with some 15 bits below the largest one (measured: 2688 - 2688 + 1/16 gives 0), which
 // is not a 32-bit sum.  So both operands become bf16, scale included, which is exact (four bits at most, and bf16's exponents
-// are f32's; only activations below 2^-126 may lose bits), and v_mfma_f32_16x16x32_bf16 adds them in f32.  (The scaled instruction
+// are f32's, subnormals included; only elements of X with scale bytes 0 to 2 lie between bf16's multiples of 2^-133, and values past
+// f32's largest are infinite), and v_mfma_f32_16x16x32_bf16 adds them in f32.  (The scaled instruction
 // would save the conversions and half the matrix cores' time; on random codes its results were off by 2.7 times what f32 sums and
 // the rounding to bf16 allow.)
 //

@@ -238,7 +238,8 @@ def lookup(rows, ids, dtype=torch.float32, scale=1.0):
 
 
 def values(rows, dtype=torch.float32):
-    """All rows as values [rows][K] of dtype (bf16 holds every value of magnitude 2^-126 and more exactly, f32 all)."""
+    """All rows as values [rows][K] of dtype.  f32 holds every value below 2^128, bf16 those of magnitude 2^-126 and more exactly;
+    past that, which only pack() and from_ggml() bring (scale bytes from 253 on in e2m1, from 247 on in e4m3), they are infinite."""
     _need_rows(rows, "rows")
     number = _type(dtype)
     out = rows._planes.new_empty((rows.rows, rows.k), dtype=dtype)
@@ -305,7 +306,11 @@ def gemm_into(x, w, y):
 
 def gemm(x, w, dtype=torch.float32):
     """x Rows [T][K] (e2m1 or e4m3) times w Rows [N][K] (e2m1) -> Y [T][N] of dtype: the sums over K of the products of what the
-    elements stand for, in f32, rounded once.  T up to 2^20 - 16, N up to 2^26; the order of the sums depends on the sizes alone."""
+    elements stand for, in f32, rounded once.  T up to 2^20 - 16, N up to 2^26; the order of the sums depends on the sizes alone.
+
+    In products with e4m3 rows both operands' values are bf16's, which is exact but at the ends: elements of rows with scale bytes 0 to 2
+    are rounded to multiples of 2^-133, and weights and rows past f32's largest (see values()) are infinite, so that sums with them
+    are infinite or NaN.  Products of e2m1 rows have no such ends."""
     _need_rows(x, "x")
     _need_weights(w, x.k, x._device, x.rows)
     _type(dtype)

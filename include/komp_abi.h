@@ -327,7 +327,9 @@ int komp_mx_pack(const komp_mx_rows* R, const uint8_t* CODES, const uint8_t* SCA
 int komp_mx_unpack(const komp_mx_rows* R, uint8_t* CODES, uint8_t* SCALES, void* stream);
 
 /* Y [X->rows][W->rows] = X W^T of what the rows stand for, W e2m1, sums in f32, rounded once to `type`.  X has at most 2^20 - 16
- * rows, W 2^26.  A product's sums run in an order that depends on the sizes alone. */
+ * rows, W 2^26.  A product's sums run in an order that depends on the sizes alone.  With X e4m3 both operands' values are bf16's: exact, but
+ * elements of rows with scale bytes 0 to 2 are rounded to multiples of 2^-133, and values of 2^128 and more (W from byte 253 on, X from
+ * 247 on, which komp_mx_pack alone brings) are infinite, so that sums with them are infinite or NaN. */
 int komp_mx_gemm(const komp_mx_rows* X, const komp_mx_rows* W, void* Y, int type, int64_t y_stride, void* stream);
 
 /* The same for T rows X [T][W->k] of floats (T at most 16), quantized to `fmt` inside the launch: equal to komp_mx_quantize and
