@@ -2,9 +2,9 @@
 //
 // The weights are the matrix instruction's A operand and the activations its B operand, so a lane's four results are four
 // consecutive outputs of one row of X.  X in e2m1: v_mfma_scale_f32_16x16x128_f8f6f4 takes codes and scale bytes as they lie in
-// memory; a product of two e2m1 elements has at most four bits, and its sums are f32's.  X in e4m3: that instruction adds a
-// block's products of e2m1 and e4m3 with some 15 bits below the largest one (measured: 2688 - 2688 + 1/16 gives 0), which
-// is not a 32-bit sum.  So both operands become bf16, scale included, which is exact (four bits at most, and bf16's exponents
+// memory; a product of two e2m1 elements has at most four bits, and its sums are f32's.  X in e4m3: that instruction aligns the
+// products of eight consecutive elements and drops what lies 14 binades and more below the group's largest (measured: 256 - 256 + 2^-5 is
+// kept, + 2^-6 is not), which is not a 32-bit sum.  So both operands become bf16, scale included, which is exact (four bits at most, and bf16's exponents
 // are f32's, subnormals included; only elements of X with scale bytes 0 to 2 lie between bf16's multiples of 2^-133, and values past
 // f32's largest are infinite), and v_mfma_f32_16x16x32_bf16 adds them in f32.  (The scaled instruction
 // would save the conversions and half the matrix cores' time; on random codes its results were off by 2.7 times what f32 sums and
@@ -214,7 +214,7 @@ __device__ __forceinline__ void quantize_rows(const GemmArgs& a, int sp, bool in
 // e4m3 64 conversions a piece of W and none of X; from 16 pieces on (K above 8192) a wave holds four pieces, as codes.  D = 2: one
 // piece on its way beside the one in use; with three the registers of P = 1 (128 for 16 waves) spill.
 template <int FMT, bool FLOATS, int P, int D>
-__global__ __launch_bounds__(P <= 2 ? 1024 : 512) void mx_step_kernel(const GemmArgs a) {
+__global__ __launch_bounds__(P == 1 ? 1024 : 512) void mx_step_kernel(const GemmArgs a) {
   constexpr bool kWide = P == 1;
   constexpr int kTiles = D > P ? D / P : 1;                   // row tiles a turn of the loop
   constexpr int kColumn = (FMT == MX_E2M1 ? 256 : 512) + 16;  // bytes of a column's piece, apart in the banks
@@ -482,20 +482,22 @@ struct TileShape {
   static constexpr int kStage = kLoads * kWaves * 1024, kScales = kScaleLoads * 4 * kWaves * 256;
 };
 
-// A workgroup of GN x GT waves has GN * WN row tiles of W and GT * WT of X.  A step's codes lie in one of NS places in shared memory,
-// loaded NS - 1 steps ahead; the scales of the next four steps are loaded beside them, a quarter a step, into one of two places.
+// Places in shared memory for a step's codes.  (Scales are read before the next but one's loads: four at most.)
+constexpr int kPlaces = 3;
+
+// A workgroup of GN x GT waves has GN * WN row tiles of W and GT * WT of X.  A step's codes lie in one of kPlaces places in shared memory,
+// loaded kPlaces - 1 steps ahead; the scales of the next four steps are loaded beside them, a quarter a step, into one of two places.
 //
 // Bound by the matrix cores, at the clock that their power leaves: 8192 x 14336 x 4096 in 632 us in e4m3 (1.52 PFLOP/s; the matrix cores
 // busy 66% of the time, conversions 46% of the issue slots) and 267 us in e2m1 (3.6 PFLOP/s, of which storing Y is some 55 us).  256 x
 // 256 tiles of eight waves, 128 x 64 each (a step reads 12 operands for 32 products); two or three places measured the same, loads by way
 // of registers and one step ahead 758 us.
-template <int FMT, int WN, int WT, int GN, int GT, int NS>
+template <int FMT, int WN, int WT, int GN, int GT>
 __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) {
   using S = TileShape<FMT, WN, WT, GN, GT>;
-  static_assert(NS >= 2 && NS <= 4, "scales are read before the next but one's loads");
   extern __shared__ f32x4 shared[];
   uint8_t* const lds = reinterpret_cast<uint8_t*>(shared);
-  uint8_t* const lds_scales = lds + NS * S::kStage;
+  uint8_t* const lds_scales = lds + kPlaces * S::kStage;
   const unsigned place0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave % GN, wt = wave / GN;
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) 
     }
   // the loads of a step, and a quarter of the next piece's scales; steps and pieces past the end are the last one again
   auto fetch_scales = [&](int q, int sp) {
-    const unsigned at = place0 + NS * S::kStage + (sp & 1) * S::kScales;
+    const unsigned at = place0 + kPlaces * S::kStage + (sp & 1) * S::kScales;
     const int64_t offset = static_cast<int64_t>(sp < supers ? sp : supers - 1) * 256;
 #pragma unroll
     for (int l = 0; l < S::kScaleLoads; ++l)
@@ -550,7 +552,7 @@ __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) 
 #pragma unroll
   for (int q = 0; q < 4; ++q) fetch_scales(q, 0);
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s) {
+  for (int s = 0; s < kPlaces - 1; ++s) {
     fetch(s, s);
     fetch_scales(s, 1);
   }
@@ -560,7 +562,7 @@ __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) 
     constexpr int STEP = decltype(step_in)::value;
     const int step = sp * 4 + STEP;
     if (step > last) return;
-    dma_wait<(NS - 2) * (S::kLoads + S::kScaleLoads)>();
+    dma_wait<(kPlaces - 2) * (S::kLoads + S::kScaleLoads)>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");  // (no read of shared memory moves up)
     if constexpr (STEP == 0) {
@@ -580,12 +582,12 @@ __global__ __launch_bounds__(GN* GT * 64) void mx_tile_kernel(const GemmArgs a) 
 #pragma unroll
       for (int h = 0; h < S::kParts; ++h) x[j].q[h] = held[(S::kW + (wt * WT + j) * S::kParts + h) * 64];
     // the next loads, while the reads are on their way: every wave is done with the place of the step before
-    const int free_slot = slot == 0 ? NS - 1 : slot - 1;
-    constexpr int AHEAD = STEP + NS - 1;
-    fetch(step + NS - 1, free_slot);
+    const int free_slot = slot == 0 ? kPlaces - 1 : slot - 1;
+    constexpr int AHEAD = STEP + kPlaces - 1;
+    fetch(step + kPlaces - 1, free_slot);
     fetch_scales(AHEAD & 3, sp + AHEAD / 4 + 1);
     mma_step<FMT, STEP>(acc, w, ws, x, xs);
-    slot = slot == NS - 1 ? 0 : slot + 1;
+    slot = slot == kPlaces - 1 ? 0 : slot + 1;
   };
   for (int sp = 0; sp < supers; ++sp) {
     one(std::integral_constant<int, 0>(), sp);
@@ -624,13 +626,13 @@ hipError_t launch_stream(const GemmArgs& a, hipStream_t stream) {
   return e != hipSuccess ? e : run(kern, grid, waves * 64, lds, stream, a);
 }
 
-template <int FMT, int WN, int WT, int GN, int GT, int NS>
+template <int FMT, int WN, int WT, int GN, int GT>
 hipError_t launch_tile(const GemmArgs& a, hipStream_t stream) {
   using S = TileShape<FMT, WN, WT, GN, GT>;
   static std::atomic<unsigned> limit[kMaxDevices];
   const dim3 grid(static_cast<unsigned>((mx_tiles(a.n) + S::kW - 1) / S::kW), static_cast<unsigned>((mx_tiles(a.t) + S::kX - 1) / S::kX));
-  const size_t lds = NS * S::kStage + 2 * S::kScales;
-  const auto kern = mx_tile_kernel<FMT, WN, WT, GN, GT, NS>;
+  const size_t lds = kPlaces * S::kStage + 2 * S::kScales;
+  const auto kern = mx_tile_kernel<FMT, WN, WT, GN, GT>;
   const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds, limit);
   return e != hipSuccess ? e : run(kern, grid, GN * GT * 64, lds, stream, a);
 }
@@ -660,8 +662,8 @@ hipError_t launch_format(const MxGemmCall& c, const GemmArgs& a, hipStream_t str
     return floats ? launch_step<FMT, true, 4, 2>(a, stream) : launch_step<FMT, false, 4, 2>(a, stream);
   }
   if (p.kernel == MX_TILE) {
-    if (p.row_tiles == 16) return launch_tile<FMT, 8, 4, 2, 4, 3>(a, stream);
-    return launch_tile<FMT, 4, 4, 2, 2, 3>(a, stream);
+    if (p.row_tiles == 16) return launch_tile<FMT, 8, 4, 2, 4>(a, stream);
+    return launch_tile<FMT, 4, 4, 2, 2>(a, stream);
   }
   if (p.col_tiles == 2) {
     if (p.row_tiles == 4) return launch_stream<FMT, -1, 4, 2, 8>(a, stream);
