@@ -209,7 +209,7 @@ __device__ __forceinline__ void quantize_rows(const GemmArgs& a, int sp, bool in
 // wave its own pieces, eight elements a lane, through shared memory into the operands' order.
 //
 // Bound by W's bytes where there are many: 128256 x 4096, one bf16 row to e4m3, in 44.7 us (6.3 TB/s; with W's loads through the
-// caches 48.9, quantizing X again for every row tile 182), 28672 x 4096, five rows to e2m1, in 12.0 us.  Small products are a chain of
+// caches 48.9, quantizing X again for every row tile 182), 28672 x 4096, five rows to e2m1, in 13.0 us cold.  Small products are a chain of
 // latencies: 6912 x 2560 and one f32 row in 6.0 us in a graph, of which reading 9.4 MB is 1.4.  X as bf16 operands in registers costs
 // e4m3 64 conversions a piece of W and none of X; from 16 pieces on (K above 8192) a wave holds four pieces, as codes.  D = 2: one
 // piece on its way beside the one in use; with three the registers of P = 1 (128 for 16 waves) spill.
@@ -333,9 +333,10 @@ __global__ __launch_bounds__(P == 1 ? 1024 : 512) void mx_step_kernel(const Gemm
 // K in turn and join in shared memory, in the waves' order.  SRC: the type of the rows that are quantized on the way (each wave
 // its own pieces; rows of more than 16384 elements, which mx_step_kernel cannot hold), -1: X is quantized already.
 //
-// For batches, whose tiles are too few for the device unless a tile is small and K is shared out inside the workgroup.  Bound by the
-// caches (each operand is read by N / (16 RT) or T / (16 CT) workgroups) and, in e4m3, by conversions: 64 x 4096 x 14336 in 15.7 us
-// with cold weights, in e2m1 11.8; 100 x 4096 x 4096 in 8.4 us.  (K shared out over workgroups, tiles of 128 x 64 through shared
+// For batches, whose tiles are too few for the device unless a tile is small and K is shared out inside the workgroup.  Bound by
+// latency: 64 x 4096 x 14336 takes 15.9 us with cold weights, in e2m1 11.8, at one wave a SIMD, of whose time the vector instructions are
+// 25% and the matrix cores 16%; 100 x 4096 x 4096 8.3 us.  Through wide weights the caches count too (each operand is read by N / (16 RT) or
+// T / (16 CT) workgroups): 32 x 131072 x 4096 in 71 us, in e2m1 59 (4.1 and 5.0 TB/s).  (K shared out over workgroups, tiles of 128 x 64 through shared
 // memory and the sums joined by a second launch: 19.0 and 14.4 us; two pieces of a wave's on their way: 18.4 and 12.6 us.)
 template <int FMT, int SRC, int RT, int CT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const GemmArgs a) {

@@ -9,6 +9,9 @@
 // lie 256 bytes apart, so 16 bytes are used of each line that is fetched), one row of 4096 is quantized in 2.9 us and read in 2.3.
 // Short rows share a wave or a workgroup: a million rows of 32 (f32 to e4m3) are quantized in 41 us (a workgroup a row tile 69), gated
 // in 73, looked up in 18 (80).
+//
+// Plain planes of 28672 x 8192 become rows in 67 us (e2m1; 113 in e4m3), ggml's blocks in 81, and rows plain planes in 142 (199); copying the codes
+// alone takes 45 (88).  An instruction of a wave has only 16 bytes (32) of each of 16 rows on the plain side; a weight goes this way once.
 #include <hip/hip_ext.h>
 
 #include <type_traits>
@@ -55,7 +58,9 @@ __device__ __forceinline__ unsigned most4(unsigned most) {
 
 // A quad of lanes' block of gated products: scale and codes.  They come from f32 products where all that these may stand for, 2^-19 to
 // either side, give the same ones (scale and rounding are monotonous), and from 64 bits otherwise: with e4m3 one block in a thousand
-// (2^-15 an element).  Blocks of products below 2^-60, with values that are no numbers, or with gates below -80 take 64 bits too.
+// (2^-15 an element).  Blocks of products below 2^-60, with values that are no numbers, or with gates below -80 take 64 bits too, and so do
+// blocks with a product of -0, whose two ends have different signs: with squared ReLU nearly every block (g <= 0 beside u < 0).  That
+// costs nothing that shows: 8192 x 4096 to e4m3 take 42 us with either activation.
 template <int FMT, int ACT>
 __device__ __forceinline__ void gate8(const float (&g)[8], const float (&u)[8], unsigned& s, unsigned (&c)[FMT == MX_E2M1 ? 1 : 2]) {
   float low[8], high[8], largest = 0.f, least = 0.f, zero = 0.f;
